@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "dtn_common.cuh"
+#include "paged.cuh"
 
 namespace dtn {
 
@@ -35,6 +36,21 @@ int* device_status_word() {
     g_status_words[dev] = p;
   }
   return g_status_words[dev];
+}
+
+int* device_status_word_unless_capturing(cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  {
+    std::lock_guard<std::mutex> lock(g_status_mutex);
+    if (g_status_words[dev]) return g_status_words[dev];
+  }
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();   // a query of the legacy stream during a capture on another one is an error of its own; there is none to report here
+    return nullptr;
+  }
+  return device_status_word();
 }
 
 int sm_count() {

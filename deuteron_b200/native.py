@@ -16,7 +16,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_WORKSPACE, ERR_UNSUPPORTED, ERR_DEVICE = range(6)
 GEMM_MODES = {'f32': 0, 'tf32x3': 1, 'bf16x3': 2, 'f32_splitk': 3}
 REDUCE_OPS = {'sum': 0, 'max': 1, 'sumsq': 2, 'softmax': 3}
 ROW_INPUT_KINDS = {'scalar': 0, 'columns': 1, 'immediate': 2}
-STORAGE = {'f32': 0, 'f16': 1}
+STORAGE = {'f32': 0, 'f16': 1, 'bf16': 2}
 ELEMENTWISE_OPS = {
     'add': 0, 'subtract': 1, 'multiply': 2, 'divide': 3, 'maximum': 4, 'minimum': 5, 'relu': 6, 'exp': 7,
     'sqrt': 8, 'rsqrt': 9, 'reciprocal': 10, 'negative': 11, 'absolute': 12, 'copy': 13, 'exp_fast': 7,
@@ -30,6 +30,10 @@ class CudaError(RuntimeError):
 
 class DeviceWaitError(RuntimeError):
     """A kernel's bounded wait ran out and the kernel returned early with a status code."""
+
+
+class PageError(IndexError):
+    """A kernel met a page number, position, row or length that a paged cache's pool or tables do not cover."""
 
 
 _I64, _P, _F, _I = ct.c_int64, ct.c_void_p, ct.c_float, ct.c_int
@@ -62,6 +66,12 @@ _SIGNATURES = {
     'dtn_attention_f32': [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _F, _P],
     'dtn_gqa_fwd': [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _I64, _I64, _P],
     'dtn_gqa_set_variant': [_I],
+    'dtn_rotary': [_P, _P, _P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _F, _I, _P],
+    'dtn_paged_append': [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                         _I64, _P, _I64, _I, _F, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P],
+    'dtn_paged_attention': [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                            _I64, _I64, _F, _I64, _I, _I, _P],
+    'dtn_copy_pages': [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P],
 }
 
 _lock = threading.Lock()
@@ -140,6 +150,9 @@ def row_fused(params: dict, x_pointer: int, input_pointers: list[int | None], ou
          out_pointer, ldo, stream)
 
 
+_PAGED_ROLES = {0x61: 'paged attention', 0x62: 'paged append', 0x63: 'copy of pages'}
+
+
 def device_status(stream: int = 0) -> int:
     """Synchronises `stream` and returns (and clears) the device status word; 0 means clean."""
     value = ct.c_int(0)
@@ -149,6 +162,8 @@ def device_status(stream: int = 0) -> int:
 
 def raise_on_device_status(stream: int = 0) -> None:
     status = device_status(stream)
+    if status >> 8 in _PAGED_ROLES:
+        raise PageError(f'{_PAGED_ROLES[status >> 8]}: a page number, position, row or length outside the pool or the tables (status {status:#x})')
     if status:
         role = {0x71: 'bounded-wait self-test', 0x11: 'attention K loader', 0x12: 'attention V loader', 0x13: 'attention Q loader', 0x31: 'attention softmax (scores)', 0x32: 'attention output', 0x33: 'attention softmax (row exchange)', 0x21: 'attention MMA issuer (queries)', 0x23: 'attention MMA issuer (values)', 0x24: 'attention MMA issuer (probabilities)', 0x25: 'attention MMA issuer (keys)', 0x26: 'attention MMA issuer (probabilities)', 0x51: 'fused-split GEMM producers', 0x52: 'fused-split GEMM MMA issuer', 0x53: 'fused-split GEMM epilogue', 5: 'TMA producer (split of A)', 1: 'TMA producer', 2: 'MMA issuer (accumulator)', 3: 'MMA issuer (operands)', 4: 'epilogue'}.get(status >> 8, 'kernel')
         raise DeviceWaitError(f'bounded wait ran out in the {role}, CTA {status & 0xff} (status {status:#x})')

@@ -6,6 +6,7 @@ libdeuteron_b200.so on the current torch stream. Tensors must live on the curren
 from __future__ import annotations
 
 import ctypes as ct
+import math
 
 import torch
 
@@ -336,6 +337,304 @@ def gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: floa
 
 def set_gqa_variant(variant: int) -> None:
     native.call('dtn_gqa_set_variant', variant)
+
+
+# ------------------------------------------------------------------------------------------------
+# rotary positions and the paged key-value cache
+# ------------------------------------------------------------------------------------------------
+
+_STORAGE_OF = {torch.float32: native.STORAGE['f32'], torch.float16: native.STORAGE['f16'], torch.bfloat16: native.STORAGE['bf16']}
+_LAYOUTS = {'half': 0, 'interleaved': 1}
+
+
+def _on_current_device(**tensors: torch.Tensor) -> None:
+    current = None
+    for label, tensor in tensors.items():
+        device = tensor.get_device()
+        if device < 0:
+            raise ValueError(f'deuteron_b200 operators take CUDA tensors: {label} is on {tensor.device}')
+        if current is None:
+            current = torch.cuda.current_device()
+        if device != current:
+            raise ValueError(f'{label} is on {tensor.device}, the current device is cuda:{current}')
+
+
+def _tensors(*tensors: torch.Tensor) -> None:
+    for tensor in tensors:
+        if not isinstance(tensor, torch.Tensor):
+            raise ValueError(f'a tensor is needed, got {type(tensor).__name__}')
+
+
+def _heads(tensor: torch.Tensor, label: str, written: bool = False) -> tuple[int, int]:
+    """Token and head strides of a [tokens, heads, dim] tensor with dense heads (0 for an extent of one)."""
+    if tensor.dim() != 3:
+        raise ValueError(f'{label} must be a [tokens, heads, dim] tensor')
+    tokens, heads, dim = tensor.shape
+    token_stride, head_stride, unit = tensor.stride()
+    if dim > 1 and unit != 1:
+        raise ValueError(f'{label} must have dense heads (unit stride in its last dimension)')
+    token_stride, head_stride = token_stride if tokens > 1 else 0, head_stride if heads > 1 else 0
+    if written and ((tokens > 1 and token_stride == 0) or (heads > 1 and head_stride == 0)):
+        raise ValueError(f'{label} must not be an expanded tensor: it is written')
+    return token_stride, head_stride
+
+
+def _index(tensor: torch.Tensor, label: str, count: int | None = None, wide: bool = False) -> None:
+    if not isinstance(tensor, torch.Tensor) or tensor.dim() != 1 or not tensor.is_contiguous():
+        raise ValueError(f'{label} must be a contiguous 1-D tensor')
+    if tensor.dtype != torch.int32 and not (wide and tensor.dtype == torch.int64):
+        raise ValueError(f'{label} must have dtype {"int32 or int64" if wide else "int32"}, got {tensor.dtype}')
+    if count is not None and tensor.shape[0] != count:
+        raise ValueError(f'{label} must have {count} entries, got {tensor.shape[0]}')
+
+
+def _rotation(frequencies: torch.Tensor | None, layout: str, dim: int) -> int:
+    """Number of rotated pairs; checks frequencies and layout."""
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    if frequencies is None:
+        return 0
+    if not isinstance(frequencies, torch.Tensor) or frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+        raise ValueError('frequencies must be a contiguous 1-D float64 tensor (radians per position)')
+    pairs = frequencies.shape[0]
+    if 2 * pairs > dim:
+        raise ValueError(f'{pairs} frequencies rotate {2 * pairs} elements, a head has {dim}')
+    return pairs
+
+
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor) -> tuple[int, int]:
+    """Page and head strides that both pools share; checks pools and tables."""
+    for label, pool in (('k_pages', k_pages), ('v_pages', v_pages)):
+        if pool.dim() != 4:
+            raise ValueError(f'{label} must be a [pages, kv_heads, page_size, dim] tensor')
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError('k_pages and v_pages must have one shape and dtype')
+    pages, heads, size, dim = k_pages.shape
+    if size < 1:
+        raise ValueError('a page holds at least one token')
+    strides = []
+    for label, pool in (('k_pages', k_pages), ('v_pages', v_pages)):
+        page, head, token, unit = pool.stride()
+        if (dim > 1 and unit != 1) or (size > 1 and token != dim):
+            raise ValueError(f'the rows of one page and head must be dense in {label}')
+        strides.append((page if pages > 1 else 0, head if heads > 1 else 0))
+    if strides[0] != strides[1]:
+        raise ValueError('k_pages and v_pages must have the same strides')
+    if tables.dtype != torch.int32 or tables.dim() != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise ValueError('tables must be a [sequences, pages per sequence] int32 tensor with unit column stride')
+    return strides[0]
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int | None = None, fast: float = 32.0, slow: float = 1.0,
+                       device: torch.device | str | None = None) -> tuple[torch.Tensor, float]:
+    """Frequencies (float64, radians per position, one per pair of `rotary_dim` elements) and amplitude for `rotary`.
+
+    w_i = base^(-2i / rotary_dim). `scaling` stretches them for contexts `factor` times longer than trained: 'linear'
+    divides every frequency by the factor; 'ntk' raises the base by factor^(rotary_dim / (rotary_dim - 2)), which leaves the
+    first pair alone and divides the last by the factor; 'yarn' (Peng et al., 2023) divides those that turn fewer than `slow`
+    times within `original_length`, keeps those that turn more than `fast` times, blends in between by the number of
+    turns, and returns the amplitude 0.1 ln(factor) + 1. `device` defaults to the current CUDA device.
+    """
+    if type(rotary_dim) is not int or rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError(f'rotary_dim must be an even non-negative integer, got {rotary_dim!r}')
+    if not (base > 0 and factor > 0) or base == float('inf') or factor == float('inf'):
+        raise ValueError('base and factor must be positive and finite')
+    if scaling not in (None, 'linear', 'ntk', 'yarn'):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if scaling is None and factor != 1.0:
+        raise ValueError('a factor needs a scaling')
+    amplitude = 1.0
+    if scaling == 'ntk':
+        if rotary_dim == 2:
+            raise ValueError("'ntk' needs more than one pair")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2)) if rotary_dim else base
+    frequencies = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if scaling == 'linear':
+        frequencies = [w / factor for w in frequencies]
+    if scaling == 'yarn':
+        if not original_length or original_length < 1 or not 0 <= slow < fast:
+            raise ValueError("'yarn' needs the original_length of training and 0 <= slow < fast")
+        kept = [min(max((original_length * w / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for w in frequencies]
+        frequencies = [w * keep + w / factor * (1.0 - keep) for w, keep in zip(frequencies, kept)]
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return torch.tensor(frequencies, dtype=torch.float64, device='cuda' if device is None else device), amplitude
+
+
+def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> torch.Tensor:
+    _tensors(x, positions, frequencies)
+    if x.dtype not in _STORAGE_OF:
+        raise ValueError(f'x must have dtype float32, float16 or bfloat16, got {x.dtype}')
+    token_stride, head_stride = _heads(x, 'x')
+    tokens, heads, dim = x.shape
+    _index(positions, 'positions', tokens, wide=True)
+    pairs = _rotation(frequencies, layout, dim)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    _tensors(out)
+    if out.dtype != x.dtype or out.shape != x.shape:
+        raise ValueError('out must have the shape and dtype of x')
+    out_token_stride, out_head_stride = _heads(out, 'out', written=True)
+    if out.data_ptr() == x.data_ptr() and (out_token_stride, out_head_stride) != (token_stride, head_stride):
+        raise ValueError('out must be x itself or lie elsewhere')
+    _on_current_device(x=x, positions=positions, frequencies=frequencies, out=out)
+    native.call('dtn_rotary', x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(),
+                tokens, heads, dim, pairs, token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose,
+                amplitude, _STORAGE_OF[x.dtype], _stream())
+    return out
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = 'half', amplitude: float = 1.0,
+           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: turns pair i of every head of token t by positions[t] * frequencies[i] and scales it by `amplitude`.
+
+    x: [tokens, heads, dim], float32 / float16 / bfloat16, any token and head strides, dense heads (a slice of a fused
+    projection); positions: int32 or int64 [tokens]; frequencies: float64 [pairs] from `rotary_frequencies`. Pair i is
+    (i, i + pairs) in the 'half' layout, (2i, 2i + 1) in the 'interleaved' one; elements from 2 * pairs on are copied. The
+    angle is formed in 64 bits, the result rounded once. `out` may be x itself; otherwise it must not overlap x.
+    """
+    return _rotary(x, positions, frequencies, layout, amplitude, out, 0)
+
+
+def rotary_backward(grad: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = 'half', amplitude: float = 1.0,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of `rotary`'s x from the gradient of its result: the transposed map (each pair turned back, times `amplitude`).
+    Same arguments; positions and frequencies have no gradient."""
+    return _rotary(grad, positions, frequencies, layout, amplitude, out, 1)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, rows: torch.Tensor,
+                 positions: torch.Tensor, frequencies: torch.Tensor | None = None, layout: str = 'half', amplitude: float = 1.0,
+                 q: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes the keys and values of new tokens into the pages of a cache; rotates keys and queries on the way. One launch.
+
+    k, v: [tokens, kv_heads, dim]; k_pages, v_pages: [pages, kv_heads, page_size, dim] with equal strides; tables: int32
+    [sequences, pages per sequence]. Token t is position positions[t] (int32 or int64) of sequence rows[t] (int32; negative:
+    padding, nothing is stored), which lies in page tables[rows[t], positions[t] // page_size] at place
+    positions[t] % page_size. With `frequencies` the keys are rotated as `rotary` does, and so is `q` [tokens, q_heads, dim],
+    which is returned (in `q_out`, which may be q itself, or a new tensor); values are stored as they are. A row, position or
+    page number outside the tables or the pool stores nothing and makes `check_device_status` raise PageError. No two
+    tokens of a call may have the same place.
+    """
+    _tensors(k, v, k_pages, v_pages, tables, rows, positions)
+    if k.dtype not in _STORAGE_OF or v.dtype != k.dtype or k_pages.dtype != k.dtype:
+        raise ValueError('k, v and the pools must share dtype float32, float16 or bfloat16')
+    (k_token, k_head), (v_token, v_head) = _heads(k, 'k'), _heads(v, 'v')
+    page_stride, page_head_stride = _pools(k_pages, v_pages, tables)
+    tokens, kv_heads, dim = k.shape
+    pages, pool_heads, page_size, pool_dim = k_pages.shape
+    if v.shape != k.shape or pool_heads != kv_heads or pool_dim != dim:
+        raise ValueError('k, v and the pools disagree in shape')
+    if (pages > 1 and page_stride == 0) or (kv_heads > 1 and page_head_stride == 0):
+        raise ValueError('the pools must not be expanded tensors: they are written')
+    _index(rows, 'rows', tokens)
+    _index(positions, 'positions', tokens, wide=True)
+    pairs = _rotation(frequencies, layout, dim)
+    q_heads = q_token = q_head = q_out_token = q_out_head = 0
+    if q is None and q_out is not None:
+        raise ValueError('q_out without q')
+    if q is not None:
+        _tensors(q)
+        q_token, q_head = _heads(q, 'q')
+        q_heads = q.shape[1]
+        if q.dtype != k.dtype or q.shape[0] != tokens or q.shape[2] != dim:
+            raise ValueError('q must be a [tokens, q_heads, dim] tensor of the dtype of k')
+        if q_out is None:
+            q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+        _tensors(q_out)
+        if q_out.dtype != q.dtype or q_out.shape != q.shape:
+            raise ValueError('q_out must have the shape and dtype of q')
+        q_out_token, q_out_head = _heads(q_out, 'q_out', written=True)
+        if q_out.data_ptr() == q.data_ptr() and (q_out_token, q_out_head) != (q_token, q_head):
+            raise ValueError('q_out must be q itself or lie elsewhere')
+        _on_current_device(q=q, q_out=q_out)
+    _on_current_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, tables=tables, rows=rows, positions=positions,
+                       frequencies=k if frequencies is None else frequencies)
+    native.call('dtn_paged_append', k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(),
+                positions.data_ptr(), positions.dtype == torch.int64, tokens, kv_heads, dim, k_token, k_head, v_token, v_head, pages, page_size,
+                page_stride, page_head_stride, tables.shape[0], tables.shape[1], tables.stride(0) if tables.shape[0] > 1 else 0,
+                frequencies.data_ptr() if pairs else None, pairs, _LAYOUTS[layout], amplitude, q.data_ptr() if q_heads else None,
+                q_out.data_ptr() if q_heads else None, q_heads, q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, scale: float,
+                    rows: torch.Tensor | None = None, window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged key-value cache: q[n, q_heads, dim] -> out[n, q_heads, dim].
+
+    Pools and tables as in `paged_append`; lengths: int32 [sequences], the tokens of each that are seen (the new one among
+    them). rows: int32 [n], the sequence of each query (None: query i is sequence i); a negative row (padding of a captured
+    batch) and a length of zero give zeros. window > 0 keeps the last `window` tokens only. Query head h reads kv head
+    h // (q_heads // kv_heads). Storage float32 / float16 / bfloat16, softmax and sums in FP32; `out` is float32 by default, as
+    `gqa_attention` returns it, or a given tensor of float32 or of q's dtype. The values in a page behind a sequence's end do
+    not matter, NaN included. A row or length outside the tables, or a page number outside the pool, makes
+    `check_device_status` raise PageError; a sequence with such a page gets NaN.
+    """
+    _tensors(q, k_pages, v_pages, tables, lengths)
+    if q.dtype not in _STORAGE_OF or k_pages.dtype != q.dtype:
+        raise ValueError('q and the pools must share dtype float32, float16 or bfloat16')
+    q_token, q_head = _heads(q, 'q')
+    page_stride, page_head_stride = _pools(k_pages, v_pages, tables)
+    count, q_heads, dim = q.shape
+    pages, kv_heads, page_size, pool_dim = k_pages.shape
+    if pool_dim != dim:
+        raise ValueError('q and the pools disagree in the head size')
+    if kv_heads == 0 or q_heads % kv_heads:
+        raise ValueError('query heads must be a multiple of kv heads')
+    _index(lengths, 'lengths', tables.shape[0])
+    if rows is not None:
+        _tensors(rows)
+        _index(rows, 'rows', count)
+    elif count > tables.shape[0]:
+        raise ValueError(f'{count} queries but {tables.shape[0]} sequences')
+    if window < 0:
+        raise ValueError('window must not be negative')
+    if out is None:
+        out = torch.empty((count, q_heads, dim), dtype=torch.float32, device=q.device)
+    _tensors(out)
+    if out.shape != q.shape or out.dtype not in (torch.float32, q.dtype):
+        raise ValueError('out must have the shape of q and dtype float32 or that of q')
+    out_token, out_head = _heads(out, 'out', written=True)
+    _on_current_device(q=q, k_pages=k_pages, v_pages=v_pages, tables=tables, lengths=lengths, rows=lengths if rows is None else rows, out=out)
+    native.call('dtn_paged_attention', q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+                None if rows is None else rows.data_ptr(), out.data_ptr(), count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head,
+                pages, page_size, page_stride, page_head_stride, tables.shape[0], tables.shape[1],
+                tables.stride(0) if tables.shape[0] > 1 else 0, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, _stream())
+    return out
+
+
+def copy_pages(pages: torch.Tensor, sources: torch.Tensor, destinations: torch.Tensor) -> None:
+    """Copies page sources[i] onto page destinations[i] for every i, in one launch.
+
+    pages: [pages, kv_heads, page_size, dim] with dense pages, or with one or two leading dimensions (layers; keys and
+    values), in each of which the same pages are copied. sources, destinations: int32 [n]. No destination may occur twice or
+    be a source. A page number outside the pool copies nothing and makes `check_device_status` raise PageError.
+    """
+    _tensors(pages, sources, destinations)
+    if not 4 <= pages.dim() <= 6:
+        raise ValueError('pages must be a [pages, kv_heads, page_size, dim] tensor, or one with one or two leading dimensions')
+    heads, size, dim = pages.shape[-3:]
+    dense = 1
+    for extent, stride in zip((dim, size, heads), reversed(pages.stride()[-3:])):
+        if extent > 1 and stride != dense:
+            raise ValueError('the values of one page must be dense')
+        dense *= extent
+    planes, plane_stride = 1, 0
+    for extent, stride in zip(reversed(pages.shape[:-4]), reversed(pages.stride()[:-4])):
+        if planes > 1 and extent > 1 and stride != planes * plane_stride:
+            raise ValueError('the leading dimensions of pages must be evenly spaced')
+        plane_stride = plane_stride if planes > 1 or extent <= 1 else stride
+        planes *= extent
+    count = pages.shape[-4]
+    page_stride = pages.stride(-4) if count > 1 else 0
+    if dense and ((count > 1 and page_stride < dense) or (planes > 1 and plane_stride == 0)):
+        raise ValueError('pages must not be an expanded tensor: it is written')
+    _index(sources, 'sources')
+    _index(destinations, 'destinations', sources.shape[0])
+    _on_current_device(pages=pages, sources=sources, destinations=destinations)
+    unit = pages.element_size()
+    native.call('dtn_copy_pages', pages.data_ptr(), planes, plane_stride * unit, count, page_stride * unit, dense * unit, sources.data_ptr(),
+                destinations.data_ptr(), sources.shape[0], _stream())
 
 
 def check_device_status() -> None:

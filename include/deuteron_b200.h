@@ -57,6 +57,7 @@ extern "C" {
 /* storage type of attention operands */
 #define DTN_STORAGE_F32 0
 #define DTN_STORAGE_F16 1
+#define DTN_STORAGE_BF16 2 /* dtn_rotary, dtn_paged_append and dtn_paged_attention only */
 
 /* binary / unary elementwise operators (compiler/codegen/lower.py:258-291) */
 #define DTN_EW_ADD 0
@@ -323,6 +324,49 @@ int dtn_gqa_fwd(const void* q, const void* k, const void* v, float* out, int64_t
  * are per head). Variants 3 and 7 give the same bits.
  * No reference counterpart. */
 int dtn_gqa_set_variant(int variant);
+
+/* Rotary positions: out[t, h] = x[t, h] with pair i of its first 2 * pairs elements turned by the angle
+ * positions[t] * frequencies[i] and scaled by `amplitude`; the other elements are copied. Pair i is (i, i + pairs), or
+ * (2 i, 2 i + 1) when `interleaved` is non-zero. A non-zero `transpose` turns the other way: the gradient of x from that of
+ * out. x and out are [tokens, heads, dim] of `storage` with the given strides in elements and dense heads (out may be x
+ * itself, with the same strides); positions are int32, or int64 when `positions_64` is non-zero; frequencies are FP64 radians
+ * per position. The angle is formed and reduced in FP64, the rotation computed in FP32 and rounded once. dim <= 1024. Any
+ * alignment of whole elements; 16-byte aligned heads are moved faster. No reference counterpart. */
+int dtn_rotary(const void* x, void* out, const void* positions, int positions_64, const double* frequencies, int64_t tokens, int64_t heads,
+               int64_t dim, int64_t pairs, int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride,
+               int64_t out_head_stride, int interleaved, int transpose, float amplitude, int storage, void* stream);
+
+/* Appends tokens to a paged key-value cache, with the rotation of dtn_rotary on the way (pairs = 0: none).
+ * Pools: k_pages and v_pages are [pages, kv_heads, page_size, dim] of `storage` with the same page_stride and
+ * page_head_stride (elements); the page_size x dim values of one page and head are dense. Position p of sequence r lies in
+ * page tables[r * table_stride + p / page_size] at place p % page_size. Token t is stored at positions[t] of sequence rows[t];
+ * a negative row stores nothing (padding). k and v are [tokens, kv_heads, dim]; q (q_heads of them, 0 for none) is rotated by
+ * the same positions into q_out, which may be q itself. A row >= sequences, a position outside the tables or a page number
+ * outside the pool stores nothing and is reported by dtn_device_status. Two tokens for one place: either may stay. */
+int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int* tables, const int* rows, const void* positions,
+                     int positions_64, int64_t tokens, int64_t kv_heads, int64_t dim, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, int64_t pages, int64_t page_size, int64_t page_stride,
+                     int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence, int64_t table_stride, const double* frequencies,
+                     int64_t pairs, int interleaved, float amplitude, const void* q, void* q_out, int64_t q_heads, int64_t q_token_stride,
+                     int64_t q_head_stride, int64_t q_out_token_stride, int64_t q_out_head_stride, int storage, void* stream);
+
+/* Attention of one new token per sequence over a paged cache (pools and tables as above):
+ * out[i, h] = sum over t of softmax_t(scale * q[i, h] . k[t]) v[t], t over the last `window` (0: all) of the first lengths[r]
+ * tokens of sequence r = rows[i] (rows NULL: r = i). Query head h reads kv head h / (q_heads / kv_heads). A negative row or a
+ * length of zero gives zeros. out is FP32, or of `storage` when out_f32 is zero. A row >= sequences or a length beyond the tables is
+ * reported by dtn_device_status (the length is cut), and so is a page number outside the pool, which makes the sequence's
+ * output NaN; nothing outside the pools is read. What lies in the pools behind a sequence's end is not used, whatever it holds. */
+int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
+                        void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
+                        int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
+                        int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
+                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* stream);
+
+/* Copies page sources[i] onto page destinations[i] in each of `planes` planes of a pool (a layer's keys or values each),
+ * i < pairs. Strides and page_bytes in bytes; a page's bytes are dense. No destination may be a source or occur twice. A
+ * page number outside [0, pages) copies nothing for its pair and is reported by dtn_device_status. */
+int dtn_copy_pages(void* pool, int64_t planes, int64_t plane_stride_bytes, int64_t pages, int64_t page_stride_bytes, int64_t page_bytes,
+                   const int* sources, const int* destinations, int64_t pairs, void* stream);
 
 #ifdef __cplusplus
 }

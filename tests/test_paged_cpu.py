@@ -1,0 +1,143 @@
+"""Refusals and host-side parts of the rotary and paged-cache operators; no GPU."""
+import math
+
+import pytest
+import torch
+
+from deuteron_b200 import native, ops
+
+
+def cache(dtype=torch.float16, pages=4, heads=2, size=8, dim=16):
+    pool = torch.zeros(2, pages, heads, size, dim, dtype=dtype)
+    return pool[0], pool[1], torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+
+
+def test_frequencies_follow_their_formulas():
+    w, amplitude = ops.rotary_frequencies(64, device='cpu')
+    assert w.dtype == torch.float64 and amplitude == 1.0
+    assert torch.allclose(w, torch.tensor([10000.0 ** (-i / 32) for i in range(32)], dtype=torch.float64), rtol=1e-15)
+    linear, amplitude = ops.rotary_frequencies(64, scaling='linear', factor=4.0, device='cpu')
+    assert torch.equal(linear, w / 4) and amplitude == 1.0
+    stretched, _ = ops.rotary_frequencies(64, scaling='ntk', factor=4.0, device='cpu')
+    assert stretched[0] == 1.0 and math.isclose(stretched[-1], w[-1] / 4, rel_tol=1e-12) and bool((stretched[1:] < w[1:]).all())
+    yarn, amplitude = ops.rotary_frequencies(64, scaling='yarn', factor=8.0, original_length=4096, device='cpu')
+    turns = 4096 * w / (2 * math.pi)
+    assert torch.equal(yarn[turns >= 32], w[turns >= 32]) and torch.equal(yarn[turns <= 1], w[turns <= 1] / 8)
+    between = (turns > 1) & (turns < 32)
+    assert bool(between.any()) and bool(((yarn < w) & (yarn > w / 8))[between].all())
+    assert math.isclose(amplitude, 0.1 * math.log(8) + 1)
+    assert ops.rotary_frequencies(64, scaling='yarn', factor=1.0, original_length=4096, device='cpu')[1] == 1.0
+    assert ops.rotary_frequencies(0, device='cpu')[0].shape == (0,)
+    for arguments in (dict(rotary_dim=7), dict(rotary_dim=-2), dict(rotary_dim=8.0), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, base=math.inf),
+                      dict(rotary_dim=8, factor=2.0), dict(rotary_dim=8, scaling='cubic'), dict(rotary_dim=8, scaling='yarn', factor=2.0),
+                      dict(rotary_dim=2, scaling='ntk', factor=2.0), dict(rotary_dim=8, scaling='linear', factor=0.0), dict(rotary_dim=8, scaling='linear', factor=math.nan),
+                      dict(rotary_dim=8, scaling='yarn', factor=2.0, original_length=10, fast=1.0, slow=1.0)):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(**arguments, device='cpu')
+
+
+def test_rotary_refuses():
+    x, at, w = torch.zeros(3, 2, 16), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.float64)
+    for arguments, message in (
+            ((x.int(), at, w), 'dtype'), ((x.double(), at, w), 'dtype'), ((x[0], at, w), 'heads'), ((x.transpose(1, 2), at, w), 'dense'), ((x, at[:2], w), 'entries'),
+            ((x, at.float(), w), 'int32 or int64'), ((x, at.expand(3, 3)[0][::2], w), '1-D'), ((x, at, w.float()), 'float64'),
+            ((x, at, torch.zeros(9, dtype=torch.float64)), 'a head has 16'), ((x, at, torch.zeros(16, dtype=torch.float64)[::2]), 'contiguous'),
+            (([1.0], at, w), 'tensor'), ((x, 5, w), 'tensor'), ((x, at, None), 'tensor'), ((x, at, w), 'CUDA')):
+        for call in (ops.rotary, ops.rotary_backward):
+            with pytest.raises(ValueError, match=message):
+                call(*arguments)
+    with pytest.raises(ValueError, match='layout'):
+        ops.rotary(x, at, w, layout='pairs')
+    for out, message in ((x.half(), 'shape and dtype'), (torch.zeros(3, 2, 18), 'shape and dtype'), (torch.zeros(1, 2, 16).expand(3, 2, 16), 'expanded'),
+                         (torch.zeros(3, 1, 16).expand(3, 2, 16), 'expanded')):
+        with pytest.raises(ValueError, match=message):
+            ops.rotary(x, at, w, out=out)
+    with pytest.raises(ValueError, match='lie elsewhere'):
+        ops.rotary(x, at, w, out=x.reshape(2, 3, 16).transpose(0, 1))
+
+
+def test_append_refuses():
+    k_pages, v_pages, tables, _ = cache()
+    k, rows, at, w = torch.zeros(3, 2, 16, dtype=torch.float16), torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int64), torch.zeros(8, dtype=torch.float64)
+    good = dict(k=k, v=k, k_pages=k_pages, v_pages=v_pages, tables=tables, rows=rows, positions=at, frequencies=w, q=k)
+    for changed, message in (
+            (dict(v=k[:2]), 'shape'), (dict(v=k.float()), 'dtype'), (dict(k_pages=k_pages.float(), v_pages=v_pages.float()), 'dtype'), (dict(k=k.double()), 'dtype'),
+            (dict(k=k[:, :1], v=k[:, :1]), 'shape'), (dict(k_pages=k_pages[0]), 'k_pages must be'), (dict(v_pages=v_pages[:2]), 'one shape'), (dict(v_pages=v_pages.float()), 'one shape'),
+            (dict(k_pages=k_pages.transpose(1, 2).contiguous().transpose(1, 2)), 'dense'), (dict(v_pages=v_pages[:1].expand(4, 2, 8, 16)), 'same strides'),
+            (dict(k_pages=k_pages[:1].expand(4, 2, 8, 16), v_pages=v_pages[:1].expand(4, 2, 8, 16)), 'expanded'),
+            (dict(tables=tables.long()), 'tables'), (dict(tables=tables[0]), 'tables'), (dict(tables=tables.t()), 'tables'), (dict(rows=rows.long()), 'int32'), (dict(rows=rows[:2]), 'entries'),
+            (dict(positions=at[:1]), 'entries'), (dict(frequencies=torch.zeros(9, dtype=torch.float64)), 'a head has'), (dict(layout='none'), 'layout'),
+            (dict(q=k.float()), 'q must be'), (dict(q=k[:2]), 'q must be'), (dict(q=None, q_out=k), 'without q'), (dict(q_out=k.float()), 'q_out'),
+            (dict(q_out=k[:, :1].expand(3, 2, 16)), 'expanded'), (dict(rows=None), 'tensor'), (dict(), 'CUDA')):
+        with pytest.raises(ValueError, match=message):
+            ops.paged_append(**{**good, **changed})
+
+
+def test_attention_refuses():
+    k_pages, v_pages, tables, lens = cache()
+    q = torch.zeros(3, 4, 16, dtype=torch.float16)
+    good = dict(q=q, k_pages=k_pages, v_pages=v_pages, tables=tables, lengths=lens, scale=0.25)
+    for changed, message in (
+            (dict(q=q.float()), 'dtype'), (dict(q=q.double()), 'dtype'), (dict(q=q[..., :8]), 'head size'), (dict(q=q[:, :3]), 'multiple'), (dict(q=q[0]), 'heads'),
+            (dict(q=torch.zeros(4, 4, 16, dtype=torch.float16)), '3 sequences'), (dict(lengths=lens.long()), 'int32'), (dict(lengths=lens[:2]), 'entries'),
+            (dict(rows=lens.long()), 'int32'), (dict(rows=lens[:2]), 'entries'), (dict(rows=[0, 1, 2]), 'tensor'), (dict(window=-1), 'window'),
+            (dict(k_pages=k_pages[:, :0], v_pages=v_pages[:, :0]), 'multiple'), (dict(k_pages=k_pages[:, :, :0], v_pages=v_pages[:, :, :0]), 'at least one'),
+            (dict(out=q.bfloat16()), 'out'), (dict(out=q.float()[:2]), 'out'), (dict(out=torch.zeros(3, 1, 16).expand(3, 4, 16)), 'expanded'), (dict(), 'CUDA')):
+        with pytest.raises(ValueError, match=message):
+            ops.paged_attention(**{**good, **changed})
+
+
+def test_copies_refuse():
+    pool, pair = torch.zeros(2, 3, 2, 8, 16), torch.zeros(1, dtype=torch.int32)
+    for arguments, message in (
+            ((pool[0, 0, 0], pair, pair), 'pages must be'), ((pool[None, None], pair, pair), 'pages must be'), ((pool.transpose(2, 3), pair, pair), 'dense'),
+            ((pool[:, :, :, :4], pair, pair), 'dense'), ((pool[..., :8], pair, pair), 'dense'), ((pool[:, :1].expand(2, 3, 2, 8, 16), pair, pair), 'expanded'),
+            ((pool[:1].expand(2, 3, 2, 8, 16), pair, pair), 'expanded'), ((pool[:, None].expand(2, 2, 3, 2, 8, 16), pair, pair), 'evenly|expanded'),
+            ((pool, pair.long(), pair), 'int32'), ((pool, pair, pair.repeat(2)), 'entries'), ((pool, [0], [1]), 'tensor'), ((pool, pair, pair), 'CUDA')):
+        with pytest.raises(ValueError, match=message):
+            ops.copy_pages(*arguments)
+
+
+def test_the_c_entries_check_before_any_cuda_call():
+    library = native.lib()
+    one = 1 << 20
+    rotary = [one, one, one, 0, one, 1, 1, 8, 4, 8, 8, 8, 8, 0, 0, 1.0, 0, None]
+    append = [one] * 7 + [0, 1, 1, 8, 8, 8, 8, 8, 4, 8, 64, 64, 1, 1, 1, one, 4, 0, 1.0, one, one, 1, 8, 8, 8, 8, 0, None]
+    attention = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 0, 1, None]
+    copies = [one, 1, 64, 4, 64, 64, one, one, 1, None]
+    for name, good, bad in (
+            ('dtn_rotary', rotary, {0: None, 1: None, 2: None, 4: None, 5: -1, 6: -1, 7: -1, 8: 5, 16: 3}),
+            ('dtn_paged_append', append, {0: None, 1: None, 2: None, 3: None, 4: None, 5: None, 6: None, 8: -1, 9: -1, 10: -1, 15: -1, 16: 0, 19: -1, 20: -1, 22: None,
+                                          23: 5, 26: None, 27: None, 28: -1, 33: -1}),
+            ('dtn_paged_attention', attention, {0: None, 1: None, 2: None, 3: None, 4: None, 6: None, 7: -1, 8: 3, 9: 2 ** 40, 15: -1, 16: 0, 19: -1, 20: -1, 23: -1, 24: 5}),
+            ('dtn_copy_pages', copies, {0: None, 1: -1, 3: -1, 5: -1, 6: None, 7: None, 8: -1})):
+        for place, value in bad.items():
+            arguments = list(good)
+            arguments[place] = value
+            if name == 'dtn_paged_attention' and place == 8:
+                arguments[9] = 2                                  # three query heads over two kv heads
+            assert getattr(library, name)(*arguments) == native.ERR_INVALID, (name, place)
+            assert native.last_error()
+    for name, good, changes in (('dtn_rotary', rotary, {7: 1025}), ('dtn_rotary', rotary, {5: 2 ** 31}), ('dtn_paged_append', append, {10: 1025}),
+                                ('dtn_paged_attention', attention, {10: 257}), ('dtn_copy_pages', copies, {8: 2 ** 31})):
+        arguments = list(good)
+        for place, value in changes.items():
+            arguments[place] = value
+        assert getattr(library, name)(*arguments) == native.ERR_UNSUPPORTED, (name, changes)
+    # nothing to do is no error, and needs no pointer and no device
+    for name, good, changes in (('dtn_rotary', rotary, {0: None, 5: 0}), ('dtn_rotary', rotary, {1: None, 6: 0}), ('dtn_paged_append', append, {0: None, 8: 0}),
+                                ('dtn_paged_attention', attention, {0: None, 7: 0}), ('dtn_copy_pages', copies, {0: None, 8: 0})):
+        arguments = list(good)
+        for place, value in changes.items():
+            arguments[place] = value
+        assert getattr(library, name)(*arguments) == native.OK, (name, changes)
+
+
+def test_page_reports_have_their_own_error(monkeypatch):
+    for word, text in ((0x6103, 'paged attention'), (0x6200, 'paged append'), (0x63ff, 'copy of pages')):
+        monkeypatch.setattr(native, 'device_status', lambda stream=0, word=word: word)
+        with pytest.raises(native.PageError, match=text):
+            native.raise_on_device_status(0)
+    monkeypatch.setattr(native, 'device_status', lambda stream=0: 0x7100)
+    with pytest.raises(native.DeviceWaitError, match='self-test'):
+        native.raise_on_device_status(0)
