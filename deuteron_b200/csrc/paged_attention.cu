@@ -1,92 +1,718 @@
 // Attention of one new token per sequence over a paged key-value cache.
+//
+// For each sequence and query head: out = sum_t p_t v_t / sum_t p_t, p_t = 2^(x_t - m), x_t = scale log2(e) q.k_t, with the
+// running maximum m, denominator and numerator of one pass over the tokens. The bytes of the keys and values are the floor:
+// with g query heads on one kv head the work is 2 g multiply-adds per element read, far below what the card does per byte, so
+// everything here serves an even, deep and unbroken stream of loads.
+//
+//   Shares. A unit is one tile of tokens (CHUNK per team of warps) of one (sequence, kv head, block of query heads); the
+//   units of the whole batch, tile fastest, then head, then sequence, are cut into equal contiguous ranges, one per block
+//   of a grid that fills the card once. So the split over a sequence's length follows from the lengths on the device: no host
+//   copy of them, one launch, any raggedness, and a captured launch follows lengths that change.
+//   Pipeline. Each team keeps a ring of stages in shared memory filled by 16-byte asynchronous copies, several stages ahead
+//   and across the ends of sequences; a token's row is looked up through the page table one stage before its copies are
+//   issued. Nothing but the stage's own warps waits for a stage.
+//   Products, 16-bit storage. mma.sync m16n8k16 with the tokens as the 16 rows and the query heads as the 8 columns:
+//   scores = K Q^T, numerators = V^T P^T, so that a group of up to 8 heads wastes nothing and the probabilities turn from
+//   result to operand layout with one movmatrix per 8 x 8. (tcgen05 would need 64 or 128 rows of heads or a round trip of P
+//   through shared memory; at 2 g products per element the tensor pipe idles either way.) P is split into two f16 or three
+//   bf16 terms, which keeps the products with V exact to about 2^-23, and a chunk's product starts from zero and is added
+//   to the FP32 numerator by fused multiply-add with the rescaling factor: the tensor core's own accumulator truncates.
+//   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
+//   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
+//   heads are split into blocks that read the keys again.
+//   Join. A block that holds a whole item writes it. Otherwise it leaves (m, sum, numerators) in the workspace and counts
+//   itself in; the last to arrive adds the parts in the order of the blocks, so the result does not depend on who was last.
+//   It leaves the counter at zero for the next launch.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace dtn {
+
+constexpr int PA_WARPS = 4;
+constexpr int PA_MAX_BLOCKS = 1024;        // counters in the workspace
+constexpr int PA_COUNTER_BYTES = PA_MAX_BLOCKS * 4;
 
 struct PagedAttentionParams {
   const void *q, *k_pages, *v_pages;
   void* out;
   const int *tables, *lengths, *rows;   // rows may be null: sequence i uses row i
-  int64_t count, sequences, pages, table_stride, capacity;
-  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  int64_t page_stride, page_head_stride;
-  int q_heads, kv_heads, group, dim, page_size;
+  int64_t count, sequences, pages, table_stride;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;   // elements
+  int64_t page_stride, page_head_stride;                                      // bytes
   int64_t window;
+  int capacity;                         // tokens that a row of the tables covers
+  int heads;                            // items per sequence: kv heads x blocks of query heads
+  int blocks;                           // blocks of query heads per kv head
+  int group, dim, page_size, row_bytes;
+  uint32_t divide_mul;                  // position / page_size = (position * divide_mul) >> divide_shift
+  int divide_shift;
   float scale_log2e;
-  int out_f32;
+  int out_f32, q_pairs;                 // q_pairs: two neighbouring elements of q lie on a 4-byte boundary
+  int min_units;                        // a block takes at least this many units
+  int* counters;
+  float* parts;
   int* status;
 };
 
-// One warp per (sequence, query head): the running maximum and sum of a softmax over the tokens, in order.
-template <typename T, int PER_LANE>
-__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const PagedAttentionParams p) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (item >= p.count * p.q_heads) return;
-  const int64_t sequence = item / p.q_heads;
-  const int head = (int)(item % p.q_heads), kv_head = head / p.group;
-  int64_t row = p.rows ? p.rows[sequence] : sequence;
-  int64_t length = row >= 0 && row < p.sequences ? p.lengths[row] : 0;
-  if (row >= p.sequences || length > p.capacity) {
+// First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
+__host__ __device__ __forceinline__ int64_t pa_share_begin(int64_t units, int64_t workers, int64_t c) { return units * c / workers; }
+__host__ __device__ __forceinline__ int64_t pa_share_owner(int64_t units, int64_t workers, int64_t unit) {
+  return ((unit + 1) * workers - 1) / units;
+}
+// Blocks that take part: each has at least min_units units, but for the only one.
+__host__ __device__ __forceinline__ int64_t pa_workers(int64_t units, int64_t min_units, int64_t grid) {
+  const int64_t most = units / min_units;
+  return most < 1 ? 1 : (most < grid ? most : grid);
+}
+
+template <typename T, int DP, int HB>
+struct PaConfig {
+  static constexpr bool HALF = sizeof(T) == 2;
+  static constexpr int CHUNK = HALF ? 16 : 8;            // tokens per stage
+  static constexpr int TEAMS = PA_WARPS / HB;
+  static constexpr int ROW = DP * (int)sizeof(T);
+  static constexpr int STAGE = 2 * CHUNK * ROW;          // keys, then values: 64 * DP bytes
+  static constexpr int SLOTS = DP == 64 ? 24 : 12;
+  static constexpr int STAGES = HB == 4 ? (HALF ? 10 : 8) : SLOTS / TEAMS;
+  static constexpr int RING = TEAMS * STAGES * STAGE;
+  static constexpr int MERGE = HB == 4 ? 128 * DP : 0;   // else the stage just read holds a team's numerators
+  static constexpr int QUERY = HALF ? 0 : HB * 8 * DP * 4;
+  static constexpr int SMEM = RING + MERGE + QUERY;
+  static constexpr int BLOCKS_PER_SM = DP == 256 ? 1 : 2;
+  static constexpr int HEADS = 8 * HB;                   // query heads of an item
+  static constexpr int PART = HEADS * DP + 2 * HEADS;    // floats: numerators, maxima, sums
+};
+
+
+__device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pa_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void pa_ldmatrix(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void pa_ldmatrix_t(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ uint32_t pa_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Rounds a pair to the storage type (low half first) and leaves what the rounding took off.
+__device__ __forceinline__ uint32_t pa_take(float& a, float& b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  a -= f.x;
+  b -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pa_take(float& a, float& b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const float2 f = __bfloat1622float2(h);
+  a -= f.x;
+  b -= f.y;
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// What is seen of a sequence: its row of the tables, its first token that is seen and how many.
+struct PaSequence {
+  int64_t table;
+  int first, seen;
+};
+
+__device__ __forceinline__ PaSequence pa_sequence(const PagedAttentionParams& p, int64_t i) {
+  PaSequence s = {0, 0, 0};
+  const int64_t row = p.rows ? (int64_t)p.rows[i] : i;
+  if (row < 0) return s;
+  if (row >= p.sequences) {
     paged_report(p.status, PAGED_STATUS_ATTENTION);
-    length = length > p.capacity ? p.capacity : length;
+    return s;
   }
-  int64_t first = p.window > 0 && length > p.window ? length - p.window : 0;
-  float q[PER_LANE], acc[PER_LANE], m = -INFINITY, l = 0.f;
-  const T* query = static_cast<const T*>(p.q) + sequence * p.q_token_stride + head * p.q_head_stride;
-  for (int i = 0; i < PER_LANE; ++i) {
-    const int d = lane + 32 * i;
-    q[i] = d < p.dim ? to_float(query[d]) : 0.f;
-    acc[i] = 0.f;
+  int length = p.lengths[row];
+  if (length > p.capacity) {
+    paged_report(p.status, PAGED_STATUS_ATTENTION);
+    length = p.capacity;
   }
-  bool bad = false;
-  for (int64_t t = first; t < length; ++t) {
-    const int64_t index = t / p.page_size;
-    int page = p.tables[row * p.table_stride + index];
-    if (page < 0 || page >= p.pages) {
-      bad = true;
-      continue;
+  if (length <= 0) return s;
+  s.table = row * p.table_stride;
+  s.first = p.window > 0 && p.window < length ? length - (int)p.window : 0;
+  s.seen = length - s.first;
+  return s;
+}
+
+template <int UNIT>
+__device__ __forceinline__ int pa_tiles(int seen) { return seen <= UNIT ? 1 : (seen - 1) / UNIT + 1; }
+
+// A place in the order of the units.
+template <int UNIT>
+struct PaCursor {
+  int64_t sequence;
+  int head, tile, tiles;
+  PaSequence s;
+
+  __device__ __forceinline__ void enter(const PagedAttentionParams& p) {
+    if (sequence < p.count) s = pa_sequence(p, sequence);
+    tiles = pa_tiles<UNIT>(s.seen);
+  }
+  __device__ __forceinline__ void step(const PagedAttentionParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++head < p.heads) return;
+    head = 0;
+    ++sequence;
+    enter(p);
+  }
+};
+
+template <typename T, int DP, int HB>
+__global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER_SM) paged_attention_kernel(const PagedAttentionParams p) {
+  using C = PaConfig<T, DP, HB>;
+  constexpr int CHUNK = C::CHUNK, TEAMS = C::TEAMS, ROW = C::ROW, STAGES = C::STAGES, UNIT = CHUNK * TEAMS, THREADS = PA_WARPS * 32;
+  constexpr int LANES = ROW / 16;                  // 16-byte vectors of a row
+  constexpr float NONE = -INFINITY;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_max[PA_WARPS][8], s_sum[PA_WARPS][8];
+  __shared__ float s_p[C::HALF ? 1 : PA_WARPS][8][8], s_alpha[C::HALF ? 1 : PA_WARPS][8];
+  __shared__ int64_t s_scan[PA_WARPS];
+  __shared__ int64_t s_start[2];
+  __shared__ int s_last;
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, team = warp / HB, member = warp % HB;
+  const int g = lane / 4, t = lane % 4;
+
+  // -- the share of this block: thread i adds up a contiguous part of the sequences ---------------
+  const int64_t per = (p.count + THREADS - 1) / THREADS, mine = tid * per, mine_end = mine + per < p.count ? mine + per : p.count;
+  int64_t sum = 0;
+  for (int64_t i = mine; i < mine_end; ++i) sum += pa_tiles<UNIT>(pa_sequence(p, i).seen);
+  int64_t before = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += other;
+  }
+  if (lane == 31) s_scan[warp] = before;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  before -= sum;
+  const int64_t units = total * p.heads;
+  const int64_t workers = pa_workers(units, p.min_units, gridDim.x);
+  if (blockIdx.x >= workers) return;
+  const int64_t begin = pa_share_begin(units, workers, blockIdx.x), end = pa_share_begin(units, workers, blockIdx.x + 1);
+  if (begin >= before * p.heads && begin < (before + sum) * p.heads) {
+    int64_t at = before * p.heads;
+    for (int64_t i = mine; i < mine_end; ++i) {
+      const int64_t here = (int64_t)pa_tiles<UNIT>(pa_sequence(p, i).seen) * p.heads;
+      if (begin < at + here) {
+        s_start[0] = i;
+        s_start[1] = begin - at;
+        break;
+      }
+      at += here;
     }
-    const int64_t at = page * p.page_stride + kv_head * p.page_head_stride + (t - index * p.page_size) * p.dim;
-    const T *k = static_cast<const T*>(p.k_pages) + at, *v = static_cast<const T*>(p.v_pages) + at;
-    float s = 0.f;
-    for (int i = 0; i < PER_LANE; ++i) s = fmaf(q[i], lane + 32 * i < p.dim ? to_float(k[lane + 32 * i]) : 0.f, s);
-    s = warp_sum(s) * p.scale_log2e;
-    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-    const float alpha = ex2_approx(m - base), pr = ex2_approx(s - base);
-    l = fmaf(l, alpha, pr);
-    for (int i = 0; i < PER_LANE; ++i) acc[i] = fmaf(acc[i], alpha, pr * (lane + 32 * i < p.dim ? to_float(v[lane + 32 * i]) : 0.f));
-    m = top;
   }
-  if (bad && lane == 0) paged_report(p.status, PAGED_STATUS_ATTENTION);
-  if (bad) l = __int_as_float(0x7fffffff);   // NaN: a page that does not exist is no zero
-  for (int i = 0; i < PER_LANE; ++i) {
-    const int d = lane + 32 * i;
-    if (d >= p.dim) continue;
-    const float y = first < length ? acc[i] / l : 0.f;
-    const int64_t to = sequence * p.out_token_stride + head * p.out_head_stride + d;
-    if (p.out_f32)
-      static_cast<float*>(p.out)[to] = y;
+  __syncthreads();
+  PaCursor<UNIT> now, ahead;
+  now.sequence = s_start[0];
+  now.s = {0, 0, 0};
+  now.enter(p);
+  now.head = (int)(s_start[1] / now.tiles);
+  now.tile = (int)(s_start[1] % now.tiles);
+  ahead = now;
+  const int steps = (int)(end - begin);
+
+  // -- copies -------------------------------------------------------------------------------------
+  uint8_t* ring = smem + team * STAGES * C::STAGE;
+  const uint32_t ring_address = smem_u32(ring);
+  int64_t offset = -1;             // of the row of token lane % CHUNK of the stage that is copied next; -1: not seen, -2: no such page
+  uint32_t bad_stages = 0;         // stages that hold a token without a page
+
+  auto look_up = [&]() {
+    const int token = (ahead.tile * TEAMS + team) * CHUNK + lane % CHUNK;
+    offset = -1;
+    if (token < ahead.s.seen) {
+      const int position = ahead.s.first + token;
+      const int index = (int)(((uint64_t)(uint32_t)position * p.divide_mul) >> p.divide_shift);
+      const int page = p.tables[ahead.s.table + index];
+      offset = -2;
+      if (page >= 0 && page < p.pages)
+        offset = page * p.page_stride + (ahead.head / p.blocks) * p.page_head_stride + (int64_t)(position - index * p.page_size) * p.row_bytes;
+    }
+  };
+  auto copy = [&](int slot) {
+    const bool bad = __any_sync(0xffffffffu, offset == -2);
+    bad_stages = (bad_stages & ~(1u << slot)) | ((uint32_t)bad << slot);
+    if (bad && lane == 0) paged_report(p.status, PAGED_STATUS_ATTENTION);
+    if (__any_sync(0xffffffffu, offset != -1)) {
+      const uint32_t stage = ring_address + slot * C::STAGE;
+#pragma unroll
+      for (int j = 0; j < CHUNK / HB * LANES / 32; ++j) {
+        const int v = lane + 32 * j, row = member * (CHUNK / HB) + v / LANES, column = v % LANES;
+        const int64_t at = __shfl_sync(0xffffffffu, offset, row);
+        const int swizzled = C::HALF ? column ^ (row & 7) : column ^ ((row & 1) << 2);
+        const uint32_t to = stage + row * ROW + swizzled * 16;
+        const bool there = at >= 0 && column * 16 < p.row_bytes;   // else zeros: neither what is not seen nor the columns past a head count
+        const int64_t from = there ? at + column * 16 : 0;
+        pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
+        pa_copy16(to + CHUNK * ROW, static_cast<const uint8_t*>(p.v_pages) + from, there ? 16 : 0);
+      }
+    }
+  };
+  auto team_barrier = [&]() {
+    if (HB == 1)
+      __syncwarp();
     else
-      static_cast<T*>(p.out)[to] = from_float<T>(y);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * HB) : "memory");
+  };
+
+  if (steps > 0) look_up();
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (i < steps) {
+      copy(i);
+      ahead.step(p);
+      if (i + 1 < steps) look_up();
+    }
+    pa_commit();
+  }
+
+  // -- queries ------------------------------------------------------------------------------------
+  constexpr int STEPS_K = DP / 16;
+  uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF ? STEPS_K : 1][2];
+  float* s_query = reinterpret_cast<float*>(smem + C::RING + C::MERGE);
+  auto head_of = [&](int item_head, int h) { return (item_head % p.blocks) * C::HEADS + h; };   // within the group
+  auto load_query = [&](int64_t sequence, int item_head) {   // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
+    const int h = head_of(item_head, member * 8 + g);
+    const bool there = h < p.group;
+    const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)(item_head / p.blocks) * p.group + (there ? h : 0)) * p.q_head_stride;
+#pragma unroll
+    for (int ks = 0; ks < STEPS_K; ++ks) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int d = ks * 16 + half * 8 + 2 * t;
+        uint32_t v = 0;
+        if (there && d < p.dim) {   // dim is even
+          if (p.q_pairs)
+            v = *reinterpret_cast<const uint32_t*>(q + d);
+          else
+            v = *reinterpret_cast<const uint16_t*>(q + d) | (uint32_t) * reinterpret_cast<const uint16_t*>(q + d + 1) << 16;
+        }
+        query_next[ks][half] = v;
+      }
+    }
+  };
+  if constexpr (C::HALF) load_query(now.sequence, now.head);
+
+  // -- the pass over the tokens -------------------------------------------------------------------
+  constexpr int COLUMNS = DP / 32;                 // FP32 storage: columns of V per lane
+  float top[2] = {NONE, NONE}, total_p[2] = {0.f, 0.f};   // of heads 2t, 2t + 1
+  float acc[C::HALF ? DP / 16 : 8][C::HALF ? 4 : COLUMNS];
+  bool fresh = true, from_start = now.tile == 0, poisoned = false;
+
+  for (int step = 0; step < steps; ++step) {
+    const int slot = step % STAGES;
+    pa_wait<STAGES - 2>();
+    team_barrier();
+    if (step + STAGES - 1 < steps) {
+      copy((step + STAGES - 1) % STAGES);
+      ahead.step(p);
+      if (step + STAGES < steps) look_up();
+    }
+    pa_commit();
+
+    if (fresh) {
+      fresh = false;
+      from_start = now.tile == 0;
+      poisoned = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) top[i] = NONE, total_p[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < (C::HALF ? DP / 16 : 8); ++i)
+#pragma unroll
+        for (int j = 0; j < (C::HALF ? 4 : COLUMNS); ++j) acc[i][j] = 0.f;
+      if constexpr (C::HALF) {
+#pragma unroll
+        for (int ks = 0; ks < STEPS_K; ++ks) query[ks][0] = query_next[ks][0], query[ks][1] = query_next[ks][1];
+        if (step + (now.tiles - now.tile) < steps) {   // the next item's, a whole item ahead
+          const bool same = now.head + 1 < p.heads;
+          load_query(same ? now.sequence : now.sequence + 1, same ? now.head + 1 : 0);
+        }
+      } else {
+        __syncthreads();
+        for (int i = tid; i < C::HEADS * DP; i += THREADS) {
+          const int h = head_of(now.head, i / DP), d = i % DP;
+          s_query[i] = h < p.group && d < p.dim ? static_cast<const float*>(p.q)[now.sequence * p.q_token_stride +
+                                                      ((int64_t)(now.head / p.blocks) * p.group + h) * p.q_head_stride + d] : 0.f;
+        }
+        __syncthreads();
+      }
+    }
+
+    const int base = (now.tile * TEAMS + team) * CHUNK, seen = now.s.seen;
+    poisoned |= (bad_stages >> slot) & 1;
+    if (base < seen) {
+      const uint32_t stage = ring_address + slot * C::STAGE;
+      constexpr int SETS = C::HALF ? 2 : 1;        // tokens g (and g + 8) of the chunk
+      float x[SETS][2];
+      if constexpr (C::HALF) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        const int row = lane % 16;
+#pragma unroll
+        for (int ks = 0; ks < STEPS_K; ++ks) {
+          uint32_t a[4];
+          pa_ldmatrix(a, stage + row * ROW + (((2 * ks + lane / 16) ^ (row & 7)) * 16));
+          pa_mma(s, a, query[ks][0], query[ks][1], T());
+        }
+        x[0][0] = s[0], x[0][1] = s[1];
+        x[SETS - 1][0] = s[2], x[SETS - 1][1] = s[3];
+      } else {
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const float* query_rows = s_query + member * 8 * DP;
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) {
+          const int column = t + 4 * j;
+          const float4 k = *reinterpret_cast<const float4*>(ring + slot * C::STAGE + g * ROW + ((column ^ ((g & 1) << 2)) * 16));
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            const float4 q = *reinterpret_cast<const float4*>(query_rows + h * DP + column * 4);
+            s[h] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[h]))));
+          }
+        }
+        // four lanes hold parts of a token's 8 scores; lane t ends with heads 2t and 2t + 1
+        float r[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float kept = t & 2 ? s[h + 4] : s[h], sent = t & 2 ? s[h] : s[h + 4];
+          r[h] = kept + __shfl_xor_sync(0xffffffffu, sent, 2);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float kept = t & 1 ? r[h + 2] : r[h], sent = t & 1 ? r[h] : r[h + 2];
+          x[0][h] = kept + __shfl_xor_sync(0xffffffffu, sent, 1);
+        }
+      }
+      float alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float high = top[i];
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {
+          x[n][i] = base + g + 8 * n < seen ? x[n][i] * p.scale_log2e : NONE;
+          high = fmaxf(high, x[n][i]);
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        const float around = high == NONE ? 0.f : high;   // every score -inf so far: the exponentials are zeros, not NaN
+        alpha[i] = ex2_approx_ftz(top[i] - around);
+        top[i] = high;
+        total_p[i] *= alpha[i];
+#pragma unroll
+        for (int n = 0; n < SETS; ++n) {
+          x[n][i] = ex2_approx_ftz(x[n][i] - around);
+          total_p[i] += x[n][i];
+        }
+      }
+      if constexpr (C::HALF) {
+        constexpr int TERMS = std::is_same_v<T, __half> ? 2 : 3;
+        const float whole_p[2][2] = {{x[0][0], x[0][1]}, {x[1][0], x[1][1]}};
+        uint32_t b[TERMS][2];
+#pragma unroll
+        for (int n = 0; n < TERMS; ++n) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) b[n][half] = pa_transpose(pa_take(x[half][0], x[half][1], T()));
+        }
+        const int row = lane % 8 + (lane / 16) * 8;
+        constexpr int TOGETHER = 4;   // 16-column tiles of V between two checks
+#pragma unroll
+        for (int first = 0; first < DP / 16; first += TOGETHER) {
+          float y[TOGETHER][4], probe = 0.f;
+#pragma unroll
+          for (int i = 0; i < TOGETHER; ++i) {
+            uint32_t a[4];
+            pa_ldmatrix_t(a, stage + CHUNK * ROW + row * ROW + (((2 * (first + i) + (lane / 8) % 2) ^ (row & 7)) * 16));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[i][j] = 0.f;
+#pragma unroll
+            for (int n = TERMS - 1; n >= 0; --n) pa_mma(y[i], a, b[n][0], b[n][1], T());   // small terms first
+#pragma unroll
+            for (int j = 0; j < 4; ++j) probe = fmaf(y[i][j], 0.f, probe);
+          }
+          if (__any_sync(0xffffffffu, probe != 0.f)) {
+            // an infinite value times a probability's small term, or zero, is not what it is times the probability: once more,
+            // with whole probabilities (held by the lane of the token and head)
+#pragma unroll
+            for (int i = 0; i < TOGETHER; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[i][j] = 0.f;
+#pragma unroll
+            for (int token = 0; token < CHUNK; ++token) {
+              const float p0 = __shfl_sync(0xffffffffu, whole_p[token / 8][0], token % 8 * 4 + t);
+              const float p1 = __shfl_sync(0xffffffffu, whole_p[token / 8][1], token % 8 * 4 + t);
+#pragma unroll
+              for (int i = 0; i < TOGETHER; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const uint8_t* at = ring + slot * C::STAGE + CHUNK * ROW + token * ROW + (((2 * (first + i) + j) ^ (token & 7)) * 16) + g * 2;
+                  const float v = to_float(*reinterpret_cast<const T*>(at));
+                  y[i][2 * j] = fmaf(p0, v, y[i][2 * j]);
+                  y[i][2 * j + 1] = fmaf(p1, v, y[i][2 * j + 1]);
+                }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < TOGETHER; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[first + i][j] = fmaf(acc[first + i][j], alpha[j % 2], y[i][j]);
+        }
+      } else {
+        s_p[warp][g][2 * t] = x[0][0];
+        s_p[warp][g][2 * t + 1] = x[0][1];
+        if (g == 0) s_alpha[warp][2 * t] = alpha[0], s_alpha[warp][2 * t + 1] = alpha[1];
+        __syncwarp();
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            const float a = s_alpha[warp][h];
+#pragma unroll
+            for (int j = 0; j < COLUMNS; ++j) acc[h][j] *= a;
+          }
+        }
+#pragma unroll
+        for (int token = 0; token < CHUNK; ++token) {
+          const uint8_t* values = ring + slot * C::STAGE + CHUNK * ROW + token * ROW;
+          float v[COLUMNS];
+          if constexpr (COLUMNS == 2) {
+            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(values + (((lane / 2) ^ ((token & 1) << 2)) * 16) + (lane % 2) * 8);
+          } else {
+#pragma unroll
+            for (int j = 0; j < COLUMNS / 4; ++j)
+              *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(values + (((lane + 32 * j) ^ ((token & 1) << 2)) * 16));
+          }
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            const float pr = s_p[warp][token][h];
+#pragma unroll
+            for (int j = 0; j < COLUMNS; ++j) acc[h][j] = fmaf(pr, v[j], acc[h][j]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+
+    // -- the end of an item, or of this block's part of it ----------------------------------------
+    const bool to_end = now.tile + 1 == now.tiles;
+    if (to_end || step + 1 == steps) {
+      // the teams' parts meet in shared memory: maxima and sums by warp, numerators in the stage that was just read (its
+      // refill is a step away). Columns are swizzled by the head so that neither side meets bank conflicts
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
+        if (g == 0) {
+          s_max[warp][2 * t + i] = top[i];
+          s_sum[warp][2 * t + i] = poisoned ? __int_as_float(0x7fffffff) : total_p[i];   // NaN: a page that does not exist is no zero
+        }
+      }
+      team_barrier();   // every warp of the team has read the stage
+      float* numerators = reinterpret_cast<float*>(HB == 4 ? smem + C::RING : ring + slot * C::STAGE) + member * 8 * DP;
+      if constexpr (C::HALF) {
+#pragma unroll
+        for (int mt = 0; mt < DP / 16; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) numerators[(2 * t + j % 2) * DP + ((mt * 16 + g + 8 * (j / 2)) ^ (t << 3))] = acc[mt][j];
+      } else {
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+#pragma unroll
+          for (int j = 0; j < COLUMNS; ++j) {
+            const int d = COLUMNS == 2 ? 2 * lane + j : (j / 4) * 128 + 4 * lane + j % 4;
+            numerators[h * DP + (d ^ ((h / 2) << 3))] = acc[h][j];
+          }
+      }
+      __syncthreads();
+      const bool whole = from_start && to_end;
+      const int64_t kv_head = now.head / p.blocks;
+      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * C::PART;
+      auto write = [&](int h, int d, float value) {   // h within the group
+        const int64_t to = now.sequence * p.out_token_stride + (kv_head * p.group + h) * p.out_head_stride + d;
+        if (p.out_f32)
+          static_cast<float*>(p.out)[to] = value;
+        else
+          static_cast<T*>(p.out)[to] = from_float<T>(value);
+      };
+      for (int i = tid; i < C::HEADS * DP; i += THREADS) {
+        const int slot_head = i / DP, d = i % DP, h = head_of(now.head, slot_head);
+        if (h >= p.group || d >= p.dim) continue;
+        float high = NONE;
+#pragma unroll
+        for (int m = 0; m < TEAMS; ++m) high = fmaxf(high, s_max[m * HB + slot_head / 8][slot_head % 8]);
+        const float around = high == NONE ? 0.f : high;
+        float value = 0.f, weight_sum = 0.f;
+#pragma unroll
+        for (int m = 0; m < TEAMS; ++m) {
+          const int w = m * HB + slot_head / 8;
+          const float weight = ex2_approx_ftz(s_max[w][slot_head % 8] - around);
+          const float* from = reinterpret_cast<const float*>(HB == 4 ? smem + C::RING : smem + (m * STAGES + slot) * C::STAGE);
+          value = fmaf(weight, from[slot_head * DP + (d ^ (((slot_head % 8) / 2) << 3))], value);
+          weight_sum = fmaf(weight, s_sum[w][slot_head % 8], weight_sum);
+        }
+        if (whole) {
+          write(h, d, now.s.seen > 0 ? value / weight_sum : 0.f);
+        } else {
+          __stcg(part + i, value);
+          if (d == 0) {
+            __stcg(part + C::HEADS * DP + slot_head, high);
+            __stcg(part + C::HEADS * DP + C::HEADS + slot_head, weight_sum);
+          }
+        }
+      }
+      if (!whole) {
+        const int64_t item = begin + step - now.tile;   // the item's first unit
+        const int64_t first = pa_share_owner(units, workers, item), last = pa_share_owner(units, workers, item + now.tiles - 1);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) s_last = atomicAdd(p.counters + first, 1) == (int)(last - first);
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          if (tid == 0) p.counters[first] = 0;
+          // the parts, added in the order of the blocks: the first block's second part, every other's first
+          const int count = (int)(last - first) + 1;
+          const float* parts = p.parts + (first * 2 + 1) * C::PART;
+          auto part_of = [&](int n) { return parts + (n == 0 ? 0 : (int64_t)(2 * n - 1) * C::PART); };
+          for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
+            const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.head, slot_head);
+            if (h >= p.group || d >= p.dim) continue;
+            float high = NONE;
+#pragma unroll 8
+            for (int n = 0; n < count; ++n) high = fmaxf(high, __ldcg(part_of(n) + C::HEADS * DP + slot_head));
+            const float around = high == NONE ? 0.f : high;
+            float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
+            float weight_sum = 0.f;
+#pragma unroll 8
+            for (int n = 0; n < count; ++n) {
+              const float* from = part_of(n);
+              const float weight = ex2_approx_ftz(__ldcg(from + C::HEADS * DP + slot_head) - around);
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(from + slot_head * DP + d));
+              weight_sum = fmaf(weight, __ldcg(from + C::HEADS * DP + C::HEADS + slot_head), weight_sum);
+              value.x = fmaf(weight, v.x, value.x);
+              value.y = fmaf(weight, v.y, value.y);
+              value.z = fmaf(weight, v.z, value.z);
+              value.w = fmaf(weight, v.w, value.w);
+            }
+            const float values[4] = {value.x, value.y, value.z, value.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (d + j < p.dim) write(h, d + j, values[j] / weight_sum);
+          }
+        }
+      }
+      __syncthreads();   // the stage and the maxima are free again
+      fresh = true;
+    }
+    now.step(p);
   }
 }
 
-template <typename T>
-static int paged_attention_launch_t(const PagedAttentionParams& p, cudaStream_t s) {
-  const int64_t items = p.count * p.q_heads;
-  paged_attention_simple_kernel<T, 8><<<(unsigned)((items + 3) / 4), 128, 0, s>>>(p);
-  DTN_LAUNCH_CHECK("paged_attention_simple_kernel");
+
+static size_t pa_workspace_bytes() {
+  // two parts per block of the largest forms: 32 heads of 128 and two blocks per SM, 32 heads of 256 and one
+  const size_t blocks = (size_t)sm_count();
+  const size_t small = 2 * blocks * 2 * PaConfig<float, 128, 4>::PART, large = blocks * 2 * PaConfig<float, 256, 4>::PART;
+  return PA_COUNTER_BYTES + (small > large ? small : large) * sizeof(float);
+}
+
+template <typename T, int DP, int HB>
+static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
+  using C = PaConfig<T, DP, HB>;
+  static thread_local int attr_dev = -1;
+  int dev = 0;
+  DTN_CUDA_CHECK(cudaGetDevice(&dev));
+  if (attr_dev != dev) {
+    DTN_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_kernel<T, DP, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_dev = dev;
+  }
+  p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
+  p.heads *= p.blocks;
+  int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
+  if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
+  const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;
+  if (p.count < grid && p.heads < grid && most_tiles < grid && p.count * p.heads * most_tiles < grid) grid = p.count * p.heads * most_tiles;
+  paged_attention_kernel<T, DP, HB><<<(unsigned)grid, PA_WARPS * 32, C::SMEM, s>>>(p);
+  DTN_LAUNCH_CHECK("paged_attention_kernel");
   return DTN_OK;
+}
+
+template <typename T, int DP>
+static int paged_attention_launch_d(PagedAttentionParams& p, cudaStream_t s) {
+  if (p.group <= 8) return paged_attention_launch_t<T, DP, 1>(p, s);
+  if (p.group <= 16) return paged_attention_launch_t<T, DP, 2>(p, s);
+  return paged_attention_launch_t<T, DP, 4>(p, s);
+}
+
+template <typename T>
+static int paged_attention_launch(PagedAttentionParams& p, cudaStream_t s) {
+  if (p.dim <= 64) return paged_attention_launch_d<T, 64>(p, s);
+  if (p.dim <= 128) return paged_attention_launch_d<T, 128>(p, s);
+  return paged_attention_launch_d<T, 256>(p, s);
 }
 
 }  // namespace dtn
 
-extern "C" int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
-                                   void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
-                                   int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
-                                   int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
-                                   int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* stream) {
+extern "C" {
+
+int dtn_paged_attention_workspace_bytes(size_t* bytes_out) {
+  DTN_REQUIRE(bytes_out != nullptr, DTN_ERR_INVALID, "paged attention: bytes_out is null");
+  *bytes_out = dtn::pa_workspace_bytes();
+  return DTN_OK;
+}
+
+int dtn_paged_attention_plan(const int64_t* tiles, int64_t count, int64_t heads, int64_t min_units, int64_t grid, int64_t* begin_out,
+                             int64_t* first_out, int64_t* last_out, int64_t* workers_out) {
+  using namespace dtn;
+  DTN_REQUIRE(tiles && count > 0 && heads > 0 && min_units > 0 && grid > 0, DTN_ERR_INVALID, "paged attention plan: bad extent");
+  int64_t units = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    DTN_REQUIRE(tiles[i] > 0, DTN_ERR_INVALID, "paged attention plan: a sequence has at least one tile");
+    units += tiles[i] * heads;
+  }
+  const int64_t workers = pa_workers(units, min_units, grid);
+  if (workers_out) *workers_out = workers;
+  if (begin_out)
+    for (int64_t c = 0; c <= workers; ++c) begin_out[c] = pa_share_begin(units, workers, c);
+  int64_t at = 0;
+  for (int64_t i = 0; i < count * heads; ++i) {
+    if (first_out) first_out[i] = pa_share_owner(units, workers, at);
+    at += tiles[i / heads];
+    if (last_out) last_out[i] = pa_share_owner(units, workers, at - 1);
+  }
+  return DTN_OK;
+}
+
+int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
+                        void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
+                        int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
+                        int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
+                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   using namespace dtn;
   DTN_REQUIRE(count >= 0 && q_heads >= 0 && kv_heads >= 0 && dim >= 0 && pages >= 0 && sequences >= 0 && pages_per_sequence >= 0 && window >= 0,
               DTN_ERR_INVALID, "paged attention: negative extent");
@@ -95,15 +721,24 @@ extern "C" int dtn_paged_attention(const void* q, const void* k_pages, const voi
   if (count == 0 || q_heads == 0 || dim == 0) return DTN_OK;
   DTN_REQUIRE(kv_heads > 0 && q_heads % kv_heads == 0, DTN_ERR_INVALID, "paged attention: query heads must be a multiple of kv heads");
   DTN_REQUIRE(dim <= 256, DTN_ERR_UNSUPPORTED, "paged attention: heads of at most 256 elements");
-  DTN_REQUIRE(q && out && (rows || count <= sequences), DTN_ERR_INVALID, "paged attention: null pointer");
+  const int64_t element = paged_storage_bytes(storage);
+  DTN_REQUIRE(dim * element % 16 == 0 && page_stride * element % 16 == 0 && page_head_stride * element % 16 == 0 && aligned_to(k_pages, 16) &&
+                  aligned_to(v_pages, 16),
+              DTN_ERR_INVALID, "paged attention: the heads of the pools must start on 16-byte boundaries and have a multiple of 16 bytes");
+  DTN_REQUIRE(q && out && lengths && (rows || count <= sequences), DTN_ERR_INVALID, "paged attention: null pointer");
   DTN_REQUIRE((k_pages && v_pages) || pages == 0, DTN_ERR_INVALID, "paged attention: null pool");
-  DTN_REQUIRE(sequences == 0 || (lengths && (tables || pages_per_sequence == 0)), DTN_ERR_INVALID, "paged attention: null tables");
-  DTN_REQUIRE(pages < (1LL << 31) && count * q_heads < (1LL << 31), DTN_ERR_UNSUPPORTED, "paged attention: too many rows for one launch");
+  DTN_REQUIRE(sequences == 0 || tables || pages_per_sequence == 0, DTN_ERR_INVALID, "paged attention: null tables");
+  DTN_REQUIRE(pages < (1LL << 31) && count < (1LL << 31) && q_heads < (1LL << 20) && pages_per_sequence < (1LL << 31), DTN_ERR_UNSUPPORTED,
+              "paged attention: too many rows or pages for one launch");
+  DTN_REQUIRE(workspace && workspace_bytes >= pa_workspace_bytes(), DTN_ERR_WORKSPACE, "paged attention: %zu bytes of workspace, %zu needed", workspace_bytes,
+              pa_workspace_bytes());
+  DTN_REQUIRE(aligned_to(workspace, 16), DTN_ERR_WORKSPACE, "paged attention: the workspace must be 16-byte aligned");
   cudaStream_t s = as_stream(stream);
+  const int64_t capacity = pages_per_sequence * page_size, most = (1LL << 31) - (1 << 16);
   PagedAttentionParams p = {};
   p.q = q;
-  p.k_pages = k_pages;
-  p.v_pages = v_pages;
+  p.k_pages = pages ? k_pages : q;   // an empty pool is never read, but copies of no bytes name an address
+  p.v_pages = pages ? v_pages : q;
   p.out = out;
   p.tables = tables;
   p.lengths = lengths;
@@ -112,23 +747,41 @@ extern "C" int dtn_paged_attention(const void* q, const void* k_pages, const voi
   p.sequences = sequences;
   p.pages = pages;
   p.table_stride = table_stride;
-  p.capacity = pages_per_sequence * page_size;
+  p.capacity = (int)(capacity < most ? capacity : most);
   p.q_token_stride = q_token_stride;
   p.q_head_stride = q_head_stride;
   p.out_token_stride = out_token_stride;
   p.out_head_stride = out_head_stride;
-  p.page_stride = page_stride;
-  p.page_head_stride = page_head_stride;
-  p.q_heads = (int)q_heads;
-  p.kv_heads = (int)kv_heads;
+  p.page_stride = page_stride * element;
+  p.page_head_stride = page_head_stride * element;
+  p.heads = (int)kv_heads;
   p.group = (int)(q_heads / kv_heads);
   p.dim = (int)dim;
   p.page_size = (int)page_size;
+  p.row_bytes = (int)(dim * element);
   p.window = window;
   p.scale_log2e = scale * 1.4426950408889634f;
   p.out_f32 = out_f32;
+  p.q_pairs = element == 2 && aligned_to(q, 4) && q_token_stride % 2 == 0 && q_head_stride % 2 == 0;
+  p.min_units = 2;
+  // position / page_size for positions below 2^31: mul = floor(2^(31 + s) / d) + 1 with 2^s >= d exceeds 2^(31 + s) / d by at
+  // most 1, so the product exceeds the quotient by less than 2^31 / 2^(31 + s) <= 1 / d: the floor is exact. mul <= 2^32 - 1
+  // needs d > 1; for d = 1 the multiplier is 1 and the shift 0.
+  if (page_size == 1) {
+    p.divide_mul = 1;
+    p.divide_shift = 0;
+  } else {
+    int bits = 1;
+    while ((1LL << bits) < page_size) ++bits;
+    p.divide_shift = 31 + bits;
+    p.divide_mul = (uint32_t)((1ULL << (31 + bits)) / (uint64_t)page_size + 1);
+  }
+  p.counters = static_cast<int*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + PA_COUNTER_BYTES);
   p.status = device_status_word_unless_capturing(s);
-  if (storage == DTN_STORAGE_F32) return paged_attention_launch_t<float>(p, s);
-  if (storage == DTN_STORAGE_F16) return paged_attention_launch_t<__half>(p, s);
-  return paged_attention_launch_t<__nv_bfloat16>(p, s);
+  if (storage == DTN_STORAGE_F32) return paged_attention_launch<float>(p, s);
+  if (storage == DTN_STORAGE_F16) return paged_attention_launch<__half>(p, s);
+  return paged_attention_launch<__nv_bfloat16>(p, s);
 }
+
+}  // extern "C"

@@ -70,7 +70,10 @@ _SIGNATURES = {
     'dtn_paged_append': [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                          _I64, _P, _I64, _I, _F, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P],
     'dtn_paged_attention': [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-                            _I64, _I64, _F, _I64, _I, _I, _P],
+                            _I64, _I64, _F, _I64, _I, _I, _P, ct.c_size_t, _P],
+    'dtn_paged_attention_workspace_bytes': [ct.POINTER(ct.c_size_t)],
+    'dtn_paged_attention_plan': [ct.POINTER(ct.c_int64), _I64, _I64, _I64, _I64, ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64),
+                                 ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64)],
     'dtn_copy_pages': [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P],
 }
 

@@ -558,6 +558,27 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     return q_out
 
 
+_paged_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_PAGED_COUNTER_BYTES = 4096
+
+
+def _paged_workspace(device: torch.device) -> tuple[int, int]:
+    """Address and size of the parts and counters of `paged_attention`, one workspace per device and stream. Its counters are zeroed
+    here once; every call leaves them zero. A call that is captured gets one of its own from the graph's memory, zeroed by each
+    replay: replays may run beside one another and beside eager calls."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    key = (device.index, _stream())
+    workspace = None if capturing else _paged_workspaces.get(key)
+    if workspace is None:
+        size = ct.c_size_t(0)
+        native.call('dtn_paged_attention_workspace_bytes', ct.byref(size))
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+        workspace[:_PAGED_COUNTER_BYTES].zero_()
+        if not capturing:
+            _paged_workspaces[key] = workspace
+    return workspace.data_ptr(), workspace.numel()
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, scale: float,
                     rows: torch.Tensor | None = None, window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per sequence over a paged key-value cache: q[n, q_heads, dim] -> out[n, q_heads, dim].
@@ -565,7 +586,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Pools and tables as in `paged_append`; lengths: int32 [sequences], the tokens of each that are seen (the new one among
     them). rows: int32 [n], the sequence of each query (None: query i is sequence i); a negative row (padding of a captured
     batch) and a length of zero give zeros. window > 0 keeps the last `window` tokens only. Query head h reads kv head
-    h // (q_heads // kv_heads). Storage float32 / float16 / bfloat16, softmax and sums in FP32; `out` is float32 by default, as
+    h // (q_heads // kv_heads). Heads have a multiple of 16 bytes (at most 256 elements) and start on 16-byte boundaries in the
+    pools. Storage float32 / float16 / bfloat16, softmax and sums in FP32; `out` is float32 by default, as
     `gqa_attention` returns it, or a given tensor of float32 or of q's dtype. The values in a page behind a sequence's end do
     not matter, NaN included. A row or length outside the tables, or a page number outside the pool, makes
     `check_device_status` raise PageError; a sequence with such a page gets NaN.
@@ -599,7 +621,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     native.call('dtn_paged_attention', q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
                 None if rows is None else rows.data_ptr(), out.data_ptr(), count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head,
                 pages, page_size, page_stride, page_head_stride, tables.shape[0], tables.shape[1],
-                tables.stride(0) if tables.shape[0] > 1 else 0, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, _stream())
+                tables.stride(0) if tables.shape[0] > 1 else 0, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, *_paged_workspace(q.device), _stream())
     return out
 
 

@@ -355,12 +355,30 @@ int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
  * tokens of sequence r = rows[i] (rows NULL: r = i). Query head h reads kv head h / (q_heads / kv_heads). A negative row or a
  * length of zero gives zeros. out is FP32, or of `storage` when out_f32 is zero. A row >= sequences or a length beyond the tables is
  * reported by dtn_device_status (the length is cut), and so is a page number outside the pool, which makes the sequence's
- * output NaN; nothing outside the pools is read. What lies in the pools behind a sequence's end is not used, whatever it holds. */
+ * output NaN; nothing outside the pools is read. What lies in the pools behind a sequence's end is not used, whatever it holds.
+ * Heads of the pools have a multiple of 16 bytes (at most 256 elements) and start on 16-byte boundaries. `workspace` has
+ * dtn_paged_attention_workspace_bytes bytes, 16-byte aligned, and is zeroed once before its first call; every call leaves its
+ * first 4096 bytes (counters) zero again. Calls that can overlap on the GPU need a workspace each. Same result on every
+ * run of the same call. */
 int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
                         void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
                         int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
                         int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
-                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* stream);
+                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that serve any dtn_paged_attention call on the current device. */
+int dtn_paged_attention_workspace_bytes(size_t* bytes_out /* host */);
+
+/* How dtn_paged_attention cuts a batch among its blocks: host arithmetic only (the kernel does the same on the device from the
+ * lengths). Sequence i has tiles[i] >= 1 tiles of tokens for each of `heads` items (kv heads x blocks of query heads); the
+ * units, tile fastest, then item, then sequence, are cut into *workers_out contiguous ranges [begin_out[c],
+ * begin_out[c + 1]), as many as `grid` allows with at least min_units each. first_out / last_out (count * heads entries) are
+ * the blocks that hold an item's first and last unit; the parts of an item are added in that order. Output pointers may be
+ * NULL; begin_out needs grid + 1 entries. */
+int dtn_paged_attention_plan(const int64_t* tiles /* host */, int64_t count, int64_t heads, int64_t min_units, int64_t grid,
+                             int64_t* begin_out /* host */, int64_t* first_out /* host */, int64_t* last_out /* host */,
+                             int64_t* workers_out /* host */);
 
 /* Copies page sources[i] onto page destinations[i] in each of `planes` planes of a pool (a layer's keys or values each),
  * i < pairs. Strides and page_bytes in bytes; a page's bytes are dense. No destination may be a source or occur twice. A

@@ -1,5 +1,7 @@
 """Refusals and host-side parts of the rotary and paged-cache operators; no GPU."""
+import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -103,7 +105,7 @@ def test_the_c_entries_check_before_any_cuda_call():
     one = 1 << 20
     rotary = [one, one, one, 0, one, 1, 1, 8, 4, 8, 8, 8, 8, 0, 0, 1.0, 0, None]
     append = [one] * 7 + [0, 1, 1, 8, 8, 8, 8, 8, 4, 8, 64, 64, 1, 1, 1, one, 4, 0, 1.0, one, one, 1, 8, 8, 8, 8, 0, None]
-    attention = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 0, 1, None]
+    attention = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 0, 1, one, 1 << 30, None]
     copies = [one, 1, 64, 4, 64, 64, one, one, 1, None]
     for name, good, bad in (
             ('dtn_rotary', rotary, {0: None, 1: None, 2: None, 4: None, 5: -1, 6: -1, 7: -1, 8: 5, 16: 3}),
@@ -131,6 +133,58 @@ def test_the_c_entries_check_before_any_cuda_call():
         for place, value in changes.items():
             arguments[place] = value
         assert getattr(library, name)(*arguments) == native.OK, (name, changes)
+
+
+def test_attention_entry_refuses_alignment_and_workspace():
+    library, one = native.lib(), 1 << 20
+    good = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 1, 1, one, 1 << 30, None]
+    size = ctypes.c_size_t(0)
+    native.call('dtn_paged_attention_workspace_bytes', ctypes.byref(size))
+    assert 4096 < size.value < 16 << 20
+    for place, value, status, text in ((1, one + 8, native.ERR_INVALID, '16-byte'), (2, one + 2, native.ERR_INVALID, '16-byte'), (10, 12, native.ERR_INVALID, '16-byte'),
+                                       (17, 60, native.ERR_INVALID, '16-byte'), (18, 4, native.ERR_INVALID, '16-byte'), (26, None, native.ERR_WORKSPACE, 'workspace'),
+                                       (27, size.value - 1, native.ERR_WORKSPACE, 'needed'), (26, one + 4, native.ERR_WORKSPACE, 'aligned')):
+        arguments = list(good)
+        arguments[place] = value
+        assert library.dtn_paged_attention(*arguments) == status and text in native.last_error(), (place, native.last_error())
+
+
+def test_the_plan_covers_every_unit_once_and_names_its_owners():
+    generator = random.Random(3)
+    cases = [([1], 1, 1, 1), ([1], 8, 2, 296), ([1000], 1, 2, 296), ([1, 1, 1], 1, 1, 2), ([2 ** 27], 8, 2, 296), ([5, 1, 700, 1, 33], 4, 2, 148)]
+    cases += [([generator.randint(1, 60) for _ in range(generator.randint(1, 40))], generator.randint(1, 9), generator.randint(1, 4), generator.randint(1, 300)) for _ in range(60)]
+    for tiles, heads, least, grid in cases:
+        items = len(tiles) * heads
+        begin, first, last, workers = ((ctypes.c_int64 * n)() for n in (grid + 1, items, items, 1))
+        native.call('dtn_paged_attention_plan', (ctypes.c_int64 * len(tiles))(*tiles), len(tiles), heads, least, grid, begin, first, last, workers)
+        count, units = workers[0], sum(tiles) * heads
+        shares = [begin[c + 1] - begin[c] for c in range(count)]
+        assert 1 <= count <= grid and begin[0] == 0 and begin[count] == units and max(shares) - min(shares) <= 1
+        assert min(shares) >= least or count == 1
+        at, started = 0, []
+        for item in range(items):
+            end = at + tiles[item // heads]
+            owners = [c for c in range(count) if begin[c] < end and begin[c + 1] > at]
+            assert (first[item], last[item]) == (owners[0], owners[-1]) and owners == list(range(owners[0], owners[-1] + 1))
+            if len(owners) > 1:
+                started.append(first[item])
+            at = end
+        assert len(set(started)) == len(started)          # one counter per block is enough: no two split items start in one block
+    assert native.lib().dtn_paged_attention_plan((ctypes.c_int64 * 1)(0), 1, 1, 1, 1, None, None, None, None) == native.ERR_INVALID
+
+
+def test_positions_are_divided_by_a_multiplication():
+    # the multiplier and shift that the kernel is given: floor(2^(31 + s) / d) + 1 and 31 + s with 2^s >= d
+    generator = random.Random(5)
+    for d in [2, 3, 5, 7, 8, 16, 24, 50, 64, 1000, 2 ** 20 - 1, 2 ** 30 + 1, 2 ** 31 - 1] + [generator.randint(2, 2 ** 31 - 1) for _ in range(200)]:
+        s = 1
+        while 1 << s < d:
+            s += 1
+        multiplier = (1 << (31 + s)) // d + 1
+        assert multiplier < 2 ** 32
+        for n in [0, 1, d - 1, d, d + 1, 2 ** 31 - 1, (2 ** 31 - 1) // d * d, (2 ** 31 - 1) // d * d - 1] + [generator.randint(0, 2 ** 31 - 1) for _ in range(50)]:
+            if 0 <= n < 2 ** 31:
+                assert n * multiplier >> (31 + s) == n // d and n * multiplier < 2 ** 64
 
 
 def test_page_reports_have_their_own_error(monkeypatch):
