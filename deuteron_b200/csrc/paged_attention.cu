@@ -5,9 +5,9 @@
 // with g query heads on one kv head the work is 2 g multiply-adds per element read, far below what the card does per byte, so
 // everything here serves an even, deep and unbroken stream of loads.
 //
-//   Shares. A unit is one tile of tokens (CHUNK per team of warps) of one (sequence, kv head, block of query heads); the
-//   units of the whole batch, tile fastest, then head, then sequence, are cut into equal contiguous ranges, one per block
-//   of a grid that fills the card once. So the split over a sequence's length follows from the lengths on the device: no host
+//   Shares. A unit is one tile of tokens (CHUNK per team of warps) of one item (sequence, kv head, block of query heads), and
+//   PA_ITEM_UNITS more stand at an item's end for what finishing it costs; the units of the whole batch, tile fastest, then
+//   head, then sequence, are cut into equal contiguous ranges, one per block of a grid that fills the card once. So the split over a sequence's length follows from the lengths on the device: no host
 //   copy of them, one launch, any raggedness, and a captured launch follows lengths that change.
 //   Pipeline. Each team keeps a ring of stages in shared memory filled by 16-byte asynchronous copies, several stages ahead
 //   and across the ends of sequences; a token's row is looked up through the page table one stage before its copies are
@@ -17,7 +17,7 @@
 //   result to operand layout with one movmatrix per 8 x 8. (tcgen05 would need 64 or 128 rows of heads or a round trip of P
 //   through shared memory; at 2 g products per element the tensor pipe idles either way.) P is split into two f16 or three
 //   bf16 terms, which keeps the products with V exact to about 2^-23, and a chunk's product starts from zero and is added
-//   to the FP32 numerator by fused multiply-add with the rescaling factor: the tensor core's own accumulator truncates.
+//   to the FP32 numerator apart: the tensor core's own accumulator truncates.
 //   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
 //   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
 //   heads are split into blocks that read the keys again.
@@ -43,18 +43,23 @@ struct PagedAttentionParams {
   int64_t page_stride, page_head_stride;                                      // bytes
   int64_t window;
   int capacity;                         // tokens that a row of the tables covers
-  int heads;                            // items per sequence: kv heads x blocks of query heads
+  int heads, kv_heads;                  // items per sequence: kv heads x blocks of query heads
   int blocks;                           // blocks of query heads per kv head
-  int group, dim, page_size, row_bytes;
+  int q_heads, group, dim, page_size, row_bytes;
   uint32_t divide_mul;                  // position / page_size = (position * divide_mul) >> divide_shift
   int divide_shift;
   float scale_log2e;
-  int out_f32, q_pairs;                 // q_pairs: two neighbouring elements of q lie on a 4-byte boundary
+  int out_f32;
+  int q_pairs, out_quads;               // neighbouring elements of q and out can be moved by two (4 bytes) and by four
+  int whole_chunks;                     // a chunk never straddles pages and rows fill their place in shared memory
   int min_units;                        // a block takes at least this many units
   int* counters;
   float* parts;
   int* status;
 };
+
+// Units for the end of an item: the teams' parts are added, the result written, the next query taken.
+constexpr int PA_ITEM_UNITS = 2;
 
 // First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
 __host__ __device__ __forceinline__ int64_t pa_share_begin(int64_t units, int64_t workers, int64_t c) { return units * c / workers; }
@@ -89,6 +94,13 @@ struct PaConfig {
 __device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Two FP32 sums in one instruction.
+__device__ __forceinline__ void pa_add2(float& a0, float& a1, float b0, float b1) {
+  asm("{ .reg .b64 a, b; mov.b64 a, {%0, %1}; mov.b64 b, {%2, %3}; add.rn.f32x2 a, a, b; mov.b64 {%0, %1}, a; }" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
 __device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void pa_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -112,6 +124,14 @@ __device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], ui
 __device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void pa_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Rounds a pair to the storage type (low half first) and leaves what the rounding took off.
 __device__ __forceinline__ uint32_t pa_take(float& a, float& b, __half) {
@@ -156,26 +176,40 @@ __device__ __forceinline__ PaSequence pa_sequence(const PagedAttentionParams& p,
 }
 
 template <int UNIT>
-__device__ __forceinline__ int pa_tiles(int seen) { return seen <= UNIT ? 1 : (seen - 1) / UNIT + 1; }
+__device__ __forceinline__ int pa_tiles(int seen) { return seen <= 0 ? 0 : (seen - 1) / UNIT + 1; }
 
-// A place in the order of the units.
+// Units of one item of a sequence; none where nothing is seen (its zeros are written apart).
+__device__ __forceinline__ int64_t pa_item_units(int tiles) { return tiles > 0 ? (int64_t)tiles + PA_ITEM_UNITS : 0; }
+
+// A place in the order of the units, always a tile.
 template <int UNIT>
 struct PaCursor {
   int64_t sequence;
-  int head, tile, tiles;
+  int left;                      // units of the share from here on
+  int kv_head, block;            // block of query heads
+  int tile, tiles;
   PaSequence s;
 
   __device__ __forceinline__ void enter(const PagedAttentionParams& p) {
-    if (sequence < p.count) s = pa_sequence(p, sequence);
+    s = pa_sequence(p, sequence);
     tiles = pa_tiles<UNIT>(s.seen);
   }
-  __device__ __forceinline__ void step(const PagedAttentionParams& p) {
-    if (++tile < tiles) return;
+  __device__ __forceinline__ void next_item(const PagedAttentionParams& p) {   // from the first unit behind this item's tiles
+    left -= PA_ITEM_UNITS;
     tile = 0;
-    if (++head < p.heads) return;
-    head = 0;
-    ++sequence;
-    enter(p);
+    if (++block < p.blocks) return;
+    block = 0;
+    if (++kv_head < p.kv_heads) return;
+    kv_head = 0;
+    do {
+      ++sequence;
+      if (sequence >= p.count) return;   // past every share
+      enter(p);
+    } while (tiles == 0);
+  }
+  __device__ __forceinline__ void step(const PagedAttentionParams& p) {
+    --left;
+    if (++tile == tiles) next_item(p);
   }
 };
 
@@ -198,7 +232,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
   // -- the share of this block: thread i adds up a contiguous part of the sequences ---------------
   const int64_t per = (p.count + THREADS - 1) / THREADS, mine = tid * per, mine_end = mine + per < p.count ? mine + per : p.count;
   int64_t sum = 0;
-  for (int64_t i = mine; i < mine_end; ++i) sum += pa_tiles<UNIT>(pa_sequence(p, i).seen);
+  for (int64_t i = mine; i < mine_end; ++i) sum += pa_item_units(pa_tiles<UNIT>(pa_sequence(p, i).seen));
   int64_t before = sum;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -214,14 +248,24 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
     total += s_scan[w];
   }
   before -= sum;
+  for (int64_t i = blockIdx.x; i < p.count; i += gridDim.x) {   // rows that see nothing
+    if (pa_sequence(p, i).seen > 0) continue;
+    for (int j = tid; j < p.q_heads * p.dim; j += THREADS) {
+      const int64_t to = i * p.out_token_stride + j / p.dim * p.out_head_stride + j % p.dim;
+      if (p.out_f32)
+        static_cast<float*>(p.out)[to] = 0.f;
+      else
+        static_cast<T*>(p.out)[to] = from_float<T>(0.f);
+    }
+  }
   const int64_t units = total * p.heads;
   const int64_t workers = pa_workers(units, p.min_units, gridDim.x);
-  if (blockIdx.x >= workers) return;
+  if (units == 0 || blockIdx.x >= workers) return;
   const int64_t begin = pa_share_begin(units, workers, blockIdx.x), end = pa_share_begin(units, workers, blockIdx.x + 1);
   if (begin >= before * p.heads && begin < (before + sum) * p.heads) {
     int64_t at = before * p.heads;
     for (int64_t i = mine; i < mine_end; ++i) {
-      const int64_t here = (int64_t)pa_tiles<UNIT>(pa_sequence(p, i).seen) * p.heads;
+      const int64_t here = pa_item_units(pa_tiles<UNIT>(pa_sequence(p, i).seen)) * p.heads;
       if (begin < at + here) {
         s_start[0] = i;
         s_start[1] = begin - at;
@@ -232,13 +276,20 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
   }
   __syncthreads();
   PaCursor<UNIT> now, ahead;
+  now.left = (int)(end - begin);
   now.sequence = s_start[0];
-  now.s = {0, 0, 0};
   now.enter(p);
-  now.head = (int)(s_start[1] / now.tiles);
-  now.tile = (int)(s_start[1] % now.tiles);
+  {
+    const int item = (int)(s_start[1] / pa_item_units(now.tiles));
+    now.kv_head = item / p.blocks;
+    now.block = item % p.blocks;
+    now.tile = (int)(s_start[1] % pa_item_units(now.tiles));
+    if (now.tile >= now.tiles) {   // the share begins behind an item's tiles
+      now.left += now.tile - now.tiles;
+      now.next_item(p);
+    }
+  }
   ahead = now;
-  const int steps = (int)(end - begin);
 
   // -- copies -------------------------------------------------------------------------------------
   uint8_t* ring = smem + team * STAGES * C::STAGE;
@@ -255,26 +306,45 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       const int page = p.tables[ahead.s.table + index];
       offset = -2;
       if (page >= 0 && page < p.pages)
-        offset = page * p.page_stride + (ahead.head / p.blocks) * p.page_head_stride + (int64_t)(position - index * p.page_size) * p.row_bytes;
+        offset = page * p.page_stride + ahead.kv_head * p.page_head_stride + (int64_t)(position - index * p.page_size) * p.row_bytes;
     }
   };
+  // Lane l copies vector l % LANES of rows l / LANES, + 32 / LANES, ...: their swizzled places differ by constants.
+  constexpr int ROWS = CHUNK / HB;                 // of a stage, copied by this warp
+  const int lane_row = member * ROWS + (LANES <= 32 ? lane / LANES : 0), lane_column = LANES <= 32 ? lane % LANES : lane;
+  const uint8_t* const k_lane = static_cast<const uint8_t*>(p.k_pages) + lane_column * 16;
+  const uint8_t* const v_lane = static_cast<const uint8_t*>(p.v_pages) + lane_column * 16;
+  const uint32_t lane_place = lane_row * ROW + ((C::HALF ? lane_column ^ (lane_row & 7) : lane_column ^ ((lane_row & 1) << 2)) * 16);
   auto copy = [&](int slot) {
+    const uint32_t seen_rows = __ballot_sync(0xffffffffu, offset >= 0);
+    const uint32_t stage = ring_address + slot * C::STAGE;
+    if (seen_rows == 0xffffffffu && p.whole_chunks) {   // one page holds the rows one after another: constant distances
+      const int64_t at = __shfl_sync(0xffffffffu, offset, 0) + (LANES <= 32 ? lane_row : member * ROWS) * ROW;
+#pragma unroll
+      for (int j = 0; j < ROWS * LANES / 32; ++j) {
+        // rows between two copies of a lane; a row of 64 vectors takes two copies, 512 bytes apart
+        const int row = LANES <= 32 ? j * (LANES <= 32 ? 32 / LANES : 1) : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;
+        const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + row * ROW + half;
+        pa_copy16(to, k_lane + at + row * ROW + half);
+        pa_copy16(to + CHUNK * ROW, v_lane + at + row * ROW + half);
+      }
+      bad_stages &= ~(1u << slot);
+      return;
+    }
     const bool bad = __any_sync(0xffffffffu, offset == -2);
     bad_stages = (bad_stages & ~(1u << slot)) | ((uint32_t)bad << slot);
     if (bad && lane == 0) paged_report(p.status, PAGED_STATUS_ATTENTION);
-    if (__any_sync(0xffffffffu, offset != -1)) {
-      const uint32_t stage = ring_address + slot * C::STAGE;
+    if (!bad && seen_rows == 0) return;
 #pragma unroll
-      for (int j = 0; j < CHUNK / HB * LANES / 32; ++j) {
-        const int v = lane + 32 * j, row = member * (CHUNK / HB) + v / LANES, column = v % LANES;
-        const int64_t at = __shfl_sync(0xffffffffu, offset, row);
-        const int swizzled = C::HALF ? column ^ (row & 7) : column ^ ((row & 1) << 2);
-        const uint32_t to = stage + row * ROW + swizzled * 16;
-        const bool there = at >= 0 && column * 16 < p.row_bytes;   // else zeros: neither what is not seen nor the columns past a head count
-        const int64_t from = there ? at + column * 16 : 0;
-        pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
-        pa_copy16(to + CHUNK * ROW, static_cast<const uint8_t*>(p.v_pages) + from, there ? 16 : 0);
-      }
+    for (int j = 0; j < ROWS * LANES / 32; ++j) {
+      const int v = lane + 32 * j, row = member * ROWS + v / LANES, column = v % LANES;
+      const int64_t at = __shfl_sync(0xffffffffu, offset, row);
+      const int swizzled = C::HALF ? column ^ (row & 7) : column ^ ((row & 1) << 2);
+      const uint32_t to = stage + row * ROW + swizzled * 16;
+      const bool there = at >= 0 && column * 16 < p.row_bytes;   // else zeros: neither what is not seen nor the columns past a head count
+      const int64_t from = there ? at + column * 16 : 0;
+      pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
+      pa_copy16(to + CHUNK * ROW, static_cast<const uint8_t*>(p.v_pages) + from, there ? 16 : 0);
     }
   };
   auto team_barrier = [&]() {
@@ -284,25 +354,29 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * HB) : "memory");
   };
 
-  if (steps > 0) look_up();
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (i < steps) {
-      copy(i);
-      ahead.step(p);
-      if (i + 1 < steps) look_up();
+  auto fill = [&]() {
+    if (ahead.left > 0) look_up();
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (ahead.left > 0) {
+        copy(i);
+        ahead.step(p);
+        if (ahead.left > 0) look_up();
+      }
+      pa_commit();
     }
-    pa_commit();
-  }
+  };
+  fill();
 
   // -- queries ------------------------------------------------------------------------------------
   constexpr int STEPS_K = DP / 16;
   uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF ? STEPS_K : 1][2];
   float* s_query = reinterpret_cast<float*>(smem + C::RING + C::MERGE);
-  auto head_of = [&](int item_head, int h) { return (item_head % p.blocks) * C::HEADS + h; };   // within the group
-  auto load_query = [&](int64_t sequence, int item_head) {   // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
-    const int h = head_of(item_head, member * 8 + g);
+  auto head_of = [&](int block, int h) { return block * C::HEADS + h; };   // within the group
+  auto load_query = [&](int64_t sequence, int kv_head, int block) {   // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
+    const int h = head_of(block, member * 8 + g);
     const bool there = h < p.group;
-    const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)(item_head / p.blocks) * p.group + (there ? h : 0)) * p.q_head_stride;
+    const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)kv_head * p.group + (there ? h : 0)) * p.q_head_stride;
 #pragma unroll
     for (int ks = 0; ks < STEPS_K; ++ks) {
 #pragma unroll
@@ -319,28 +393,29 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       }
     }
   };
-  if constexpr (C::HALF) load_query(now.sequence, now.head);
+  if (now.left <= 0) return;   // nothing but the ends of items
+  if constexpr (C::HALF) load_query(now.sequence, now.kv_head, now.block);
 
   // -- the pass over the tokens -------------------------------------------------------------------
   constexpr int COLUMNS = DP / 32;                 // FP32 storage: columns of V per lane
   float top[2] = {NONE, NONE}, total_p[2] = {0.f, 0.f};   // of heads 2t, 2t + 1
   float acc[C::HALF ? DP / 16 : 8][C::HALF ? 4 : COLUMNS];
-  bool fresh = true, from_start = now.tile == 0, poisoned = false;
+  bool fresh = true, poisoned = false, exactly = false;
+  int start = 0, slot = 0;                         // the item's first tile here; the stage read next
 
-  for (int step = 0; step < steps; ++step) {
-    const int slot = step % STAGES;
+  while (now.left > 0) {
     pa_wait<STAGES - 2>();
     team_barrier();
-    if (step + STAGES - 1 < steps) {
-      copy((step + STAGES - 1) % STAGES);
+    if (ahead.left > 0) {
+      copy(slot == 0 ? STAGES - 1 : slot - 1);
       ahead.step(p);
-      if (step + STAGES < steps) look_up();
+      if (ahead.left > 0) look_up();
     }
     pa_commit();
 
     if (fresh) {
       fresh = false;
-      from_start = now.tile == 0;
+      start = now.tile;
       poisoned = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) top[i] = NONE, total_p[i] = 0.f;
@@ -351,16 +426,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       if constexpr (C::HALF) {
 #pragma unroll
         for (int ks = 0; ks < STEPS_K; ++ks) query[ks][0] = query_next[ks][0], query[ks][1] = query_next[ks][1];
-        if (step + (now.tiles - now.tile) < steps) {   // the next item's, a whole item ahead
-          const bool same = now.head + 1 < p.heads;
-          load_query(same ? now.sequence : now.sequence + 1, same ? now.head + 1 : 0);
-        }
+        PaCursor<UNIT> next = now;   // the next item's, a whole item ahead
+        next.left -= now.tiles - now.tile;
+        next.next_item(p);
+        if (next.left > 0) load_query(next.sequence, next.kv_head, next.block);
       } else {
         __syncthreads();
         for (int i = tid; i < C::HEADS * DP; i += THREADS) {
-          const int h = head_of(now.head, i / DP), d = i % DP;
+          const int h = head_of(now.block, i / DP), d = i % DP;
           s_query[i] = h < p.group && d < p.dim ? static_cast<const float*>(p.q)[now.sequence * p.q_token_stride +
-                                                      ((int64_t)(now.head / p.blocks) * p.group + h) * p.q_head_stride + d] : 0.f;
+                                                      ((int64_t)now.kv_head * p.group + h) * p.q_head_stride + d] : 0.f;
         }
         __syncthreads();
       }
@@ -373,16 +448,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       constexpr int SETS = C::HALF ? 2 : 1;        // tokens g (and g + 8) of the chunk
       float x[SETS][2];
       if constexpr (C::HALF) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        const int row = lane % 16;
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};   // two chains of products
+        const uint32_t k_place = stage + lane % 16 * ROW + ((lane / 16) ^ (lane % 8)) * 16;   // stages are multiples of 128 bytes
 #pragma unroll
         for (int ks = 0; ks < STEPS_K; ++ks) {
           uint32_t a[4];
-          pa_ldmatrix(a, stage + row * ROW + (((2 * ks + lane / 16) ^ (row & 7)) * 16));
-          pa_mma(s, a, query[ks][0], query[ks][1], T());
+          pa_ldmatrix(a, (k_place ^ (ks % 4 * 32)) + ks / 4 * 128);
+          pa_mma(ks % 2 ? s2 : s, a, query[ks][0], query[ks][1], T());
         }
-        x[0][0] = s[0], x[0][1] = s[1];
-        x[SETS - 1][0] = s[2], x[SETS - 1][1] = s[3];
+        x[0][0] = s[0] + s2[0], x[0][1] = s[1] + s2[1];
+        x[SETS - 1][0] = s[2] + s2[2], x[SETS - 1][1] = s[3] + s2[3];
       } else {
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         const float* query_rows = s_query + member * 8 * DP;
@@ -409,21 +484,50 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           x[0][h] = kept + __shfl_xor_sync(0xffffffffu, sent, 1);
         }
       }
-      float alpha[2];
+#pragma unroll
+      for (int n = 0; n < SETS; ++n) x[n][0] *= p.scale_log2e, x[n][1] *= p.scale_log2e;
+      if (base + CHUNK > seen) {
+#pragma unroll
+        for (int n = 0; n < SETS; ++n)
+          if (base + g + 8 * n >= seen) x[n][0] = x[n][1] = NONE;
+      }
+      // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
+      // neither f16 terms nor FP32 sums mind, and nothing is exchanged or rescaled.
+      constexpr float GROWTH = 8.f;
+      bool higher = false;
+#pragma unroll
+      for (int n = 0; n < SETS; ++n) higher |= x[n][0] > top[0] + GROWTH || x[n][1] > top[1] + GROWTH;
+      if (__any_sync(0xffffffffu, higher)) {
+        float alpha[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float high = fmaxf(top[i], fmaxf(x[0][i], x[SETS - 1][i]));
+#pragma unroll
+          for (int o = 4; o < 32; o *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+          alpha[i] = ex2_approx_ftz(top[i] - (high == NONE ? 0.f : high));
+          top[i] = high;
+          total_p[i] *= alpha[i];
+        }
+        if constexpr (C::HALF) {
+#pragma unroll
+          for (int mt = 0; mt < DP / 16; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[mt][j] *= alpha[j % 2];
+        } else {
+          if (g == 0) s_alpha[warp][2 * t] = alpha[0], s_alpha[warp][2 * t + 1] = alpha[1];
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            const float a = s_alpha[warp][h];
+#pragma unroll
+            for (int j = 0; j < COLUMNS; ++j) acc[h][j] *= a;
+          }
+          __syncwarp();
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float high = top[i];
-#pragma unroll
-        for (int n = 0; n < SETS; ++n) {
-          x[n][i] = base + g + 8 * n < seen ? x[n][i] * p.scale_log2e : NONE;
-          high = fmaxf(high, x[n][i]);
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-        const float around = high == NONE ? 0.f : high;   // every score -inf so far: the exponentials are zeros, not NaN
-        alpha[i] = ex2_approx_ftz(top[i] - around);
-        top[i] = high;
-        total_p[i] *= alpha[i];
+        const float around = top[i] == NONE ? 0.f : top[i];   // every score -inf so far: the exponentials are zeros, not NaN
 #pragma unroll
         for (int n = 0; n < SETS; ++n) {
           x[n][i] = ex2_approx_ftz(x[n][i] - around);
@@ -431,70 +535,46 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
         }
       }
       if constexpr (C::HALF) {
-        constexpr int TERMS = std::is_same_v<T, __half> ? 2 : 3;
-        const float whole_p[2][2] = {{x[0][0], x[0][1]}, {x[1][0], x[1][1]}};
-        uint32_t b[TERMS][2];
+        if (!exactly) {
+          constexpr int TERMS = std::is_same_v<T, __half> ? 2 : 3;
+          uint32_t b[TERMS][2];
 #pragma unroll
-        for (int n = 0; n < TERMS; ++n) {
+          for (int n = 0; n < TERMS; ++n) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) b[n][half] = pa_transpose(pa_take(x[half][0], x[half][1], T()));
-        }
-        const int row = lane % 8 + (lane / 16) * 8;
-        constexpr int TOGETHER = 4;   // 16-column tiles of V between two checks
+            for (int half = 0; half < 2; ++half) b[n][half] = pa_transpose(pa_take(x[half][0], x[half][1], T()));
+          }
+          const uint32_t v_place = stage + CHUNK * ROW + (lane % 8 + lane / 16 * 8) * ROW + ((lane / 8 % 2) ^ (lane % 8)) * 16;
 #pragma unroll
-        for (int first = 0; first < DP / 16; first += TOGETHER) {
-          float y[TOGETHER][4], probe = 0.f;
-#pragma unroll
-          for (int i = 0; i < TOGETHER; ++i) {
+          for (int mt = 0; mt < DP / 16; ++mt) {
             uint32_t a[4];
-            pa_ldmatrix_t(a, stage + CHUNK * ROW + row * ROW + (((2 * (first + i) + (lane / 8) % 2) ^ (row & 7)) * 16));
+            float y[4];
+            pa_ldmatrix_t(a, (v_place ^ (mt % 4 * 32)) + mt / 4 * 128);
+            pa_mma_first(y, a, b[TERMS - 1][0], b[TERMS - 1][1], T());   // small terms first
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[i][j] = 0.f;
-#pragma unroll
-            for (int n = TERMS - 1; n >= 0; --n) pa_mma(y[i], a, b[n][0], b[n][1], T());   // small terms first
-#pragma unroll
-            for (int j = 0; j < 4; ++j) probe = fmaf(y[i][j], 0.f, probe);
+            for (int n = TERMS - 2; n >= 0; --n) pa_mma(y, a, b[n][0], b[n][1], T());
+            pa_add2(acc[mt][0], acc[mt][1], y[0], y[1]);
+            pa_add2(acc[mt][2], acc[mt][3], y[2], y[3]);
           }
-          if (__any_sync(0xffffffffu, probe != 0.f)) {
-            // an infinite value times a probability's small term, or zero, is not what it is times the probability: once more,
-            // with whole probabilities (held by the lane of the token and head)
+        } else {
+#pragma unroll 1
+          for (int token = 0; token < CHUNK; ++token) {
+            const float p0 = __shfl_sync(0xffffffffu, token < 8 ? x[0][0] : x[1][0], token % 8 * 4 + t);
+            const float p1 = __shfl_sync(0xffffffffu, token < 8 ? x[0][1] : x[1][1], token % 8 * 4 + t);
+            const uint8_t* values = ring + slot * C::STAGE + CHUNK * ROW + token * ROW + g * 2;
 #pragma unroll
-            for (int i = 0; i < TOGETHER; ++i)
+            for (int mt = 0; mt < DP / 16; ++mt)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y[i][j] = 0.f;
-#pragma unroll
-            for (int token = 0; token < CHUNK; ++token) {
-              const float p0 = __shfl_sync(0xffffffffu, whole_p[token / 8][0], token % 8 * 4 + t);
-              const float p1 = __shfl_sync(0xffffffffu, whole_p[token / 8][1], token % 8 * 4 + t);
-#pragma unroll
-              for (int i = 0; i < TOGETHER; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const uint8_t* at = ring + slot * C::STAGE + CHUNK * ROW + token * ROW + (((2 * (first + i) + j) ^ (token & 7)) * 16) + g * 2;
-                  const float v = to_float(*reinterpret_cast<const T*>(at));
-                  y[i][2 * j] = fmaf(p0, v, y[i][2 * j]);
-                  y[i][2 * j + 1] = fmaf(p1, v, y[i][2 * j + 1]);
-                }
-            }
+              for (int j = 0; j < 2; ++j) {
+                const float v = to_float(*reinterpret_cast<const T*>(values + ((2 * mt + j) ^ (token & 7)) * 16));
+                acc[mt][2 * j] = fmaf(p0, v, acc[mt][2 * j]);
+                acc[mt][2 * j + 1] = fmaf(p1, v, acc[mt][2 * j + 1]);
+              }
           }
-#pragma unroll
-          for (int i = 0; i < TOGETHER; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[first + i][j] = fmaf(acc[first + i][j], alpha[j % 2], y[i][j]);
         }
       } else {
         s_p[warp][g][2 * t] = x[0][0];
         s_p[warp][g][2 * t + 1] = x[0][1];
-        if (g == 0) s_alpha[warp][2 * t] = alpha[0], s_alpha[warp][2 * t + 1] = alpha[1];
         __syncwarp();
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int h = 0; h < 8; ++h) {
-            const float a = s_alpha[warp][h];
-#pragma unroll
-            for (int j = 0; j < COLUMNS; ++j) acc[h][j] *= a;
-          }
-        }
 #pragma unroll
         for (int token = 0; token < CHUNK; ++token) {
           const uint8_t* values = ring + slot * C::STAGE + CHUNK * ROW + token * ROW;
@@ -519,7 +599,31 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
 
     // -- the end of an item, or of this block's part of it ----------------------------------------
     const bool to_end = now.tile + 1 == now.tiles;
-    if (to_end || step + 1 == steps) {
+    if (to_end || now.left == 1) {
+      if constexpr (C::HALF) {
+        // An infinite value times one term of a probability, negative or zero, is not what it is times the probability. Where
+        // a numerator is not finite the block goes over its tiles of the item once more, with whole probabilities.
+        float probe = 0.f;
+        if (!exactly) {
+#pragma unroll
+          for (int mt = 0; mt < DP / 16; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) probe = fmaf(acc[mt][j], 0.f, probe);
+        }
+        if (__syncthreads_or(probe != 0.f)) {
+          pa_wait<0>();
+          __syncthreads();   // no stage is read or written any more
+          now.left += now.tile - start;
+          now.tile = start;
+          ahead = now;
+          fill();
+          load_query(now.sequence, now.kv_head, now.block);
+          exactly = fresh = true;
+          slot = 0;
+          continue;
+        }
+        exactly = false;
+      }
       // the teams' parts meet in shared memory: maxima and sums by warp, numerators in the stage that was just read (its
       // refill is a step away). Columns are swizzled by the head so that neither side meets bank conflicts
 #pragma unroll
@@ -531,7 +635,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           s_sum[warp][2 * t + i] = poisoned ? __int_as_float(0x7fffffff) : total_p[i];   // NaN: a page that does not exist is no zero
         }
       }
-      team_barrier();   // every warp of the team has read the stage
+      if constexpr (!C::HALF) team_barrier();   // every warp of the team has read the stage
       float* numerators = reinterpret_cast<float*>(HB == 4 ? smem + C::RING : ring + slot * C::STAGE) + member * 8 * DP;
       if constexpr (C::HALF) {
 #pragma unroll
@@ -548,36 +652,48 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           }
       }
       __syncthreads();
-      const bool whole = from_start && to_end;
-      const int64_t kv_head = now.head / p.blocks;
-      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * C::PART;
-      auto write = [&](int h, int d, float value) {   // h within the group
-        const int64_t to = now.sequence * p.out_token_stride + (kv_head * p.group + h) * p.out_head_stride + d;
-        if (p.out_f32)
-          static_cast<float*>(p.out)[to] = value;
-        else
-          static_cast<T*>(p.out)[to] = from_float<T>(value);
+      const bool whole = start == 0 && to_end;
+      float* part = p.parts + ((int64_t)blockIdx.x * 2 + (start == 0 ? 1 : 0)) * C::PART;
+      auto write = [&](int h, int d, float4 y) {   // h within the group, d a multiple of four
+        const int64_t to = now.sequence * p.out_token_stride + ((int64_t)now.kv_head * p.group + h) * p.out_head_stride + d;
+        if (p.out_f32) {
+          float* out = static_cast<float*>(p.out) + to;
+          if (p.out_quads)
+            *reinterpret_cast<float4*>(out) = y;
+          else
+            out[0] = y.x, out[1] = y.y, out[2] = y.z, out[3] = y.w;
+        } else {
+          T* out = static_cast<T*>(p.out) + to;
+          alignas(8) const T rounded[4] = {from_float<T>(y.x), from_float<T>(y.y), from_float<T>(y.z), from_float<T>(y.w)};
+          if (p.out_quads && C::HALF)
+            *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(rounded);
+          else
+            out[0] = rounded[0], out[1] = rounded[1], out[2] = rounded[2], out[3] = rounded[3];
+        }
       };
-      for (int i = tid; i < C::HEADS * DP; i += THREADS) {
-        const int slot_head = i / DP, d = i % DP, h = head_of(now.head, slot_head);
+#pragma unroll 1
+      for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
+        const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.block, slot_head);
         if (h >= p.group || d >= p.dim) continue;
         float high = NONE;
 #pragma unroll
         for (int m = 0; m < TEAMS; ++m) high = fmaxf(high, s_max[m * HB + slot_head / 8][slot_head % 8]);
         const float around = high == NONE ? 0.f : high;
-        float value = 0.f, weight_sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float weight_sum = 0.f;
 #pragma unroll
         for (int m = 0; m < TEAMS; ++m) {
           const int w = m * HB + slot_head / 8;
           const float weight = ex2_approx_ftz(s_max[w][slot_head % 8] - around);
           const float* from = reinterpret_cast<const float*>(HB == 4 ? smem + C::RING : smem + (m * STAGES + slot) * C::STAGE);
-          value = fmaf(weight, from[slot_head * DP + (d ^ (((slot_head % 8) / 2) << 3))], value);
+          const float4 x = *reinterpret_cast<const float4*>(from + slot_head * DP + (d ^ (((slot_head % 8) / 2) << 3)));
+          y.x = fmaf(weight, x.x, y.x), y.y = fmaf(weight, x.y, y.y), y.z = fmaf(weight, x.z, y.z), y.w = fmaf(weight, x.w, y.w);
           weight_sum = fmaf(weight, s_sum[w][slot_head % 8], weight_sum);
         }
         if (whole) {
-          write(h, d, now.s.seen > 0 ? value / weight_sum : 0.f);
+          write(h, d, make_float4(y.x / weight_sum, y.y / weight_sum, y.z / weight_sum, y.w / weight_sum));
         } else {
-          __stcg(part + i, value);
+          __stcg(reinterpret_cast<float4*>(part + slot_head * DP + d), y);
           if (d == 0) {
             __stcg(part + C::HEADS * DP + slot_head, high);
             __stcg(part + C::HEADS * DP + C::HEADS + slot_head, weight_sum);
@@ -585,7 +701,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
         }
       }
       if (!whole) {
-        const int64_t item = begin + step - now.tile;   // the item's first unit
+        const int64_t item = end - now.left - now.tile;   // the item's first unit
         const int64_t first = pa_share_owner(units, workers, item), last = pa_share_owner(units, workers, item + now.tiles - 1);
         __threadfence();
         __syncthreads();
@@ -599,7 +715,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           const float* parts = p.parts + (first * 2 + 1) * C::PART;
           auto part_of = [&](int n) { return parts + (n == 0 ? 0 : (int64_t)(2 * n - 1) * C::PART); };
           for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
-            const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.head, slot_head);
+            const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.block, slot_head);
             if (h >= p.group || d >= p.dim) continue;
             float high = NONE;
 #pragma unroll 8
@@ -618,10 +734,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
               value.z = fmaf(weight, v.z, value.z);
               value.w = fmaf(weight, v.w, value.w);
             }
-            const float values[4] = {value.x, value.y, value.z, value.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (d + j < p.dim) write(h, d + j, values[j] / weight_sum);
+            write(h, d, make_float4(value.x / weight_sum, value.y / weight_sum, value.z / weight_sum, value.w / weight_sum));
           }
         }
       }
@@ -629,6 +742,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       fresh = true;
     }
     now.step(p);
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
   }
 }
 
@@ -651,10 +765,13 @@ static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
     attr_dev = dev;
   }
   p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
-  p.heads *= p.blocks;
+  p.heads = p.kv_heads * p.blocks;
+  p.whole_chunks = p.page_size % C::CHUNK == 0 && p.window == 0 && p.row_bytes == C::ROW;
   int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
   const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;
+  DTN_REQUIRE((double)p.count * p.heads * (double)(most_tiles + PA_ITEM_UNITS) < 2147483648.0 * (double)grid, DTN_ERR_UNSUPPORTED,
+              "paged attention: the tables cover too many tokens for one launch");
   if (p.count < grid && p.heads < grid && most_tiles < grid && p.count * p.heads * most_tiles < grid) grid = p.count * p.heads * most_tiles;
   paged_attention_kernel<T, DP, HB><<<(unsigned)grid, PA_WARPS * 32, C::SMEM, s>>>(p);
   DTN_LAUNCH_CHECK("paged_attention_kernel");
@@ -691,18 +808,19 @@ int dtn_paged_attention_plan(const int64_t* tiles, int64_t count, int64_t heads,
   DTN_REQUIRE(tiles && count > 0 && heads > 0 && min_units > 0 && grid > 0, DTN_ERR_INVALID, "paged attention plan: bad extent");
   int64_t units = 0;
   for (int64_t i = 0; i < count; ++i) {
-    DTN_REQUIRE(tiles[i] > 0, DTN_ERR_INVALID, "paged attention plan: a sequence has at least one tile");
-    units += tiles[i] * heads;
+    DTN_REQUIRE(tiles[i] >= 0, DTN_ERR_INVALID, "paged attention plan: negative tiles");
+    units += tiles[i] > 0 ? (tiles[i] + PA_ITEM_UNITS) * heads : 0;
   }
-  const int64_t workers = pa_workers(units, min_units, grid);
+  const int64_t workers = units > 0 ? pa_workers(units, min_units, grid) : 0;
   if (workers_out) *workers_out = workers;
   if (begin_out)
-    for (int64_t c = 0; c <= workers; ++c) begin_out[c] = pa_share_begin(units, workers, c);
+    for (int64_t c = 0; c <= workers; ++c) begin_out[c] = workers > 0 ? pa_share_begin(units, workers, c) : 0;
   int64_t at = 0;
   for (int64_t i = 0; i < count * heads; ++i) {
-    if (first_out) first_out[i] = pa_share_owner(units, workers, at);
-    at += tiles[i / heads];
-    if (last_out) last_out[i] = pa_share_owner(units, workers, at - 1);
+    const int64_t here = tiles[i / heads];
+    if (first_out) first_out[i] = here > 0 ? pa_share_owner(units, workers, at) : -1;
+    if (last_out) last_out[i] = here > 0 ? pa_share_owner(units, workers, at + here - 1) : -1;
+    at += here > 0 ? here + PA_ITEM_UNITS : 0;
   }
   return DTN_OK;
 }
@@ -754,7 +872,8 @@ int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   p.out_head_stride = out_head_stride;
   p.page_stride = page_stride * element;
   p.page_head_stride = page_head_stride * element;
-  p.heads = (int)kv_heads;
+  p.kv_heads = (int)kv_heads;
+  p.q_heads = (int)q_heads;
   p.group = (int)(q_heads / kv_heads);
   p.dim = (int)dim;
   p.page_size = (int)page_size;
@@ -763,7 +882,9 @@ int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   p.scale_log2e = scale * 1.4426950408889634f;
   p.out_f32 = out_f32;
   p.q_pairs = element == 2 && aligned_to(q, 4) && q_token_stride % 2 == 0 && q_head_stride % 2 == 0;
-  p.min_units = 2;
+  const int64_t out_element = out_f32 ? 4 : element;
+  p.out_quads = aligned_to(out, 4 * out_element) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0;
+  p.min_units = 1 + PA_ITEM_UNITS;
   // position / page_size for positions below 2^31: mul = floor(2^(31 + s) / d) + 1 with 2^s >= d exceeds 2^(31 + s) / d by at
   // most 1, so the product exceeds the quotient by less than 2^31 / 2^(31 + s) <= 1 / d: the floor is exact. mul <= 2^32 - 1
   // needs d > 1; for d = 1 the multiplier is 1 and the shift 0.

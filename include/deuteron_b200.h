@@ -371,11 +371,11 @@ int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages,
 int dtn_paged_attention_workspace_bytes(size_t* bytes_out /* host */);
 
 /* How dtn_paged_attention cuts a batch among its blocks: host arithmetic only (the kernel does the same on the device from the
- * lengths). Sequence i has tiles[i] >= 1 tiles of tokens for each of `heads` items (kv heads x blocks of query heads); the
- * units, tile fastest, then item, then sequence, are cut into *workers_out contiguous ranges [begin_out[c],
- * begin_out[c + 1]), as many as `grid` allows with at least min_units each. first_out / last_out (count * heads entries) are
- * the blocks that hold an item's first and last unit; the parts of an item are added in that order. Output pointers may be
- * NULL; begin_out needs grid + 1 entries. */
+ * lengths). Sequence i has tiles[i] tiles of tokens for each of `heads` items (kv heads x blocks of query heads); an item has
+ * a unit for each of its tiles and two for its end, none without tiles. The units, tile fastest, then item, then sequence, are
+ * cut into *workers_out contiguous ranges [begin_out[c], begin_out[c + 1]), as many as `grid` allows with at least min_units
+ * each. first_out / last_out (count * heads entries) are the blocks that hold an item's first and last tile (-1 without tiles);
+ * the parts of an item are added in that order. Output pointers may be NULL; begin_out needs grid + 1 entries. */
 int dtn_paged_attention_plan(const int64_t* tiles /* host */, int64_t count, int64_t heads, int64_t min_units, int64_t grid,
                              int64_t* begin_out /* host */, int64_t* first_out /* host */, int64_t* last_out /* host */,
                              int64_t* workers_out /* host */);

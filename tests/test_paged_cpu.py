@@ -151,26 +151,32 @@ def test_attention_entry_refuses_alignment_and_workspace():
 
 def test_the_plan_covers_every_unit_once_and_names_its_owners():
     generator = random.Random(3)
-    cases = [([1], 1, 1, 1), ([1], 8, 2, 296), ([1000], 1, 2, 296), ([1, 1, 1], 1, 1, 2), ([2 ** 27], 8, 2, 296), ([5, 1, 700, 1, 33], 4, 2, 148)]
-    cases += [([generator.randint(1, 60) for _ in range(generator.randint(1, 40))], generator.randint(1, 9), generator.randint(1, 4), generator.randint(1, 300)) for _ in range(60)]
+    cases = [([1], 1, 1, 1), ([1], 8, 2, 296), ([1000], 1, 2, 296), ([1, 0, 1], 1, 1, 2), ([2 ** 27], 8, 2, 296), ([5, 1, 700, 0, 33], 4, 2, 148), ([0, 0], 3, 4, 9)]
+    cases += [([generator.randint(0, 60) for _ in range(generator.randint(1, 40))], generator.randint(1, 9), generator.randint(1, 4), generator.randint(1, 300)) for _ in range(60)]
     for tiles, heads, least, grid in cases:
         items = len(tiles) * heads
         begin, first, last, workers = ((ctypes.c_int64 * n)() for n in (grid + 1, items, items, 1))
         native.call('dtn_paged_attention_plan', (ctypes.c_int64 * len(tiles))(*tiles), len(tiles), heads, least, grid, begin, first, last, workers)
-        count, units = workers[0], sum(tiles) * heads
+        count, units = workers[0], sum(n + 2 for n in tiles if n) * heads
+        if not units:
+            assert count == 0 and set(first) == set(last) == {-1}
+            continue
         shares = [begin[c + 1] - begin[c] for c in range(count)]
         assert 1 <= count <= grid and begin[0] == 0 and begin[count] == units and max(shares) - min(shares) <= 1
         assert min(shares) >= least or count == 1
         at, started = 0, []
         for item in range(items):
+            if tiles[item // heads] == 0:
+                assert first[item] == last[item] == -1
+                continue
             end = at + tiles[item // heads]
             owners = [c for c in range(count) if begin[c] < end and begin[c + 1] > at]
             assert (first[item], last[item]) == (owners[0], owners[-1]) and owners == list(range(owners[0], owners[-1] + 1))
             if len(owners) > 1:
                 started.append(first[item])
-            at = end
+            at = end + 2
         assert len(set(started)) == len(started)          # one counter per block is enough: no two split items start in one block
-    assert native.lib().dtn_paged_attention_plan((ctypes.c_int64 * 1)(0), 1, 1, 1, 1, None, None, None, None) == native.ERR_INVALID
+    assert native.lib().dtn_paged_attention_plan((ctypes.c_int64 * 1)(-1), 1, 1, 1, 1, None, None, None, None) == native.ERR_INVALID
 
 
 def test_positions_are_divided_by_a_multiplication():
