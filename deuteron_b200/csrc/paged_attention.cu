@@ -60,6 +60,7 @@ struct PagedAttentionParams {
 
 // Units for the end of an item: the teams' parts are added, the result written, the next query taken.
 constexpr int PA_ITEM_UNITS = 2;
+constexpr int PA_JOIN = 16;
 
 // First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
 __host__ __device__ __forceinline__ int64_t pa_share_begin(int64_t units, int64_t workers, int64_t c) { return units * c / workers; }
@@ -147,6 +148,13 @@ __device__ __forceinline__ uint32_t pa_take(float& a, float& b, __nv_bfloat16) {
   a -= f.x;
   b -= f.y;
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Counts a block in; what its threads wrote before the barrier ahead of this is seen by whoever reads after the last arrival.
+__device__ __forceinline__ int pa_arrive(int* counter) {
+  int before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
 }
 
 // What is seen of a sequence: its row of the tables, its first token that is seen and how many.
@@ -370,10 +378,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
 
   // -- queries ------------------------------------------------------------------------------------
   constexpr int STEPS_K = DP / 16;
-  uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF ? STEPS_K : 1][2];
+  uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF && DP < 256 ? STEPS_K : 1][2];
   float* s_query = reinterpret_cast<float*>(smem + C::RING + C::MERGE);
   auto head_of = [&](int block, int h) { return block * C::HEADS + h; };   // within the group
-  auto load_query = [&](int64_t sequence, int kv_head, int block) {   // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
+  auto load_query = [&](uint32_t (&to)[C::HALF ? STEPS_K : 1][2], int64_t sequence, int kv_head, int block) {
+    // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
     const int h = head_of(block, member * 8 + g);
     const bool there = h < p.group;
     const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)kv_head * p.group + (there ? h : 0)) * p.q_head_stride;
@@ -389,12 +398,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           else
             v = *reinterpret_cast<const uint16_t*>(q + d) | (uint32_t) * reinterpret_cast<const uint16_t*>(q + d + 1) << 16;
         }
-        query_next[ks][half] = v;
+        to[ks][half] = v;
       }
     }
   };
   if (now.left <= 0) return;   // nothing but the ends of items
-  if constexpr (C::HALF) load_query(now.sequence, now.kv_head, now.block);
+  if constexpr (C::HALF && DP < 256) load_query(query_next, now.sequence, now.kv_head, now.block);
 
   // -- the pass over the tokens -------------------------------------------------------------------
   constexpr int COLUMNS = DP / 32;                 // FP32 storage: columns of V per lane
@@ -423,13 +432,15 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       for (int i = 0; i < (C::HALF ? DP / 16 : 8); ++i)
 #pragma unroll
         for (int j = 0; j < (C::HALF ? 4 : COLUMNS); ++j) acc[i][j] = 0.f;
-      if constexpr (C::HALF) {
+      if constexpr (C::HALF && DP == 256) {
+        load_query(query, now.sequence, now.kv_head, now.block);   // registers for one item's query only
+      } else if constexpr (C::HALF) {
 #pragma unroll
         for (int ks = 0; ks < STEPS_K; ++ks) query[ks][0] = query_next[ks][0], query[ks][1] = query_next[ks][1];
         PaCursor<UNIT> next = now;   // the next item's, a whole item ahead
         next.left -= now.tiles - now.tile;
         next.next_item(p);
-        if (next.left > 0) load_query(next.sequence, next.kv_head, next.block);
+        if (next.left > 0) load_query(query_next, next.sequence, next.kv_head, next.block);
       } else {
         __syncthreads();
         for (int i = tid; i < C::HEADS * DP; i += THREADS) {
@@ -617,7 +628,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           now.tile = start;
           ahead = now;
           fill();
-          load_query(now.sequence, now.kv_head, now.block);
+          if constexpr (DP < 256) load_query(query_next, now.sequence, now.kv_head, now.block);
           exactly = fresh = true;
           slot = 0;
           continue;
@@ -703,38 +714,50 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       if (!whole) {
         const int64_t item = end - now.left - now.tile;   // the item's first unit
         const int64_t first = pa_share_owner(units, workers, item), last = pa_share_owner(units, workers, item + now.tiles - 1);
-        __threadfence();
         __syncthreads();
-        if (tid == 0) s_last = atomicAdd(p.counters + first, 1) == (int)(last - first);
+        if (tid == 0) s_last = pa_arrive(p.counters + first) == (int)(last - first);
         __syncthreads();
         if (s_last) {
-          __threadfence();
           if (tid == 0) p.counters[first] = 0;
           // the parts, added in the order of the blocks: the first block's second part, every other's first
           const int count = (int)(last - first) + 1;
           const float* parts = p.parts + (first * 2 + 1) * C::PART;
           auto part_of = [&](int n) { return parts + (n == 0 ? 0 : (int64_t)(2 * n - 1) * C::PART); };
+#pragma unroll 1
           for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
             const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.block, slot_head);
             if (h >= p.group || d >= p.dim) continue;
-            float high = NONE;
-#pragma unroll 8
-            for (int n = 0; n < count; ++n) high = fmaxf(high, __ldcg(part_of(n) + C::HEADS * DP + slot_head));
-            const float around = high == NONE ? 0.f : high;
-            float4 value = make_float4(0.f, 0.f, 0.f, 0.f);
-            float weight_sum = 0.f;
-#pragma unroll 8
-            for (int n = 0; n < count; ++n) {
-              const float* from = part_of(n);
-              const float weight = ex2_approx_ftz(__ldcg(from + C::HEADS * DP + slot_head) - around);
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(from + slot_head * DP + d));
-              weight_sum = fmaf(weight, __ldcg(from + C::HEADS * DP + C::HEADS + slot_head), weight_sum);
-              value.x = fmaf(weight, v.x, value.x);
-              value.y = fmaf(weight, v.y, value.y);
-              value.z = fmaf(weight, v.z, value.z);
-              value.w = fmaf(weight, v.w, value.w);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            float high = NONE, sum_p = 0.f;
+#pragma unroll 1
+            for (int n = 0; n < count; n += PA_JOIN) {   // PA_JOIN parts requested at once; past the last one nothing
+              float4 x[PA_JOIN];
+              float part_high[PA_JOIN], part_sum[PA_JOIN], up = high;
+#pragma unroll
+              for (int j = 0; j < PA_JOIN; ++j) {
+                part_high[j] = NONE;
+                part_sum[j] = 0.f;
+                x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (n + j < count) {
+                  const float* from = part_of(n + j);
+                  part_high[j] = __ldcg(from + C::HEADS * DP + slot_head);
+                  part_sum[j] = __ldcg(from + C::HEADS * DP + C::HEADS + slot_head);
+                  x[j] = __ldcg(reinterpret_cast<const float4*>(from + slot_head * DP + d));
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < PA_JOIN; ++j) up = fmaxf(up, part_high[j]);
+              const float around = up == NONE ? 0.f : up, before_weight = ex2_approx_ftz(high - around);
+              high = up;
+              y.x *= before_weight, y.y *= before_weight, y.z *= before_weight, y.w *= before_weight, sum_p *= before_weight;
+#pragma unroll
+              for (int j = 0; j < PA_JOIN; ++j) {
+                const float weight = ex2_approx_ftz(part_high[j] - around);
+                y.x = fmaf(weight, x[j].x, y.x), y.y = fmaf(weight, x[j].y, y.y), y.z = fmaf(weight, x[j].z, y.z), y.w = fmaf(weight, x[j].w, y.w);
+                sum_p = fmaf(weight, part_sum[j], sum_p);
+              }
             }
-            write(h, d, make_float4(value.x / weight_sum, value.y / weight_sum, value.z / weight_sum, value.w / weight_sum));
+            write(h, d, make_float4(y.x / sum_p, y.y / sum_p, y.z / sum_p, y.w / sum_p));
           }
         }
       }
