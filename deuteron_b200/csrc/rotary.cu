@@ -46,8 +46,8 @@ __device__ __forceinline__ int64_t position_of(const RotaryParams& p, int64_t to
 }
 
 // amplitude * (cos, sin) of position * frequency.
-__device__ __forceinline__ float2 turn(const RotaryParams& p, int64_t position, int pair) {
-  const double turns = (double)position * p.frequencies[pair] * 0.15915494309189533577;   // 1 / (2 pi)
+__device__ __forceinline__ float2 turn(const RotaryParams& p, double position, int pair) {
+  const double turns = position * p.frequencies[pair] * 0.15915494309189533577;   // 1 / (2 pi)
   const float half_turns = (float)(2.0 * (turns - rint(turns)));
   float s, c;
   sincospif(half_turns, &s, &c);
@@ -72,275 +72,261 @@ __device__ __forceinline__ int64_t page_offset(const RotaryParams& p, int64_t to
   return page * p.page_stride + (position - index * p.page_size) * p.dim;
 }
 
-// How the work is laid out: a block has `tokens` tokens and `heads` heads (counted over queries, keys, values), a head `units`
-// units. The multipliers divide small numbers: n / d = umulhi(n, ceil(2^32 / d)) while n * d < 2^32.
-struct RotaryLayout {
-  int tokens, heads, units;
-  uint32_t units_mul, heads_mul;
-};
-
-__device__ __forceinline__ int small_divide(int n, int d, uint32_t mul) { return d == 1 ? n : (int)__umulhi((uint32_t)n, mul); }
-
-// Where head `head` of a token is read.
-template <typename T>
-__device__ __forceinline__ const T* head_source(const RotaryParams& p, int64_t token, int head) {
-  if (head < p.q.heads) return static_cast<const T*>(p.q.src) + token * p.q.token_stride + head * p.q.head_stride;
-  head -= p.q.heads;
-  if (head < p.k.heads) return static_cast<const T*>(p.k.src) + token * p.k.token_stride + head * p.k.head_stride;
-  head -= p.k.heads;
-  return static_cast<const T*>(p.v.src) + token * p.v.token_stride + head * p.v.head_stride;
-}
-// Where it is written (offset: the token's place in the pools, or -1); null: nowhere. Values are not rotated.
-template <typename T>
-__device__ __forceinline__ T* head_target(const RotaryParams& p, int64_t token, int head, int64_t offset, bool& rotated) {
-  rotated = true;
-  if (head < p.q.heads) return static_cast<T*>(p.q_out) + token * p.q_out_token_stride + head * p.q_out_head_stride;
-  if (offset < 0) return nullptr;
-  head -= p.q.heads;
-  if (head < p.k.heads) return static_cast<T*>(p.k_pages) + offset + head * p.page_head_stride;
-  rotated = false;
-  return static_cast<T*>(p.v_pages) + offset + (head - p.k.heads) * p.page_head_stride;
-}
-
-constexpr int R_THREADS = 256;
-constexpr int R_TURNS = 512;      // cosines and sines a block holds: tokens per block x pairs
-constexpr int R_MAX_TOKENS = 64;  // per block
-constexpr int R_AHEAD = 2;        // units a thread has in flight
-
-// Whole 16-byte vectors on both sides of every pair. A unit is the two vectors that hold the halves of VECTOR pairs (half
-// layout) or one vector of whole pairs (interleaved), or one vector that is copied; the pairs of a unit are in one thread,
-// so out may be x itself. A block's first loads are issued before its angles are formed.
-//
-// 16384 tokens x 40 heads x 128 bf16 (336 MB, 51.3 us at the copy rate): see the table of measured times.
-template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(R_THREADS) rotary_vector_kernel(const RotaryParams p, const RotaryLayout l) {
-  constexpr int VECTOR = 16 / (int)sizeof(T);
-  __shared__ __align__(16) float cosines[R_TURNS], sines[R_TURNS];
-  __shared__ int64_t places[R_MAX_TOKENS];
-  const int64_t token0 = (int64_t)blockIdx.x * l.tokens;
-  const int tokens = (int)(p.tokens - token0 < l.tokens ? p.tokens - token0 : l.tokens);
-  const int all_heads = p.q.heads + p.k.heads + p.v.heads, head0 = blockIdx.y * l.heads;
-  const int heads = all_heads - head0 < l.heads ? all_heads - head0 : l.heads;
-  const int total = tokens * l.heads * l.units, turned = INTERLEAVED ? 0 : p.pairs / VECTOR;
-
-  struct Unit {
-    int token, head, unit;
-    uint4 a, b;
-  } units[R_AHEAD];
-  auto find = [&](Unit& u, int flat) {
-    const int row = small_divide(flat, l.units, l.units_mul);
-    u.unit = flat - row * l.units;
-    u.token = small_divide(row, l.heads, l.heads_mul);
-    u.head = row - u.token * l.heads;
-    if (flat >= total || u.head >= heads) u.token = -1;
-  };
-  auto load = [&](Unit& u) {
-    if (u.token < 0) return;
-    const T* src = head_source<T>(p, token0 + u.token, head0 + u.head);
-    if (!INTERLEAVED && u.unit < turned) {
-      u.a = *reinterpret_cast<const uint4*>(src + u.unit * VECTOR);
-      u.b = *reinterpret_cast<const uint4*>(src + p.pairs + u.unit * VECTOR);
-    } else {
-      u.a = *reinterpret_cast<const uint4*>(src + (INTERLEAVED ? u.unit : u.unit + turned) * VECTOR);
-    }
-  };
-  auto store = [&](Unit& u) {
-    if (u.token < 0) return;
-    bool rotated;
-    T* dst = head_target<T>(p, token0 + u.token, head0 + u.head, places[u.token], rotated);
-    if (dst == nullptr) return;
-    T* a = reinterpret_cast<T*>(&u.a);
-    if (INTERLEAVED) {
-      if (rotated && u.unit * VECTOR < 2 * p.pairs) {
-        const float* c = cosines + u.token * p.pairs + u.unit * (VECTOR / 2);
-        const float* s = sines + u.token * p.pairs + u.unit * (VECTOR / 2);
-#pragma unroll
-        for (int i = 0; i < VECTOR / 2; ++i) {
-          const float x = to_float(a[2 * i]), y = to_float(a[2 * i + 1]);
-          a[2 * i] = from_float<T>(fmaf(x, c[i], -y * s[i]));
-          a[2 * i + 1] = from_float<T>(fmaf(y, c[i], x * s[i]));
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + u.unit * VECTOR) = u.a;
-    } else if (u.unit < turned) {
-      T* b = reinterpret_cast<T*>(&u.b);
-      if (rotated) {
-        const float4* c4 = reinterpret_cast<const float4*>(cosines + u.token * p.pairs + u.unit * VECTOR);
-        const float4* s4 = reinterpret_cast<const float4*>(sines + u.token * p.pairs + u.unit * VECTOR);
-#pragma unroll
-        for (int i = 0; i < VECTOR / 4; ++i) {
-          const float4 cv = c4[i], sv = s4[i];
-          const float c[4] = {cv.x, cv.y, cv.z, cv.w}, s[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = to_float(a[4 * i + j]), y = to_float(b[4 * i + j]);
-            a[4 * i + j] = from_float<T>(fmaf(x, c[j], -y * s[j]));
-            b[4 * i + j] = from_float<T>(fmaf(y, c[j], x * s[j]));
-          }
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + u.unit * VECTOR) = u.a;
-      *reinterpret_cast<uint4*>(dst + p.pairs + u.unit * VECTOR) = u.b;
-    } else {
-      *reinterpret_cast<uint4*>(dst + (u.unit + turned) * VECTOR) = u.a;
-    }
-  };
-
-#pragma unroll
-  for (int i = 0; i < R_AHEAD; ++i) {
-    find(units[i], threadIdx.x + i * R_THREADS);
-    load(units[i]);
-  }
-  for (int i = threadIdx.x; i < tokens * p.pairs; i += R_THREADS) {
-    const int t = i / p.pairs;
-    const float2 cs = turn(p, position_of(p, token0 + t), i - t * p.pairs);
-    cosines[i] = cs.x;
-    sines[i] = cs.y;
-  }
-  if ((int)threadIdx.x < tokens) places[threadIdx.x] = p.k.heads > 0 ? page_offset(p, token0 + threadIdx.x) : -1;
-  __syncthreads();
-  for (int base = 0; base < total; base += R_AHEAD * R_THREADS) {
-    if (base > 0) {
-#pragma unroll
-      for (int i = 0; i < R_AHEAD; ++i) {
-        find(units[i], base + threadIdx.x + i * R_THREADS);
-        load(units[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < R_AHEAD; ++i) store(units[i]);
-  }
-}
-
-// Any number of pairs, any alignment: rows of heads are staged in shared memory, by 16-byte vectors where the rows allow it
-// (WIDE), and each thread writes what it staged with the partners read from there. A pass holds whole rows and reads all of
-// them before it writes any.
 constexpr int R_MAX_DIM = 1024;
+constexpr int R_THREADS = 256;
+constexpr int R_FILL = 8192;   // threads per SM wanted of a launch
 
-template <typename T, bool INTERLEAVED, bool WIDE>
-__global__ void __launch_bounds__(R_THREADS) rotary_staged_kernel(const RotaryParams p, const RotaryLayout l) {
-  constexpr int VECTOR = WIDE ? 16 / (int)sizeof(T) : 1, EACH = WIDE ? R_AHEAD : 8, CAPACITY = EACH * R_THREADS;
-  __shared__ float2 turns[R_TURNS];
-  __shared__ __align__(16) T staged[CAPACITY * VECTOR];
-  __shared__ int64_t places[R_MAX_TOKENS];
-  const int64_t token0 = (int64_t)blockIdx.x * l.tokens;
-  const int tokens = (int)(p.tokens - token0 < l.tokens ? p.tokens - token0 : l.tokens);
-  const int all_heads = p.q.heads + p.k.heads + p.v.heads, head0 = blockIdx.y * l.heads;
-  const int heads = all_heads - head0 < l.heads ? all_heads - head0 : l.heads;
-  const int rows = tokens * l.heads, rows_of_pass = CAPACITY / l.units;   // a unit is one vector here
-  for (int i = threadIdx.x; i < tokens * p.pairs; i += R_THREADS) {
-    const int t = i / p.pairs;
-    turns[i] = turn(p, position_of(p, token0 + t), i - t * p.pairs);
-  }
-  if ((int)threadIdx.x < tokens) places[threadIdx.x] = p.k.heads > 0 ? page_offset(p, token0 + threadIdx.x) : -1;
-  __syncthreads();
-  for (int first = 0; first < rows; first += rows_of_pass) {
+// V elements in one access.
+template <int BYTES> struct Access;
+template <> struct Access<16> { using type = uint4; };
+template <> struct Access<8> { using type = uint2; };
+template <> struct Access<4> { using type = uint32_t; };
+template <> struct Access<2> { using type = uint16_t; };
+
+// A thread keeps one unit of one token: it forms the angles of its pairs once, in registers, and walks over a range of heads
+// of one stream with them, so the 64-bit work is done once per token and pair and slice of heads. A unit is the two accesses of
+// V elements that hold the halves of V pairs (TWO), or one access of whole pairs (interleaved), or one access that is copied;
+// neighbouring threads have neighbouring units, so the accesses of a warp are whole lines whatever V is. The pairs of a unit
+// are in one thread and the loads of a head precede its stores, so out may be x itself. The loads of the first heads are
+// issued before the angles are formed and before a key or value's page is looked up.
+//
+// Bound by memory. V is the widest that divides the head, its strides and addresses and, in the half layout, the number of
+// pairs: 16 bytes in practice, one element for an odd number of pairs. Measured (one element against a form that staged heads
+// in shared memory by 16-byte vectors): see the launch below.
+template <typename T, bool TWO, int V>
+__global__ void __launch_bounds__(R_THREADS) rotary_kernel(const RotaryParams p, const int interleaved, const int units, const int tokens_per_block,
+                                                           const int heads_per_thread, const int q_slices, const int k_slices) {
+  using Word = typename Access<V * (int)sizeof(T)>::type;
+  constexpr int WORDS = TWO ? 2 : 1, PAIRS = TWO ? V : V / 2, AHEAD = 4;
+  const int width = units < R_THREADS ? units : R_THREADS, local = threadIdx.x / width, unit = threadIdx.x - local * width + blockIdx.z * R_THREADS;
+  const int64_t token = (int64_t)blockIdx.x * tokens_per_block + local;
+  if (local >= tokens_per_block || token >= p.tokens || unit >= units) return;
+  int slice = blockIdx.y;
+  const bool query = slice < q_slices, key = !query && slice < q_slices + k_slices;
+  slice -= query ? 0 : (key ? q_slices : q_slices + k_slices);
+  const HeadStream& from = query ? p.q : (key ? p.k : p.v);
+  const int head0 = slice * heads_per_thread, heads = from.heads - head0 < heads_per_thread ? from.heads - head0 : heads_per_thread;
+  // the unit's first column, how far its pairs' other halves are and how many of its pairs are turned
+  const int turned = TWO ? p.pairs / V : 0;
+  const bool two = TWO && unit < turned;
+  const int other = interleaved ? 1 : p.pairs;   // TWO and interleaved only with V = 1: elements that cannot be moved in pairs
+  const int column = !TWO ? unit * V : (two ? (interleaved ? 2 * unit : unit * V) : (unit + turned) * V);
+  const int left = TWO ? (two ? PAIRS : 0) : p.pairs - unit * PAIRS, turning = query || key ? left : 0;
+  const T* src = static_cast<const T*>(from.src) + token * from.token_stride + head0 * from.head_stride + column;
+
+  Word x[AHEAD][WORDS];
+  auto load = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int flat = threadIdx.x + i * R_THREADS, row = small_divide(flat, l.units, l.units_mul), unit = flat - row * l.units;
-      const int token = small_divide(first + row, l.heads, l.heads_mul), head = first + row - token * l.heads;
-      if (row >= rows_of_pass || first + row >= rows || head >= heads) continue;
-      const T* src = head_source<T>(p, token0 + token, head0 + head) + unit * VECTOR;
-      if (WIDE)
-        *reinterpret_cast<uint4*>(staged + flat * VECTOR) = *reinterpret_cast<const uint4*>(src);
-      else
-        staged[flat] = *src;
+    for (int i = 0; i < AHEAD; ++i)
+      if (h + i < heads) {
+        x[i][0] = *reinterpret_cast<const Word*>(src + (h + i) * from.head_stride);
+        if (TWO && two) x[i][WORDS - 1] = *reinterpret_cast<const Word*>(src + (h + i) * from.head_stride + other);
+      }
+  };
+  load(0);
+  float c[PAIRS], s[PAIRS];
+  if (turning > 0) {
+    const double position = (double)position_of(p, token);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i)
+      if (i < turning) {
+        const float2 cs = turn(p, position, unit * PAIRS + i);
+        c[i] = cs.x;
+        s[i] = cs.y;
+      }
+  }
+  T* dst;
+  int64_t head_stride;
+  if (query) {
+    dst = static_cast<T*>(p.q_out) + token * p.q_out_token_stride + head0 * p.q_out_head_stride + column;
+    head_stride = p.q_out_head_stride;
+  } else {
+    const int64_t offset = page_offset(p, token);
+    if (offset < 0) return;
+    dst = static_cast<T*>(key ? p.k_pages : p.v_pages) + offset + head0 * p.page_head_stride + column;
+    head_stride = p.page_head_stride;
+  }
+  for (int h = 0; h < heads; h += AHEAD) {
+    if (h > 0) load(h);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (h + i >= heads) break;
+      T* a = reinterpret_cast<T*>(&x[i][0]);
+      T* b = reinterpret_cast<T*>(&x[i][WORDS - 1]);
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+        if (j < turning) {
+          T& first = TWO ? a[j] : a[2 * j];
+          T& second = TWO ? b[j] : a[2 * j + 1];
+          const float u = to_float(first), v = to_float(second);
+          first = from_float<T>(fmaf(u, c[j], -v * s[j]));
+          second = from_float<T>(fmaf(v, c[j], u * s[j]));
+        }
+      *reinterpret_cast<Word*>(dst + (h + i) * head_stride) = x[i][0];
+      if (TWO && two) *reinterpret_cast<Word*>(dst + (h + i) * head_stride + other) = x[i][WORDS - 1];
     }
+  }
+}
+
+// The heads are cut into slices of one stream until the card has `fill` threads per SM (a thread per head for a handful of
+// tokens), each of at least the heads that a thread has in flight while the tokens alone give the card a block per SM.
+static int64_t rotary_heads_per_thread(const RotaryParams& p, int units, int ahead, int64_t fill) {
+  const int64_t heads = p.q.heads + p.k.heads + p.v.heads, threads = p.tokens * units, slices = fill * sm_count() / threads + 1;
+  int64_t each = (heads + slices - 1) / slices;
+  if (each > ahead || threads >= (int64_t)R_THREADS * sm_count()) each = (each + ahead - 1) / ahead * ahead;
+  return each;
+}
+
+template <typename T, bool TWO, int V>
+static int rotary_launch_v(const RotaryParams& p, int interleaved, cudaStream_t s) {
+  const int units = (TWO ? p.dim - p.pairs : p.dim) / V, width = units < R_THREADS ? units : R_THREADS, tokens = R_THREADS / width;
+  const int64_t each = rotary_heads_per_thread(p, units, 4, R_FILL);
+  const int64_t q_slices = (p.q.heads + each - 1) / each, k_slices = (p.k.heads + each - 1) / each;
+  DTN_REQUIRE(q_slices + 2 * k_slices < 65536, DTN_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
+  const dim3 grid((unsigned)((p.tokens + tokens - 1) / tokens), (unsigned)(q_slices + 2 * k_slices), (unsigned)((units + R_THREADS - 1) / R_THREADS));
+  rotary_kernel<T, TWO, V><<<grid, tokens * width, 0, s>>>(p, interleaved, units, tokens, (int)each, (int)q_slices, (int)k_slices);
+  DTN_LAUNCH_CHECK("rotary_kernel");
+  return DTN_OK;
+}
+
+// Half layout, heads of whole 16-byte vectors, pairs that are not: a thread keeps one vector of one token and takes the other
+// halves of its elements' pairs from shared memory, where every thread of the head puts its vector: two vectors, out of
+// which OFF = pairs % V elements are shifted (a constant, so the shift costs no instruction or one per word). Between two
+// barriers all loads of R_SHARED heads precede their stores, and a head's threads are in one block, so out may be x itself.
+constexpr int R_SHARED = 4, R_FILL_SHARED = 4096;
+
+template <typename T, int OFF>
+__global__ void __launch_bounds__(R_THREADS) rotary_shared_kernel(const RotaryParams p, const int units, const int tokens_per_block, const int heads_per_thread,
+                                                                  const int q_slices, const int k_slices) {
+  constexpr int V = 16 / (int)sizeof(T);
+  __shared__ __align__(16) T staged[R_SHARED][R_THREADS * V];
+  const int local = threadIdx.x / units, unit = threadIdx.x - local * units;
+  const int64_t token = (int64_t)blockIdx.x * tokens_per_block + local;
+  const bool there = token < p.tokens;
+  int slice = blockIdx.y;
+  const bool query = slice < q_slices, key = !query && slice < q_slices + k_slices;
+  slice -= query ? 0 : (key ? q_slices : q_slices + k_slices);
+  const HeadStream& from = query ? p.q : (key ? p.k : p.v);
+  const int head0 = slice * heads_per_thread, heads = from.heads - head0 < heads_per_thread ? from.heads - head0 : heads_per_thread;
+  const int column = unit * V;
+  // elements of the vector that are first halves, and that are turned at all
+  const int whole = p.pairs / V, firsts = p.pairs - column, turning = there && (query || key) ? 2 * p.pairs - column : 0;
+  const T* src = static_cast<const T*>(from.src) + token * from.token_stride + head0 * from.head_stride + column;
+
+  uint4 x[R_SHARED];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < R_SHARED; ++i)
+      if (there && h + i < heads) x[i] = *reinterpret_cast<const uint4*>(src + (h + i) * from.head_stride);
+  };
+  load(0);
+  float c[V], s[V];
+  if (turning > 0) {
+    const double position = (double)position_of(p, token);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < turning) {
+        const float2 cs = turn(p, position, e < firsts ? column + e : column + e - p.pairs);
+        c[e] = cs.x;
+        s[e] = e < firsts ? -cs.y : cs.y;
+      }
+  }
+  T* dst = nullptr;
+  int64_t head_stride = 0;
+  if (there && query) {
+    dst = static_cast<T*>(p.q_out) + token * p.q_out_token_stride + head0 * p.q_out_head_stride + column;
+    head_stride = p.q_out_head_stride;
+  } else if (there) {
+    const int64_t offset = page_offset(p, token);
+    if (offset >= 0) dst = static_cast<T*>(key ? p.k_pages : p.v_pages) + offset + head0 * p.page_head_stride + column;
+    head_stride = p.page_head_stride;
+  }
+  for (int h = 0; h < heads; h += R_SHARED) {
+    if (h > 0) load(h);
+#pragma unroll
+    for (int i = 0; i < R_SHARED; ++i)
+      if (there && h + i < heads) *reinterpret_cast<uint4*>(&staged[i][threadIdx.x * V]) = x[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int flat = threadIdx.x + i * R_THREADS, row = small_divide(flat, l.units, l.units_mul), unit = flat - row * l.units;
-      const int token = small_divide(first + row, l.heads, l.heads_mul), head = first + row - token * l.heads;
-      if (row >= rows_of_pass || first + row >= rows || head >= heads) continue;
-      bool rotated;
-      T* dst = head_target<T>(p, token0 + token, head0 + head, places[token], rotated);
-      if (dst == nullptr) continue;
-      const T* line = staged + row * l.units * VECTOR;
-      const float2* line_turns = turns + token * p.pairs;
-      __align__(16) T out[VECTOR];
-#pragma unroll
-      for (int e = 0; e < VECTOR; ++e) {
-        const int d = unit * VECTOR + e;
-        out[e] = line[d];
-        if (rotated && d < 2 * p.pairs) {
-          const bool is_first = INTERLEAVED ? d % 2 == 0 : d < p.pairs;
-          const int pair = INTERLEAVED ? d / 2 : (is_first ? d : d - p.pairs), partner = INTERLEAVED ? d ^ 1 : (is_first ? d + p.pairs : pair);
-          const float x = to_float(out[e]), y = to_float(line[partner]);
-          const float2 cs = line_turns[pair];
-          out[e] = from_float<T>(is_first ? fmaf(x, cs.x, -y * cs.y) : fmaf(x, cs.x, y * cs.y));
+    for (int i = 0; i < R_SHARED; ++i) {
+      if (h + i >= heads || dst == nullptr) break;
+      T* a = reinterpret_cast<T*>(&x[i]);
+      if (turning > 0) {
+        const uint4* line = reinterpret_cast<const uint4*>(staged[i]) + local * units;
+        uint4 up[2], down[2];   // the second halves of first ones, the first halves of second ones
+        if (firsts > 0) {
+          up[0] = line[unit + whole];
+          up[1] = line[unit + whole + 1 < units ? unit + whole + 1 : units - 1];   // past the head: not used
         }
+        if (firsts < V) {
+          down[0] = line[unit - whole - 1 > 0 ? unit - whole - 1 : 0];             // before the head: not used
+          down[1] = line[unit - whole];
+        }
+        const T* up_at = reinterpret_cast<const T*>(up) + OFF;
+        const T* down_at = reinterpret_cast<const T*>(down) + V - OFF;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < turning) a[e] = from_float<T>(fmaf(to_float(a[e]), c[e], to_float(e < firsts ? up_at[e] : down_at[e]) * s[e]));
       }
-      if (WIDE)
-        *reinterpret_cast<uint4*>(dst + unit * VECTOR) = *reinterpret_cast<const uint4*>(out);
-      else
-        dst[unit] = out[0];
+      *reinterpret_cast<uint4*>(dst + (h + i) * head_stride) = x[i];
     }
     __syncthreads();
   }
 }
 
-// Tokens and heads per block. Many tokens: as many per block as share the work of R_TURNS angles and still leave several
-// blocks per SM. Few: one, its heads cut so that the card is not left to a handful of blocks.
-static RotaryLayout rotary_layout(const RotaryParams& p, int units, int per_pass, dim3& grid) {
-  RotaryLayout l = {};
-  const int64_t heads = p.q.heads + p.k.heads + p.v.heads, target = 4 * (int64_t)sm_count();
-  int64_t tokens = p.pairs > 0 ? R_TURNS / p.pairs : R_MAX_TOKENS;
-  tokens = tokens < 1 ? 1 : (tokens > R_MAX_TOKENS ? R_MAX_TOKENS : tokens);
-  if (tokens > p.tokens / target) tokens = p.tokens / target < 1 ? 1 : p.tokens / target;
-  int64_t cut = heads;
-  const int64_t fill = (per_pass + units - 1) / units, wanted = p.tokens < target ? target / p.tokens : 1;   // heads of one pass; blocks per token
-  if (wanted > 1) cut = (heads + wanted - 1) / wanted;
-  if (cut < fill) cut = fill;
-  if (cut > heads) cut = heads;
-  const int64_t most = 32768 / units;   // units <= 1024: a block's numbers of units and rows stay below 2^16, their products with a divisor below 2^32
-  if (cut > most) cut = most;
-  if (tokens * cut > most) tokens = most / cut;
-  l.tokens = (int)tokens;
-  l.heads = (int)cut;
-  l.units = units;
-  l.units_mul = (uint32_t)(((1ULL << 32) + units - 1) / units);
-  l.heads_mul = (uint32_t)(((1ULL << 32) + cut - 1) / cut);
-  grid = dim3((unsigned)((p.tokens + tokens - 1) / tokens), (unsigned)((heads + cut - 1) / cut));
-  return l;
+template <typename T, int OFF>
+static int rotary_launch_shared(const RotaryParams& p, cudaStream_t s) {
+  const int units = p.dim * (int)sizeof(T) / 16, tokens = R_THREADS / units;
+  const int64_t each = rotary_heads_per_thread(p, units, R_SHARED, R_FILL_SHARED);
+  const int64_t q_slices = (p.q.heads + each - 1) / each, k_slices = (p.k.heads + each - 1) / each;
+  DTN_REQUIRE(q_slices + 2 * k_slices < 65536, DTN_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
+  const dim3 grid((unsigned)((p.tokens + tokens - 1) / tokens), (unsigned)(q_slices + 2 * k_slices));
+  rotary_shared_kernel<T, OFF><<<grid, tokens * units, 0, s>>>(p, units, tokens, (int)each, (int)q_slices, (int)k_slices);
+  DTN_LAUNCH_CHECK("rotary_shared_kernel");
+  return DTN_OK;
 }
 
 template <typename T>
 static int rotary_launch_t(const RotaryParams& p, int interleaved, cudaStream_t s) {
-  constexpr int VECTOR = 16 / (int)sizeof(T);
-  auto wide = [](const HeadStream& h, const void* base) {
-    return h.heads == 0 || (aligned_to(base, 16) && h.token_stride % VECTOR == 0 && h.head_stride % VECTOR == 0);
+  // elements that every head's address and extent and, in the half layout, the distance within a pair are multiples of
+  uint64_t common = (uint64_t)p.dim;
+  auto add = [&](const void* base, int64_t token_stride, int64_t head_stride, int heads) {
+    if (heads > 0) common |= (reinterpret_cast<uintptr_t>(base) / sizeof(T)) | (uint64_t)token_stride | (uint64_t)head_stride;
   };
-  const HeadStream q_target = {p.q_out, p.q_out_token_stride, p.q_out_head_stride, p.q.heads};
-  const HeadStream pages = {p.k_pages, p.page_stride, p.page_head_stride, p.k.heads};
-  const bool vectors = p.dim % VECTOR == 0 && wide(p.q, p.q.src) && wide(p.k, p.k.src) && wide(p.v, p.v.src) && wide(q_target, p.q_out) &&
-                       wide(pages, p.k_pages) && wide(pages, p.v_pages);
-  const bool whole = vectors && (interleaved ? 2 * p.pairs : p.pairs) % VECTOR == 0;
-  dim3 grid;
-  if (whole) {
-    const int units = interleaved ? p.dim / VECTOR : (p.dim - p.pairs) / VECTOR;
-    const RotaryLayout l = rotary_layout(p, units, R_AHEAD * R_THREADS, grid);
-    DTN_REQUIRE(grid.y < 65536, DTN_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
-    if (interleaved)
-      rotary_vector_kernel<T, true><<<grid, R_THREADS, 0, s>>>(p, l);
-    else
-      rotary_vector_kernel<T, false><<<grid, R_THREADS, 0, s>>>(p, l);
-  } else if (vectors) {
-    const RotaryLayout l = rotary_layout(p, p.dim / VECTOR, R_AHEAD * R_THREADS, grid);
-    DTN_REQUIRE(grid.y < 65536, DTN_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
-    if (interleaved)
-      rotary_staged_kernel<T, true, true><<<grid, R_THREADS, 0, s>>>(p, l);
-    else
-      rotary_staged_kernel<T, false, true><<<grid, R_THREADS, 0, s>>>(p, l);
-  } else {
-    const RotaryLayout l = rotary_layout(p, p.dim, 8 * R_THREADS, grid);
-    DTN_REQUIRE(grid.y < 65536, DTN_ERR_UNSUPPORTED, "rotary: too many heads for one launch");
-    if (interleaved)
-      rotary_staged_kernel<T, true, false><<<grid, R_THREADS, 0, s>>>(p, l);
-    else
-      rotary_staged_kernel<T, false, false><<<grid, R_THREADS, 0, s>>>(p, l);
+  add(p.q.src, p.q.token_stride, p.q.head_stride, p.q.heads);
+  add(p.q_out, p.q_out_token_stride, p.q_out_head_stride, p.q.heads);
+  add(p.k.src, p.k.token_stride, p.k.head_stride, p.k.heads);
+  add(p.v.src, p.v.token_stride, p.v.head_stride, p.v.heads);
+  add(p.k_pages, p.page_stride, p.page_head_stride, p.k.heads);
+  add(p.v_pages, p.page_stride, p.page_head_stride, p.v.heads);
+  constexpr int WHOLE = 16 / (int)sizeof(T);
+  if (common % WHOLE == 0) {
+    if (interleaved) return rotary_launch_v<T, false, WHOLE>(p, 1, s);
+    if (p.pairs % WHOLE == 0) return rotary_launch_v<T, true, WHOLE>(p, 0, s);
+    if constexpr (WHOLE == 8) {
+      switch (p.pairs % 8) {
+        case 1: return rotary_launch_shared<T, 1>(p, s);
+        case 2: return rotary_launch_shared<T, 2>(p, s);
+        case 3: return rotary_launch_shared<T, 3>(p, s);
+        case 5: return rotary_launch_shared<T, 5>(p, s);
+        case 6: return rotary_launch_shared<T, 6>(p, s);
+        case 7: return rotary_launch_shared<T, 7>(p, s);
+        default: return rotary_launch_shared<T, 4>(p, s);
+      }
+    } else {
+      switch (p.pairs % 4) {
+        case 1: return rotary_launch_shared<T, 1>(p, s);
+        case 2: return rotary_launch_shared<T, 2>(p, s);
+        default: return rotary_launch_shared<T, 3>(p, s);
+      }
+    }
   }
-  DTN_LAUNCH_CHECK("rotary kernel");
-  return DTN_OK;
+  if (!interleaved) common |= (uint64_t)p.pairs;
+  if constexpr (sizeof(T) == 2) {
+    if (common % 4 == 0) return interleaved ? rotary_launch_v<T, false, 4>(p, 1, s) : rotary_launch_v<T, true, 4>(p, 0, s);
+  }
+  if (common % 2 == 0) return interleaved ? rotary_launch_v<T, false, 2>(p, 1, s) : rotary_launch_v<T, true, 2>(p, 0, s);
+  return rotary_launch_v<T, true, 1>(p, interleaved, s);
 }
 
 static int rotary_launch(const RotaryParams& p, int interleaved, int storage, cudaStream_t s) {
