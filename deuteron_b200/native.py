@@ -125,7 +125,9 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    status = getattr(_library or lib(), name)(*args)
+    if status:
+        check(status)
 
 
 def elementwise_program(params: dict, input_pointers: list[int], out_pointer: int, stream: int) -> None:

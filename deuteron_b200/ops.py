@@ -13,8 +13,13 @@ import torch
 from . import native
 
 
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)   # the handle alone: 0.3 us where the Stream object takes 3.2
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -347,16 +352,13 @@ _STORAGE_OF = {torch.float32: native.STORAGE['f32'], torch.float16: native.STORA
 _LAYOUTS = {'half': 0, 'interleaved': 1}
 
 
-def _on_current_device(**tensors: torch.Tensor) -> None:
-    current = None
-    for label, tensor in tensors.items():
-        device = tensor.get_device()
-        if device < 0:
-            raise ValueError(f'deuteron_b200 operators take CUDA tensors: {label} is on {tensor.device}')
-        if current is None:
-            current = torch.cuda.current_device()
-        if device != current:
-            raise ValueError(f'{label} is on {tensor.device}, the current device is cuda:{current}')
+def _on_current_device(*tensors: torch.Tensor) -> None:
+    if not all([tensor.is_cuda for tensor in tensors]):
+        raise ValueError('deuteron_b200 operators take CUDA tensors')
+    current = torch.cuda.current_device()
+    for tensor in tensors:
+        if tensor.get_device() != current:
+            raise ValueError(f'a tensor is on {tensor.device}, the current device is cuda:{current}')
 
 
 def _tensors(*tensors: torch.Tensor) -> None:
@@ -402,27 +404,30 @@ def _rotation(frequencies: torch.Tensor | None, layout: str, dim: int) -> int:
     return pairs
 
 
-def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor) -> tuple[int, int]:
-    """Page and head strides that both pools share; checks pools and tables."""
-    for label, pool in (('k_pages', k_pages), ('v_pages', v_pages)):
-        if pool.dim() != 4:
-            raise ValueError(f'{label} must be a [pages, kv_heads, page_size, dim] tensor')
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor) -> tuple[int, int, int, int, int, int, int, int, int]:
+    """Pages, kv heads, page size, head size, page and head strides of both pools, then sequences, pages per sequence and row
+    stride of the tables, all checked."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.dim() != 4:
+        raise ValueError(f'{"k_pages" if len(shape) != 4 else "v_pages"} must be a [pages, kv_heads, page_size, dim] tensor')
+    if shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError('k_pages and v_pages must have one shape and dtype')
-    pages, heads, size, dim = k_pages.shape
+    pages, heads, size, dim = shape
     if size < 1:
         raise ValueError('a page holds at least one token')
-    strides = []
-    for label, pool in (('k_pages', k_pages), ('v_pages', v_pages)):
-        page, head, token, unit = pool.stride()
-        if (dim > 1 and unit != 1) or (size > 1 and token != dim):
-            raise ValueError(f'the rows of one page and head must be dense in {label}')
-        strides.append((page if pages > 1 else 0, head if heads > 1 else 0))
-    if strides[0] != strides[1]:
-        raise ValueError('k_pages and v_pages must have the same strides')
-    if tables.dtype != torch.int32 or tables.dim() != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1):
-        raise ValueError('tables must be a [sequences, pages per sequence] int32 tensor with unit column stride')
-    return strides[0]
+    strides = k_pages.stride()
+    page, head, token, unit = strides
+    if (dim > 1 and unit != 1) or (size > 1 and token != dim):
+        raise ValueError('the rows of one page and head must be dense in k_pages and v_pages')
+    if strides != v_pages.stride():   # strides of extents of one are nobody's business
+        if any(extent > 1 and a != b for extent, a, b in zip(shape, strides, v_pages.stride())):
+            raise ValueError('k_pages and v_pages must have the same strides')
+    if tables.dtype != torch.int32 or tables.dim() != 2:
+        raise ValueError('tables must be a [sequences, pages per sequence] int32 tensor')
+    (sequences, width), (row, column) = tables.shape, tables.stride()
+    if width > 1 and column != 1:
+        raise ValueError('tables must have unit column stride')
+    return pages, heads, size, dim, page if pages > 1 else 0, head if heads > 1 else 0, sequences, width, row if sequences > 1 else 0
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -470,14 +475,14 @@ def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> tor
     _index(positions, 'positions', tokens, wide=True)
     pairs = _rotation(frequencies, layout, dim)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     _tensors(out)
     if out.dtype != x.dtype or out.shape != x.shape:
         raise ValueError('out must have the shape and dtype of x')
     out_token_stride, out_head_stride = _heads(out, 'out', written=True)
     if out.data_ptr() == x.data_ptr() and (out_token_stride, out_head_stride) != (token_stride, head_stride):
         raise ValueError('out must be x itself or lie elsewhere')
-    _on_current_device(x=x, positions=positions, frequencies=frequencies, out=out)
+    _on_current_device(x, positions, frequencies, out)
     native.call('dtn_rotary', x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(),
                 tokens, heads, dim, pairs, token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose,
                 amplitude, _STORAGE_OF[x.dtype], _stream())
@@ -520,9 +525,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if k.dtype not in _STORAGE_OF or v.dtype != k.dtype or k_pages.dtype != k.dtype:
         raise ValueError('k, v and the pools must share dtype float32, float16 or bfloat16')
     (k_token, k_head), (v_token, v_head) = _heads(k, 'k'), _heads(v, 'v')
-    page_stride, page_head_stride = _pools(k_pages, v_pages, tables)
+    pages, pool_heads, page_size, pool_dim, page_stride, page_head_stride, sequences, width, table_stride = _pools(k_pages, v_pages, tables)
     tokens, kv_heads, dim = k.shape
-    pages, pool_heads, page_size, pool_dim = k_pages.shape
     if v.shape != k.shape or pool_heads != kv_heads or pool_dim != dim:
         raise ValueError('k, v and the pools disagree in shape')
     if (pages > 1 and page_stride == 0) or (kv_heads > 1 and page_head_stride == 0):
@@ -540,43 +544,42 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         if q.dtype != k.dtype or q.shape[0] != tokens or q.shape[2] != dim:
             raise ValueError('q must be a [tokens, q_heads, dim] tensor of the dtype of k')
         if q_out is None:
-            q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _tensors(q_out)
         if q_out.dtype != q.dtype or q_out.shape != q.shape:
             raise ValueError('q_out must have the shape and dtype of q')
         q_out_token, q_out_head = _heads(q_out, 'q_out', written=True)
         if q_out.data_ptr() == q.data_ptr() and (q_out_token, q_out_head) != (q_token, q_head):
             raise ValueError('q_out must be q itself or lie elsewhere')
-        _on_current_device(q=q, q_out=q_out)
-    _on_current_device(k=k, v=v, k_pages=k_pages, v_pages=v_pages, tables=tables, rows=rows, positions=positions,
-                       frequencies=k if frequencies is None else frequencies)
+        _on_current_device(q, q_out)
+    _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, k if frequencies is None else frequencies)
     native.call('dtn_paged_append', k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(),
                 positions.data_ptr(), positions.dtype == torch.int64, tokens, kv_heads, dim, k_token, k_head, v_token, v_head, pages, page_size,
-                page_stride, page_head_stride, tables.shape[0], tables.shape[1], tables.stride(0) if tables.shape[0] > 1 else 0,
-                frequencies.data_ptr() if pairs else None, pairs, _LAYOUTS[layout], amplitude, q.data_ptr() if q_heads else None,
-                q_out.data_ptr() if q_heads else None, q_heads, q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
+                page_stride, page_head_stride, sequences, width, table_stride, frequencies.data_ptr() if pairs else None, pairs,
+                _LAYOUTS[layout], amplitude, q.data_ptr() if q_heads else None, q_out.data_ptr() if q_heads else None, q_heads, q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
     return q_out
 
 
-_paged_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_paged_workspaces: dict[tuple[int, int], tuple[torch.Tensor, int, int]] = {}
 _PAGED_COUNTER_BYTES = 4096
 
 
-def _paged_workspace(device: torch.device) -> tuple[int, int]:
+def _paged_workspace(q: torch.Tensor, stream: int) -> tuple[int, int]:
     """Address and size of the parts and counters of `paged_attention`, one workspace per device and stream. Its counters are zeroed
     here once; every call leaves them zero. A call that is captured gets one of its own from the graph's memory, zeroed by each
     replay: replays may run beside one another and beside eager calls."""
     capturing = torch.cuda.is_current_stream_capturing()
-    key = (device.index, _stream())
-    workspace = None if capturing else _paged_workspaces.get(key)
-    if workspace is None:
+    key = (q.get_device(), stream)
+    held = None if capturing else _paged_workspaces.get(key)
+    if held is None:
         size = ct.c_size_t(0)
         native.call('dtn_paged_attention_workspace_bytes', ct.byref(size))
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=q.device)
         workspace[:_PAGED_COUNTER_BYTES].zero_()
+        held = workspace, workspace.data_ptr(), size.value
         if not capturing:
-            _paged_workspaces[key] = workspace
-    return workspace.data_ptr(), workspace.numel()
+            _paged_workspaces[key] = held
+    return held[1:]
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, scale: float,
@@ -596,32 +599,30 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dtype not in _STORAGE_OF or k_pages.dtype != q.dtype:
         raise ValueError('q and the pools must share dtype float32, float16 or bfloat16')
     q_token, q_head = _heads(q, 'q')
-    page_stride, page_head_stride = _pools(k_pages, v_pages, tables)
+    pages, kv_heads, page_size, pool_dim, page_stride, page_head_stride, sequences, width, table_stride = _pools(k_pages, v_pages, tables)
     count, q_heads, dim = q.shape
-    pages, kv_heads, page_size, pool_dim = k_pages.shape
     if pool_dim != dim:
         raise ValueError('q and the pools disagree in the head size')
     if kv_heads == 0 or q_heads % kv_heads:
         raise ValueError('query heads must be a multiple of kv heads')
-    _index(lengths, 'lengths', tables.shape[0])
+    _index(lengths, 'lengths', sequences)
     if rows is not None:
         _tensors(rows)
         _index(rows, 'rows', count)
-    elif count > tables.shape[0]:
-        raise ValueError(f'{count} queries but {tables.shape[0]} sequences')
+    elif count > sequences:
+        raise ValueError(f'{count} queries but {sequences} sequences')
     if window < 0:
         raise ValueError('window must not be negative')
     if out is None:
-        out = torch.empty((count, q_heads, dim), dtype=torch.float32, device=q.device)
+        out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)
     _tensors(out)
     if out.shape != q.shape or out.dtype not in (torch.float32, q.dtype):
         raise ValueError('out must have the shape of q and dtype float32 or that of q')
     out_token, out_head = _heads(out, 'out', written=True)
-    _on_current_device(q=q, k_pages=k_pages, v_pages=v_pages, tables=tables, lengths=lengths, rows=lengths if rows is None else rows, out=out)
+    _on_current_device(q, k_pages, v_pages, tables, lengths, lengths if rows is None else rows, out)
     native.call('dtn_paged_attention', q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
                 None if rows is None else rows.data_ptr(), out.data_ptr(), count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head,
-                pages, page_size, page_stride, page_head_stride, tables.shape[0], tables.shape[1],
-                tables.stride(0) if tables.shape[0] > 1 else 0, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, *_paged_workspace(q.device), _stream())
+                pages, page_size, page_stride, page_head_stride, sequences, width, table_stride, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, *_paged_workspace(q, stream := _stream()), stream)
     return out
 
 
@@ -653,7 +654,7 @@ def copy_pages(pages: torch.Tensor, sources: torch.Tensor, destinations: torch.T
         raise ValueError('pages must not be an expanded tensor: it is written')
     _index(sources, 'sources')
     _index(destinations, 'destinations', sources.shape[0])
-    _on_current_device(pages=pages, sources=sources, destinations=destinations)
+    _on_current_device(pages, sources, destinations)
     unit = pages.element_size()
     native.call('dtn_copy_pages', pages.data_ptr(), planes, plane_stride * unit, count, page_stride * unit, dense * unit, sources.data_ptr(),
                 destinations.data_ptr(), sources.shape[0], _stream())
