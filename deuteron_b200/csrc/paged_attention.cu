@@ -51,7 +51,7 @@ struct PagedAttentionParams {
   float scale_log2e;
   int out_f32;
   int q_pairs, out_quads;               // neighbouring elements of q and out can be moved by two (4 bytes) and by four
-  int whole_chunks;                     // a chunk never straddles pages and rows fill their place in shared memory
+  int whole_sets;                       // the tokens of a set lie in one page, one after another, and fill their rows in shared memory
   int min_units;                        // a block takes at least this many units
   int* counters;
   float* parts;
@@ -73,24 +73,26 @@ __host__ __device__ __forceinline__ int64_t pa_workers(int64_t units, int64_t mi
   return most < 1 ? 1 : (most < grid ? most : grid);
 }
 
-template <typename T, int DP, int HB>
+template <typename T, int DP, int HB, int NH>
 struct PaConfig {
   static constexpr bool HALF = sizeof(T) == 2;
-  static constexpr int CHUNK = HALF ? 16 : 8;            // tokens per stage
+  static constexpr int SUB = HALF ? 16 : 8;              // tokens of one set of products
+  // sets that a team takes in one step: one per member keeps as many tokens in work whatever the group; twice that for small
+  // rows, whose chain of dependent instructions would otherwise outlast their bytes
+  static constexpr int SETS = DP == 64 ? (HB == 1 ? 2 : 4) : (DP == 256 && HB == 4 ? 2 : HB);
+  static constexpr int CHUNK = SUB * SETS;               // tokens per stage
   static constexpr int TEAMS = PA_WARPS / HB;
   static constexpr int ROW = DP * (int)sizeof(T);
-  static constexpr int STAGE = 2 * CHUNK * ROW;          // keys, then values: 64 * DP bytes
-  static constexpr int SLOTS = DP == 64 ? 24 : 12;
-  static constexpr int STAGES = HB == 4 ? (HALF ? 10 : 8) : SLOTS / TEAMS;
-  static constexpr int RING = TEAMS * STAGES * STAGE;
-  static constexpr int MERGE = HB == 4 ? 128 * DP : 0;   // else the stage just read holds a team's numerators
-  static constexpr int QUERY = HALF ? 0 : HB * 8 * DP * 4;
-  static constexpr int SMEM = RING + MERGE + QUERY;
+  static constexpr int STAGE = 2 * CHUNK * ROW;          // keys, then values: 64 * DP * SETS bytes; at an item's end numerators of HB x 8 heads
+  static constexpr int RING = (DP == 256 ? 192 : 96) * 1024;
+  static constexpr int STAGES = RING / (TEAMS * STAGE);
+  static constexpr int QUERY = HALF ? 0 : HB * NH * DP * 4;
+  static constexpr int SMEM = RING + QUERY;
   static constexpr int BLOCKS_PER_SM = DP == 256 ? 1 : 2;
-  static constexpr int HEADS = 8 * HB;                   // query heads of an item
+  static constexpr int HEADS = 8 * HB;                   // query heads of an item (the first NH of each 8 are looked at)
   static constexpr int PART = HEADS * DP + 2 * HEADS;    // floats: numerators, maxima, sums
+  static_assert(STAGES >= 3 && STAGE >= HEADS * DP * 4, "a ring of three stages, numerators that fit one");
 };
-
 
 __device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -221,15 +223,15 @@ struct PaCursor {
   }
 };
 
-template <typename T, int DP, int HB>
-__global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER_SM) paged_attention_kernel(const PagedAttentionParams p) {
-  using C = PaConfig<T, DP, HB>;
-  constexpr int CHUNK = C::CHUNK, TEAMS = C::TEAMS, ROW = C::ROW, STAGES = C::STAGES, UNIT = CHUNK * TEAMS, THREADS = PA_WARPS * 32;
+template <typename T, int DP, int HB, int NH>
+__global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS_PER_SM) paged_attention_kernel(const PagedAttentionParams p) {
+  using C = PaConfig<T, DP, HB, NH>;
+  constexpr int CHUNK = C::CHUNK, SETS = C::SETS, TEAMS = C::TEAMS, ROW = C::ROW, STAGES = C::STAGES, UNIT = CHUNK * TEAMS, THREADS = PA_WARPS * 32;
   constexpr int LANES = ROW / 16;                  // 16-byte vectors of a row
   constexpr float NONE = -INFINITY;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_max[PA_WARPS][8], s_sum[PA_WARPS][8];
-  __shared__ float s_p[C::HALF ? 1 : PA_WARPS][8][8], s_alpha[C::HALF ? 1 : PA_WARPS][8];
+  __shared__ __align__(16) float s_p[C::HALF ? 1 : PA_WARPS][C::HALF ? 1 : CHUNK][NH], s_alpha[C::HALF ? 1 : PA_WARPS][8];
   __shared__ int64_t s_scan[PA_WARPS];
   __shared__ int64_t s_start[2];
   __shared__ int s_last;
@@ -302,11 +304,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
   // -- copies -------------------------------------------------------------------------------------
   uint8_t* ring = smem + team * STAGES * C::STAGE;
   const uint32_t ring_address = smem_u32(ring);
-  int64_t offset = -1;             // of the row of token lane % CHUNK of the stage that is copied next; -1: not seen, -2: no such page
-  uint32_t bad_stages = 0;         // stages that hold a token without a page
+  constexpr int ROWS = CHUNK / HB;                 // of a stage, copied by this warp: rows member * ROWS + 0, 1, ...
+  int64_t offset = -1;             // of row lane % ROWS of them in the stage that is copied next; -1: not seen, -2: no such page
 
   auto look_up = [&]() {
-    const int token = (ahead.tile * TEAMS + team) * CHUNK + lane % CHUNK;
+    const int token = (ahead.tile * TEAMS + team) * CHUNK + member * ROWS + lane % ROWS;
     offset = -1;
     if (token < ahead.s.seen) {
       const int position = ahead.s.first + token;
@@ -318,40 +320,45 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
     }
   };
   // Lane l copies vector l % LANES of rows l / LANES, + 32 / LANES, ...: their swizzled places differ by constants.
-  constexpr int ROWS = CHUNK / HB;                 // of a stage, copied by this warp
-  const int lane_row = member * ROWS + (LANES <= 32 ? lane / LANES : 0), lane_column = LANES <= 32 ? lane % LANES : lane;
+  const int lane_row = LANES <= 32 ? lane / LANES : 0, lane_column = LANES <= 32 ? lane % LANES : lane;
   const uint8_t* const k_lane = static_cast<const uint8_t*>(p.k_pages) + lane_column * 16;
   const uint8_t* const v_lane = static_cast<const uint8_t*>(p.v_pages) + lane_column * 16;
-  const uint32_t lane_place = lane_row * ROW + ((C::HALF ? lane_column ^ (lane_row & 7) : lane_column ^ ((lane_row & 1) << 2)) * 16);
+  const uint32_t lane_place = (member * ROWS + lane_row) * ROW +
+                              (C::HALF ? lane_column ^ ((member * ROWS + lane_row) & 7) : lane_column ^ (((member * ROWS + lane_row) & 1) << 2)) * 16;
   auto copy = [&](int slot) {
     const uint32_t seen_rows = __ballot_sync(0xffffffffu, offset >= 0);
     const uint32_t stage = ring_address + slot * C::STAGE;
-    if (seen_rows == 0xffffffffu && p.whole_chunks) {   // one page holds the rows one after another: constant distances
-      const int64_t at = __shfl_sync(0xffffffffu, offset, 0) + (LANES <= 32 ? lane_row : member * ROWS) * ROW;
+    if (seen_rows == 0xffffffffu && p.whole_sets) {   // one page holds the rows of a set one after another: constant distances
+      constexpr int TOGETHER = ROWS < C::SUB ? ROWS : C::SUB;
 #pragma unroll
-      for (int j = 0; j < ROWS * LANES / 32; ++j) {
-        // rows between two copies of a lane; a row of 64 vectors takes two copies, 512 bytes apart
-        const int row = LANES <= 32 ? j * (LANES <= 32 ? 32 / LANES : 1) : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;
-        const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + row * ROW + half;
-        pa_copy16(to, k_lane + at + row * ROW + half);
-        pa_copy16(to + CHUNK * ROW, v_lane + at + row * ROW + half);
+      for (int set = 0; set < ROWS / TOGETHER; ++set) {
+        const int64_t at = __shfl_sync(0xffffffffu, offset, set * TOGETHER) + lane_row * ROW;
+#pragma unroll
+        for (int j = 0; j < TOGETHER * LANES / 32; ++j) {
+          // rows between two copies of a lane; a row of 64 vectors takes two copies, 512 bytes apart
+          const int row = LANES <= 32 ? j * (LANES <= 32 ? 32 / LANES : 1) : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;
+          const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + (set * TOGETHER + row) * ROW + half;
+          pa_copy16(to, k_lane + at + row * ROW + half);
+          pa_copy16(to + CHUNK * ROW, v_lane + at + row * ROW + half);
+        }
       }
-      bad_stages &= ~(1u << slot);
       return;
     }
     const bool bad = __any_sync(0xffffffffu, offset == -2);
-    bad_stages = (bad_stages & ~(1u << slot)) | ((uint32_t)bad << slot);
     if (bad && lane == 0) paged_report(p.status, PAGED_STATUS_ATTENTION);
-    if (!bad && seen_rows == 0) return;
+    if (!bad && seen_rows == 0 && HB == 1) return;   // nothing of this stage is looked at
 #pragma unroll
     for (int j = 0; j < ROWS * LANES / 32; ++j) {
-      const int v = lane + 32 * j, row = member * ROWS + v / LANES, column = v % LANES;
-      const int64_t at = __shfl_sync(0xffffffffu, offset, row);
+      const int v = lane + 32 * j, own = v / LANES, row = member * ROWS + own, column = v % LANES;
+      const int64_t at = __shfl_sync(0xffffffffu, offset, own);
       const int swizzled = C::HALF ? column ^ (row & 7) : column ^ ((row & 1) << 2);
       const uint32_t to = stage + row * ROW + swizzled * 16;
       const bool there = at >= 0 && column * 16 < p.row_bytes;   // else zeros: neither what is not seen nor the columns past a head count
       const int64_t from = there ? at + column * 16 : 0;
-      pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
+      if (at == -2)   // keys of a page that does not exist are NaN, and so is all that sees them
+        *reinterpret_cast<uint4*>(ring + (to - ring_address)) = make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
+      else
+        pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
       pa_copy16(to + CHUNK * ROW, static_cast<const uint8_t*>(p.v_pages) + from, there ? 16 : 0);
     }
   };
@@ -379,7 +386,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
   // -- queries ------------------------------------------------------------------------------------
   constexpr int STEPS_K = DP / 16;
   uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF && DP < 256 ? STEPS_K : 1][2];
-  float* s_query = reinterpret_cast<float*>(smem + C::RING + C::MERGE);
+  float* s_query = reinterpret_cast<float*>(smem + C::RING);
   auto head_of = [&](int block, int h) { return block * C::HEADS + h; };   // within the group
   auto load_query = [&](uint32_t (&to)[C::HALF ? STEPS_K : 1][2], int64_t sequence, int kv_head, int block) {
     // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
@@ -408,8 +415,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
   // -- the pass over the tokens -------------------------------------------------------------------
   constexpr int COLUMNS = DP / 32;                 // FP32 storage: columns of V per lane
   float top[2] = {NONE, NONE}, total_p[2] = {0.f, 0.f};   // of heads 2t, 2t + 1
-  float acc[C::HALF ? DP / 16 : 8][C::HALF ? 4 : COLUMNS];
-  bool fresh = true, poisoned = false, exactly = false;
+  constexpr int A = C::HALF ? DP / 16 : NH, B = C::HALF ? 4 : COLUMNS;
+  float acc[A][B];                                 // numerators: 16 columns of V by 2 heads, or NH heads by COLUMNS
+  bool fresh = true, exactly = false;
   int start = 0, slot = 0;                         // the item's first tile here; the stage read next
 
   while (now.left > 0) {
@@ -425,13 +433,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
     if (fresh) {
       fresh = false;
       start = now.tile;
-      poisoned = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) top[i] = NONE, total_p[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < (C::HALF ? DP / 16 : 8); ++i)
+      for (int i = 0; i < A; ++i)
 #pragma unroll
-        for (int j = 0; j < (C::HALF ? 4 : COLUMNS); ++j) acc[i][j] = 0.f;
+        for (int j = 0; j < B; ++j) acc[i][j] = 0.f;
       if constexpr (C::HALF && DP == 256) {
         load_query(query, now.sequence, now.kv_head, now.block);   // registers for one item's query only
       } else if constexpr (C::HALF) {
@@ -443,8 +450,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
         if (next.left > 0) load_query(query_next, next.sequence, next.kv_head, next.block);
       } else {
         __syncthreads();
-        for (int i = tid; i < C::HEADS * DP; i += THREADS) {
-          const int h = head_of(now.block, i / DP), d = i % DP;
+        for (int i = tid; i < HB * NH * DP; i += THREADS) {
+          const int h = head_of(now.block, i / DP / NH * 8 + i / DP % NH), d = i % DP;
           s_query[i] = h < p.group && d < p.dim ? static_cast<const float*>(p.q)[now.sequence * p.q_token_stride +
                                                       ((int64_t)now.kv_head * p.group + h) * p.q_head_stride + d] : 0.f;
         }
@@ -453,53 +460,63 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
     }
 
     const int base = (now.tile * TEAMS + team) * CHUNK, seen = now.s.seen;
-    poisoned |= (bad_stages >> slot) & 1;
     if (base < seen) {
       const uint32_t stage = ring_address + slot * C::STAGE;
-      constexpr int SETS = C::HALF ? 2 : 1;        // tokens g (and g + 8) of the chunk
-      float x[SETS][2];
+      constexpr int EIGHTS = CHUNK / 8;            // tokens g + 8 n of the chunk
+      float x[EIGHTS][2];                          // scores, then probabilities, of heads 2t and 2t + 1
       if constexpr (C::HALF) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};   // two chains of products
         const uint32_t k_place = stage + lane % 16 * ROW + ((lane / 16) ^ (lane % 8)) * 16;   // stages are multiples of 128 bytes
 #pragma unroll
-        for (int ks = 0; ks < STEPS_K; ++ks) {
-          uint32_t a[4];
-          pa_ldmatrix(a, (k_place ^ (ks % 4 * 32)) + ks / 4 * 128);
-          pa_mma(ks % 2 ? s2 : s, a, query[ks][0], query[ks][1], T());
+        for (int set = 0; set < SETS; ++set) {
+          float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};   // two chains of products
+#pragma unroll
+          for (int ks = 0; ks < STEPS_K; ++ks) {
+            uint32_t a[4];
+            pa_ldmatrix(a, (k_place ^ (ks % 4 * 32)) + ks / 4 * 128 + set * 16 * ROW);
+            pa_mma(ks % 2 ? s2 : s, a, query[ks][0], query[ks][1], T());
+          }
+          x[2 * set][0] = s[0] + s2[0], x[2 * set][1] = s[1] + s2[1];
+          x[2 * set + 1][0] = s[2] + s2[2], x[2 * set + 1][1] = s[3] + s2[3];
         }
-        x[0][0] = s[0] + s2[0], x[0][1] = s[1] + s2[1];
-        x[SETS - 1][0] = s[2] + s2[2], x[SETS - 1][1] = s[3] + s2[3];
       } else {
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const float* query_rows = s_query + member * 8 * DP;
+        const float* query_rows = s_query + member * NH * DP;
+        float s[SETS][8] = {};
 #pragma unroll
         for (int j = 0; j < DP / 16; ++j) {
           const int column = t + 4 * j;
-          const float4 k = *reinterpret_cast<const float4*>(ring + slot * C::STAGE + g * ROW + ((column ^ ((g & 1) << 2)) * 16));
+          float4 k[SETS];
 #pragma unroll
-          for (int h = 0; h < 8; ++h) {
+          for (int set = 0; set < SETS; ++set)
+            k[set] = *reinterpret_cast<const float4*>(ring + slot * C::STAGE + (set * 8 + g) * ROW + ((column ^ ((g & 1) << 2)) * 16));
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
             const float4 q = *reinterpret_cast<const float4*>(query_rows + h * DP + column * 4);
-            s[h] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[h]))));
+#pragma unroll
+            for (int set = 0; set < SETS; ++set)
+              s[set][h] = fmaf(k[set].x, q.x, fmaf(k[set].y, q.y, fmaf(k[set].z, q.z, fmaf(k[set].w, q.w, s[set][h]))));
           }
         }
-        // four lanes hold parts of a token's 8 scores; lane t ends with heads 2t and 2t + 1
-        float r[4];
+        // four lanes hold parts of a token's scores; lane t ends with heads 2t and 2t + 1 (those past NH: zeros)
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const float kept = t & 2 ? s[h + 4] : s[h], sent = t & 2 ? s[h] : s[h + 4];
-          r[h] = kept + __shfl_xor_sync(0xffffffffu, sent, 2);
-        }
+        for (int set = 0; set < SETS; ++set) {
+          float r[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float kept = t & 1 ? r[h + 2] : r[h], sent = t & 1 ? r[h] : r[h + 2];
-          x[0][h] = kept + __shfl_xor_sync(0xffffffffu, sent, 1);
+          for (int h = 0; h < 4; ++h) {
+            const float kept = t & 2 ? s[set][h + 4] : s[set][h], sent = t & 2 ? s[set][h] : s[set][h + 4];
+            r[h] = h < NH ? kept + __shfl_xor_sync(0xffffffffu, sent, 2) : 0.f;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float kept = t & 1 ? r[h + 2] : r[h], sent = t & 1 ? r[h] : r[h + 2];
+            x[set][h] = h < NH ? kept + __shfl_xor_sync(0xffffffffu, sent, 1) : 0.f;
+          }
         }
       }
 #pragma unroll
-      for (int n = 0; n < SETS; ++n) x[n][0] *= p.scale_log2e, x[n][1] *= p.scale_log2e;
+      for (int n = 0; n < EIGHTS; ++n) x[n][0] *= p.scale_log2e, x[n][1] *= p.scale_log2e;
       if (base + CHUNK > seen) {
 #pragma unroll
-        for (int n = 0; n < SETS; ++n)
+        for (int n = 0; n < EIGHTS; ++n)
           if (base + g + 8 * n >= seen) x[n][0] = x[n][1] = NONE;
       }
       // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
@@ -507,12 +524,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       constexpr float GROWTH = 8.f;
       bool higher = false;
 #pragma unroll
-      for (int n = 0; n < SETS; ++n) higher |= x[n][0] > top[0] + GROWTH || x[n][1] > top[1] + GROWTH;
+      for (int n = 0; n < EIGHTS; ++n) higher |= x[n][0] > top[0] + GROWTH || x[n][1] > top[1] + GROWTH;
       if (__any_sync(0xffffffffu, higher)) {
         float alpha[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float high = fmaxf(top[i], fmaxf(x[0][i], x[SETS - 1][i]));
+          float high = top[i];
+#pragma unroll
+          for (int n = 0; n < EIGHTS; ++n) high = fmaxf(high, x[n][i]);
 #pragma unroll
           for (int o = 4; o < 32; o *= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
           alpha[i] = ex2_approx_ftz(top[i] - (high == NONE ? 0.f : high));
@@ -528,7 +547,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           if (g == 0) s_alpha[warp][2 * t] = alpha[0], s_alpha[warp][2 * t + 1] = alpha[1];
           __syncwarp();
 #pragma unroll
-          for (int h = 0; h < 8; ++h) {
+          for (int h = 0; h < NH; ++h) {
             const float a = s_alpha[warp][h];
 #pragma unroll
             for (int j = 0; j < COLUMNS; ++j) acc[h][j] *= a;
@@ -540,7 +559,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       for (int i = 0; i < 2; ++i) {
         const float around = top[i] == NONE ? 0.f : top[i];   // every score -inf so far: the exponentials are zeros, not NaN
 #pragma unroll
-        for (int n = 0; n < SETS; ++n) {
+        for (int n = 0; n < EIGHTS; ++n) {
           x[n][i] = ex2_approx_ftz(x[n][i] - around);
           total_p[i] += x[n][i];
         }
@@ -548,43 +567,56 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
       if constexpr (C::HALF) {
         if (!exactly) {
           constexpr int TERMS = std::is_same_v<T, __half> ? 2 : 3;
-          uint32_t b[TERMS][2];
+          uint32_t b[SETS][TERMS][2];
 #pragma unroll
-          for (int n = 0; n < TERMS; ++n) {
+          for (int set = 0; set < SETS; ++set)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) b[n][half] = pa_transpose(pa_take(x[half][0], x[half][1], T()));
-          }
+            for (int n = 0; n < TERMS; ++n)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) b[set][n][half] = pa_transpose(pa_take(x[2 * set + half][0], x[2 * set + half][1], T()));
           const uint32_t v_place = stage + CHUNK * ROW + (lane % 8 + lane / 16 * 8) * ROW + ((lane / 8 % 2) ^ (lane % 8)) * 16;
 #pragma unroll
           for (int mt = 0; mt < DP / 16; ++mt) {
-            uint32_t a[4];
             float y[4];
-            pa_ldmatrix_t(a, (v_place ^ (mt % 4 * 32)) + mt / 4 * 128);
-            pa_mma_first(y, a, b[TERMS - 1][0], b[TERMS - 1][1], T());   // small terms first
 #pragma unroll
-            for (int n = TERMS - 2; n >= 0; --n) pa_mma(y, a, b[n][0], b[n][1], T());
+            for (int set = 0; set < SETS; ++set) {
+              uint32_t a[4];
+              pa_ldmatrix_t(a, (v_place ^ (mt % 4 * 32)) + mt / 4 * 128 + set * 16 * ROW);
+#pragma unroll
+              for (int n = TERMS - 1; n >= 0; --n) {   // small terms first
+                if (set == 0 && n == TERMS - 1)
+                  pa_mma_first(y, a, b[set][n][0], b[set][n][1], T());
+                else
+                  pa_mma(y, a, b[set][n][0], b[set][n][1], T());
+              }
+            }
             pa_add2(acc[mt][0], acc[mt][1], y[0], y[1]);
             pa_add2(acc[mt][2], acc[mt][3], y[2], y[3]);
           }
         } else {
+#pragma unroll
+          for (int n = 0; n < EIGHTS; ++n) {
 #pragma unroll 1
-          for (int token = 0; token < CHUNK; ++token) {
-            const float p0 = __shfl_sync(0xffffffffu, token < 8 ? x[0][0] : x[1][0], token % 8 * 4 + t);
-            const float p1 = __shfl_sync(0xffffffffu, token < 8 ? x[0][1] : x[1][1], token % 8 * 4 + t);
-            const uint8_t* values = ring + slot * C::STAGE + CHUNK * ROW + token * ROW + g * 2;
+            for (int token = 0; token < 8; ++token) {
+              const float p0 = __shfl_sync(0xffffffffu, x[n][0], token * 4 + t), p1 = __shfl_sync(0xffffffffu, x[n][1], token * 4 + t);
+              const uint8_t* values = ring + slot * C::STAGE + CHUNK * ROW + (8 * n + token) * ROW + g * 2;
 #pragma unroll
-            for (int mt = 0; mt < DP / 16; ++mt)
+              for (int mt = 0; mt < DP / 16; ++mt)
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float v = to_float(*reinterpret_cast<const T*>(values + ((2 * mt + j) ^ (token & 7)) * 16));
-                acc[mt][2 * j] = fmaf(p0, v, acc[mt][2 * j]);
-                acc[mt][2 * j + 1] = fmaf(p1, v, acc[mt][2 * j + 1]);
-              }
+                for (int j = 0; j < 2; ++j) {
+                  const float v = to_float(*reinterpret_cast<const T*>(values + ((2 * mt + j) ^ token) * 16));
+                  acc[mt][2 * j] = fmaf(p0, v, acc[mt][2 * j]);
+                  acc[mt][2 * j + 1] = fmaf(p1, v, acc[mt][2 * j + 1]);
+                }
+            }
           }
         }
       } else {
-        s_p[warp][g][2 * t] = x[0][0];
-        s_p[warp][g][2 * t + 1] = x[0][1];
+#pragma unroll
+        for (int n = 0; n < EIGHTS; ++n) {
+          if (2 * t < NH) s_p[warp][8 * n + g][2 * t] = x[n][0];
+          if (2 * t + 1 < NH) s_p[warp][8 * n + g][2 * t + 1] = x[n][1];
+        }
         __syncwarp();
 #pragma unroll
         for (int token = 0; token < CHUNK; ++token) {
@@ -598,7 +630,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
               *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(values + (((lane + 32 * j) ^ ((token & 1) << 2)) * 16));
           }
 #pragma unroll
-          for (int h = 0; h < 8; ++h) {
+          for (int h = 0; h < NH; ++h) {
             const float pr = s_p[warp][token][h];
 #pragma unroll
             for (int j = 0; j < COLUMNS; ++j) acc[h][j] = fmaf(pr, v[j], acc[h][j]);
@@ -643,11 +675,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
         for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
         if (g == 0) {
           s_max[warp][2 * t + i] = top[i];
-          s_sum[warp][2 * t + i] = poisoned ? __int_as_float(0x7fffffff) : total_p[i];   // NaN: a page that does not exist is no zero
+          s_sum[warp][2 * t + i] = total_p[i];
         }
       }
       if constexpr (!C::HALF) team_barrier();   // every warp of the team has read the stage
-      float* numerators = reinterpret_cast<float*>(HB == 4 ? smem + C::RING : ring + slot * C::STAGE) + member * 8 * DP;
+      float* numerators = reinterpret_cast<float*>(ring + slot * C::STAGE) + member * 8 * DP;
       if constexpr (C::HALF) {
 #pragma unroll
         for (int mt = 0; mt < DP / 16; ++mt)
@@ -655,7 +687,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
           for (int j = 0; j < 4; ++j) numerators[(2 * t + j % 2) * DP + ((mt * 16 + g + 8 * (j / 2)) ^ (t << 3))] = acc[mt][j];
       } else {
 #pragma unroll
-        for (int h = 0; h < 8; ++h)
+        for (int h = 0; h < NH; ++h)
 #pragma unroll
           for (int j = 0; j < COLUMNS; ++j) {
             const int d = COLUMNS == 2 ? 2 * lane + j : (j / 4) * 128 + 4 * lane + j % 4;
@@ -696,7 +728,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
         for (int m = 0; m < TEAMS; ++m) {
           const int w = m * HB + slot_head / 8;
           const float weight = ex2_approx_ftz(s_max[w][slot_head % 8] - around);
-          const float* from = reinterpret_cast<const float*>(HB == 4 ? smem + C::RING : smem + (m * STAGES + slot) * C::STAGE);
+          const float* from = reinterpret_cast<const float*>(smem + (m * STAGES + slot) * C::STAGE);
           const float4 x = *reinterpret_cast<const float4*>(from + slot_head * DP + (d ^ (((slot_head % 8) / 2) << 3)));
           y.x = fmaf(weight, x.x, y.x), y.y = fmaf(weight, x.y, y.y), y.z = fmaf(weight, x.z, y.z), y.w = fmaf(weight, x.w, y.w);
           weight_sum = fmaf(weight, s_sum[w][slot_head % 8], weight_sum);
@@ -773,39 +805,44 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB>::BLOCKS_PER
 static size_t pa_workspace_bytes() {
   // two parts per block of the largest forms: 32 heads of 128 and two blocks per SM, 32 heads of 256 and one
   const size_t blocks = (size_t)sm_count();
-  const size_t small = 2 * blocks * 2 * PaConfig<float, 128, 4>::PART, large = blocks * 2 * PaConfig<float, 256, 4>::PART;
+  const size_t small = 2 * blocks * 2 * PaConfig<float, 128, 4, 8>::PART, large = blocks * 2 * PaConfig<float, 256, 4, 8>::PART;
   return PA_COUNTER_BYTES + (small > large ? small : large) * sizeof(float);
 }
 
-template <typename T, int DP, int HB>
+template <typename T, int DP, int HB, int NH>
 static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
-  using C = PaConfig<T, DP, HB>;
+  using C = PaConfig<T, DP, HB, NH>;
   static thread_local int attr_dev = -1;
   int dev = 0;
   DTN_CUDA_CHECK(cudaGetDevice(&dev));
   if (attr_dev != dev) {
-    DTN_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_kernel<T, DP, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    DTN_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_kernel<T, DP, HB, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_dev = dev;
   }
   p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
   p.heads = p.kv_heads * p.blocks;
-  p.whole_chunks = p.page_size % C::CHUNK == 0 && p.window == 0 && p.row_bytes == C::ROW;
+  p.whole_sets = p.page_size % C::SUB == 0 && p.window == 0 && p.row_bytes == C::ROW;
   int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
   const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;
   DTN_REQUIRE((double)p.count * p.heads * (double)(most_tiles + PA_ITEM_UNITS) < 2147483648.0 * (double)grid, DTN_ERR_UNSUPPORTED,
               "paged attention: the tables cover too many tokens for one launch");
   if (p.count < grid && p.heads < grid && most_tiles < grid && p.count * p.heads * most_tiles < grid) grid = p.count * p.heads * most_tiles;
-  paged_attention_kernel<T, DP, HB><<<(unsigned)grid, PA_WARPS * 32, C::SMEM, s>>>(p);
+  paged_attention_kernel<T, DP, HB, NH><<<(unsigned)grid, PA_WARPS * 32, C::SMEM, s>>>(p);
   DTN_LAUNCH_CHECK("paged_attention_kernel");
   return DTN_OK;
 }
 
 template <typename T, int DP>
 static int paged_attention_launch_d(PagedAttentionParams& p, cudaStream_t s) {
-  if (p.group <= 8) return paged_attention_launch_t<T, DP, 1>(p, s);
-  if (p.group <= 16) return paged_attention_launch_t<T, DP, 2>(p, s);
-  return paged_attention_launch_t<T, DP, 4>(p, s);
+  // FP32 multiply-adds are paid per head: a form for a head or four of the eight that the products of 16-bit storage have anyway
+  if constexpr (sizeof(T) == 4) {
+    if (p.group == 1) return paged_attention_launch_t<T, DP, 1, 1>(p, s);
+    if (p.group <= 4) return paged_attention_launch_t<T, DP, 1, 4>(p, s);
+  }
+  if (p.group <= 8) return paged_attention_launch_t<T, DP, 1, 8>(p, s);
+  if (p.group <= 16) return paged_attention_launch_t<T, DP, 2, 8>(p, s);
+  return paged_attention_launch_t<T, DP, 4, 8>(p, s);
 }
 
 template <typename T>
