@@ -643,9 +643,39 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
     // -- the end of an item, or of this block's part of it ----------------------------------------
     const bool to_end = now.tile + 1 == now.tiles;
     if (to_end || now.left == 1) {
+      // the teams' parts meet in shared memory: maxima and sums by warp, numerators in the stage that was just read (its
+      // refill is a step away). Columns are swizzled by the head so that neither side meets bank conflicts
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
+        if (g == 0) {
+          s_max[warp][2 * t + i] = top[i];
+          s_sum[warp][2 * t + i] = total_p[i];
+        }
+      }
+      team_barrier();   // every member has read the stage
+      float* numerators = reinterpret_cast<float*>(ring + slot * C::STAGE) + member * 8 * DP;
       if constexpr (C::HALF) {
-        // An infinite value times one term of a probability, negative or zero, is not what it is times the probability. Where
-        // a numerator is not finite the block goes over its tiles of the item once more, with whole probabilities.
+#pragma unroll
+        for (int mt = 0; mt < DP / 16; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) numerators[(2 * t + j % 2) * DP + ((mt * 16 + g + 8 * (j / 2)) ^ (t << 3))] = acc[mt][j];
+      } else {
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int j = 0; j < COLUMNS; ++j) {
+            const int d = COLUMNS == 2 ? 2 * lane + j : (j / 4) * 128 + 4 * lane + j % 4;
+            numerators[h * DP + (d ^ ((h / 2) << 3))] = acc[h][j];
+          }
+      }
+      if constexpr (!C::HALF) {
+        __syncthreads();
+      } else {
+        // Everybody's part is there behind this barrier. An infinite value times one term of a probability, negative or zero, is
+        // not what it is times the probability: where a numerator is not finite the block goes over its tiles of the item once
+        // more, with whole probabilities.
         float probe = 0.f;
         if (!exactly) {
 #pragma unroll
@@ -667,34 +697,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
         }
         exactly = false;
       }
-      // the teams' parts meet in shared memory: maxima and sums by warp, numerators in the stage that was just read (its
-      // refill is a step away). Columns are swizzled by the head so that neither side meets bank conflicts
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
-        if (g == 0) {
-          s_max[warp][2 * t + i] = top[i];
-          s_sum[warp][2 * t + i] = total_p[i];
-        }
-      }
-      if constexpr (!C::HALF) team_barrier();   // every warp of the team has read the stage
-      float* numerators = reinterpret_cast<float*>(ring + slot * C::STAGE) + member * 8 * DP;
-      if constexpr (C::HALF) {
-#pragma unroll
-        for (int mt = 0; mt < DP / 16; ++mt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) numerators[(2 * t + j % 2) * DP + ((mt * 16 + g + 8 * (j / 2)) ^ (t << 3))] = acc[mt][j];
-      } else {
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-#pragma unroll
-          for (int j = 0; j < COLUMNS; ++j) {
-            const int d = COLUMNS == 2 ? 2 * lane + j : (j / 4) * 128 + 4 * lane + j % 4;
-            numerators[h * DP + (d ^ ((h / 2) << 3))] = acc[h][j];
-          }
-      }
-      __syncthreads();
       const bool whole = start == 0 && to_end;
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + (start == 0 ? 1 : 0)) * C::PART;
       auto write = [&](int h, int d, float4 y) {   // h within the group, d a multiple of four
