@@ -905,7 +905,7 @@ int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   DTN_REQUIRE(dim * element % 16 == 0 && page_stride * element % 16 == 0 && page_head_stride * element % 16 == 0 && aligned_to(k_pages, 16) &&
                   aligned_to(v_pages, 16),
               DTN_ERR_INVALID, "paged attention: the heads of the pools must start on 16-byte boundaries and have a multiple of 16 bytes");
-  DTN_REQUIRE(q && out && lengths && (rows || count <= sequences), DTN_ERR_INVALID, "paged attention: null pointer");
+  DTN_REQUIRE(q && out && (lengths || sequences == 0) && (rows || count <= sequences), DTN_ERR_INVALID, "paged attention: null pointer");
   DTN_REQUIRE((k_pages && v_pages) || pages == 0, DTN_ERR_INVALID, "paged attention: null pool");
   DTN_REQUIRE(sequences == 0 || tables || pages_per_sequence == 0, DTN_ERR_INVALID, "paged attention: null tables");
   DTN_REQUIRE(pages < (1LL << 31) && count < (1LL << 31) && q_heads < (1LL << 20) && pages_per_sequence < (1LL << 31), DTN_ERR_UNSUPPORTED,

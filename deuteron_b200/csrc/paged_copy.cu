@@ -12,18 +12,46 @@ struct CopyParams {
   int* status;
 };
 
-// One block per (pair, plane); V is the widest vector that divides every address and extent.
-template <typename V>
-__global__ void __launch_bounds__(256) copy_pages_kernel(const CopyParams p) {
-  const int64_t pair = blockIdx.x % p.pairs, plane = blockIdx.x / p.pairs;
+// GROUP threads copy one page of one plane, COPY_AHEAD vectors each at a time, all requested before the first is stored; V is
+// the widest vector that divides every address and extent.
+constexpr int COPY_THREADS = 256;
+constexpr int COPY_AHEAD = 8;
+
+template <typename V, int GROUP>
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const CopyParams p) {
+  const int64_t page = (int64_t)blockIdx.x * (COPY_THREADS / GROUP) + threadIdx.x / GROUP;
+  if (page >= p.pairs * p.planes) return;
+  const int64_t plane = page / p.pairs, pair = page - plane * p.pairs;
+  const int lane = threadIdx.x % GROUP;
   const int from = p.sources[pair], to = p.destinations[pair];
   if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
-    if (threadIdx.x == 0) paged_report(p.status, PAGED_STATUS_COPY);
+    if (lane == 0) paged_report(p.status, PAGED_STATUS_COPY);
     return;
   }
   const V* src = reinterpret_cast<const V*>(p.pool + plane * p.plane_stride + from * p.page_stride);
   V* dst = reinterpret_cast<V*>(p.pool + plane * p.plane_stride + to * p.page_stride);
-  for (int64_t i = threadIdx.x; i < p.page_bytes / (int64_t)sizeof(V); i += blockDim.x) dst[i] = src[i];
+  const int64_t vectors = p.page_bytes / (int64_t)sizeof(V);
+  for (int64_t i = lane; i < vectors; i += COPY_AHEAD * GROUP) {
+    V x[COPY_AHEAD];
+#pragma unroll
+    for (int j = 0; j < COPY_AHEAD; ++j)
+      if (i + j * GROUP < vectors) x[j] = src[i + j * GROUP];
+#pragma unroll
+    for (int j = 0; j < COPY_AHEAD; ++j)
+      if (i + j * GROUP < vectors) dst[i + j * GROUP] = x[j];
+  }
+}
+
+template <typename V>
+static int copy_pages_launch(const CopyParams& p, cudaStream_t s) {
+  const int64_t pages = p.pairs * p.planes;
+  // a block per page, or a warp where a block's threads would have less than two vectors each
+  if (p.page_bytes / (int64_t)sizeof(V) >= 2 * COPY_THREADS)
+    copy_pages_kernel<V, COPY_THREADS><<<(unsigned)pages, COPY_THREADS, 0, s>>>(p);
+  else
+    copy_pages_kernel<V, 32><<<(unsigned)((pages + COPY_THREADS / 32 - 1) / (COPY_THREADS / 32)), COPY_THREADS, 0, s>>>(p);
+  DTN_LAUNCH_CHECK("copy_pages_kernel");
+  return DTN_OK;
 }
 
 }  // namespace dtn
@@ -39,13 +67,7 @@ extern "C" int dtn_copy_pages(void* pool, int64_t planes, int64_t plane_stride_b
   CopyParams p = {static_cast<char*>(pool), plane_stride_bytes, page_stride_bytes, page_bytes, planes, pages, pairs, sources, destinations,
                   device_status_word_unless_capturing(s)};
   const uint64_t all = reinterpret_cast<uintptr_t>(pool) | (uint64_t)plane_stride_bytes | (uint64_t)page_stride_bytes | (uint64_t)page_bytes;
-  const unsigned blocks = (unsigned)(planes * pairs);
-  if (all % 16 == 0)
-    copy_pages_kernel<uint4><<<blocks, 256, 0, s>>>(p);
-  else if (all % 4 == 0)
-    copy_pages_kernel<uint32_t><<<blocks, 256, 0, s>>>(p);
-  else
-    copy_pages_kernel<uint8_t><<<blocks, 256, 0, s>>>(p);
-  DTN_LAUNCH_CHECK("copy_pages_kernel");
-  return DTN_OK;
+  if (all % 16 == 0) return copy_pages_launch<uint4>(p, s);
+  if (all % 4 == 0) return copy_pages_launch<uint32_t>(p, s);
+  return copy_pages_launch<uint8_t>(p, s);
 }

@@ -353,12 +353,12 @@ _LAYOUTS = {'half': 0, 'interleaved': 1}
 
 
 def _on_current_device(*tensors: torch.Tensor) -> None:
-    if not all([tensor.is_cuda for tensor in tensors]):
-        raise ValueError('deuteron_b200 operators take CUDA tensors')
-    current = torch.cuda.current_device()
+    current = torch.cuda.current_device() if tensors[0].is_cuda else None
     for tensor in tensors:
         if tensor.get_device() != current:
-            raise ValueError(f'a tensor is on {tensor.device}, the current device is cuda:{current}')
+            if not tensor.is_cuda:
+                raise ValueError('deuteron_b200 operators take CUDA tensors')
+            raise ValueError(f'a tensor is on {tensor.device}, the current device is {torch.cuda.current_device()}')
 
 
 def _tensors(*tensors: torch.Tensor) -> None:
@@ -369,9 +369,12 @@ def _tensors(*tensors: torch.Tensor) -> None:
 
 def _heads(tensor: torch.Tensor, label: str, written: bool = False) -> tuple[int, int]:
     """Token and head strides of a [tokens, heads, dim] tensor with dense heads (0 for an extent of one)."""
-    if tensor.dim() != 3:
+    shape = tensor.shape
+    if len(shape) != 3:
         raise ValueError(f'{label} must be a [tokens, heads, dim] tensor')
-    tokens, heads, dim = tensor.shape
+    tokens, heads, dim = shape
+    if tensor.is_contiguous():
+        return heads * dim if tokens > 1 else 0, dim if heads > 1 else 0
     token_stride, head_stride, unit = tensor.stride()
     if dim > 1 and unit != 1:
         raise ValueError(f'{label} must have dense heads (unit stride in its last dimension)')
@@ -382,12 +385,13 @@ def _heads(tensor: torch.Tensor, label: str, written: bool = False) -> tuple[int
 
 
 def _index(tensor: torch.Tensor, label: str, count: int | None = None, wide: bool = False) -> None:
-    if not isinstance(tensor, torch.Tensor) or tensor.dim() != 1 or not tensor.is_contiguous():
+    dtype, shape = tensor.dtype, tensor.shape
+    if len(shape) != 1 or not tensor.is_contiguous():
         raise ValueError(f'{label} must be a contiguous 1-D tensor')
-    if tensor.dtype != torch.int32 and not (wide and tensor.dtype == torch.int64):
-        raise ValueError(f'{label} must have dtype {"int32 or int64" if wide else "int32"}, got {tensor.dtype}')
-    if count is not None and tensor.shape[0] != count:
-        raise ValueError(f'{label} must have {count} entries, got {tensor.shape[0]}')
+    if dtype is not torch.int32 and not (wide and dtype is torch.int64):
+        raise ValueError(f'{label} must have dtype {"int32 or int64" if wide else "int32"}, got {dtype}')
+    if count is not None and shape[0] != count:
+        raise ValueError(f'{label} must have {count} entries, got {shape[0]}')
 
 
 def _rotation(frequencies: torch.Tensor | None, layout: str, dim: int) -> int:
@@ -415,16 +419,21 @@ def _pools(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor) -
     pages, heads, size, dim = shape
     if size < 1:
         raise ValueError('a page holds at least one token')
-    strides = k_pages.stride()
-    page, head, token, unit = strides
-    if (dim > 1 and unit != 1) or (size > 1 and token != dim):
-        raise ValueError('the rows of one page and head must be dense in k_pages and v_pages')
-    if strides != v_pages.stride():   # strides of extents of one are nobody's business
-        if any(extent > 1 and a != b for extent, a, b in zip(shape, strides, v_pages.stride())):
-            raise ValueError('k_pages and v_pages must have the same strides')
+    if k_pages.is_contiguous() and v_pages.is_contiguous():
+        head = size * dim
+        page = heads * head
+    else:
+        strides = k_pages.stride()
+        page, head, token, unit = strides
+        if (dim > 1 and unit != 1) or (size > 1 and token != dim):
+            raise ValueError('the rows of one page and head must be dense in k_pages and v_pages')
+        if strides != v_pages.stride():   # strides of extents of one are nobody's business
+            if any(extent > 1 and a != b for extent, a, b in zip(shape, strides, v_pages.stride())):
+                raise ValueError('k_pages and v_pages must have the same strides')
     if tables.dtype != torch.int32 or tables.dim() != 2:
         raise ValueError('tables must be a [sequences, pages per sequence] int32 tensor')
-    (sequences, width), (row, column) = tables.shape, tables.stride()
+    sequences, width = tables.shape
+    row, column = tables.stride()
     if width > 1 and column != 1:
         raise ValueError('tables must have unit column stride')
     return pages, heads, size, dim, page if pages > 1 else 0, head if heads > 1 else 0, sequences, width, row if sequences > 1 else 0
@@ -485,7 +494,7 @@ def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> tor
     _on_current_device(x, positions, frequencies, out)
     native.call('dtn_rotary', x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(),
                 tokens, heads, dim, pairs, token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose,
-                amplitude, _STORAGE_OF[x.dtype], _stream())
+                float(amplitude), _STORAGE_OF[x.dtype], _stream())
     return out
 
 
@@ -556,7 +565,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     native.call('dtn_paged_append', k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(),
                 positions.data_ptr(), positions.dtype == torch.int64, tokens, kv_heads, dim, k_token, k_head, v_token, v_head, pages, page_size,
                 page_stride, page_head_stride, sequences, width, table_stride, frequencies.data_ptr() if pairs else None, pairs,
-                _LAYOUTS[layout], amplitude, q.data_ptr() if q_heads else None, q_out.data_ptr() if q_heads else None, q_heads, q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
+                _LAYOUTS[layout], float(amplitude), q.data_ptr() if q_heads else None, q_out.data_ptr() if q_heads else None, q_heads,
+                q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
     return q_out
 
 
@@ -611,8 +621,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _index(rows, 'rows', count)
     elif count > sequences:
         raise ValueError(f'{count} queries but {sequences} sequences')
-    if window < 0:
-        raise ValueError('window must not be negative')
+    if type(window) is not int or window < 0:
+        raise ValueError(f'window must be a non-negative integer, got {window!r}')
     if out is None:
         out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)
     _tensors(out)
@@ -634,24 +644,24 @@ def copy_pages(pages: torch.Tensor, sources: torch.Tensor, destinations: torch.T
     be a source. A page number outside the pool copies nothing and makes `check_device_status` raise PageError.
     """
     _tensors(pages, sources, destinations)
-    if not 4 <= pages.dim() <= 6:
+    shape = pages.shape
+    if not 4 <= len(shape) <= 6:
         raise ValueError('pages must be a [pages, kv_heads, page_size, dim] tensor, or one with one or two leading dimensions')
-    heads, size, dim = pages.shape[-3:]
-    dense = 1
-    for extent, stride in zip((dim, size, heads), reversed(pages.stride()[-3:])):
-        if extent > 1 and stride != dense:
-            raise ValueError('the values of one page must be dense')
-        dense *= extent
-    planes, plane_stride = 1, 0
-    for extent, stride in zip(reversed(pages.shape[:-4]), reversed(pages.stride()[:-4])):
-        if planes > 1 and extent > 1 and stride != planes * plane_stride:
+    count, heads, size, dim = shape[-4:]
+    dense, planes = heads * size * dim, math.prod(shape[:-4])
+    page_stride, plane_stride = dense, count * dense
+    if not pages.is_contiguous():
+        strides = pages.stride()
+        for extent, stride, expected in zip(shape[-3:], strides[-3:], (size * dim, dim, 1)):
+            if extent > 1 and stride != expected:
+                raise ValueError('the values of one page must be dense')
+        page_stride = strides[-4] if count > 1 else dense
+        leading = [(extent, stride) for extent, stride in zip(shape[:-4], strides[:-4]) if extent > 1]
+        plane_stride = leading[-1][1] if leading else 0
+        if len(leading) == 2 and leading[0][1] != leading[1][0] * plane_stride:
             raise ValueError('the leading dimensions of pages must be evenly spaced')
-        plane_stride = plane_stride if planes > 1 or extent <= 1 else stride
-        planes *= extent
-    count = pages.shape[-4]
-    page_stride = pages.stride(-4) if count > 1 else 0
-    if dense and ((count > 1 and page_stride < dense) or (planes > 1 and plane_stride == 0)):
-        raise ValueError('pages must not be an expanded tensor: it is written')
+        if dense and (page_stride < dense or (planes > 1 and plane_stride == 0)):
+            raise ValueError('pages must not be an expanded tensor: it is written')
     _index(sources, 'sources')
     _index(destinations, 'destinations', sources.shape[0])
     _on_current_device(pages, sources, destinations)

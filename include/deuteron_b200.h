@@ -342,7 +342,8 @@ int dtn_rotary(const void* x, void* out, const void* positions, int positions_64
  * page tables[r * table_stride + p / page_size] at place p % page_size. Token t is stored at positions[t] of sequence rows[t];
  * a negative row stores nothing (padding). k and v are [tokens, kv_heads, dim]; q (q_heads of them, 0 for none) is rotated by
  * the same positions into q_out, which may be q itself. A row >= sequences, a position outside the tables or a page number
- * outside the pool stores nothing and is reported by dtn_device_status. Two tokens for one place: either may stay. */
+ * outside the pool stores nothing and is reported by dtn_device_status (not where the first call on a device is being captured:
+ * the status word is allocated outside captures). Two tokens for one place: either may stay. */
 int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int* tables, const int* rows, const void* positions,
                      int positions_64, int64_t tokens, int64_t kv_heads, int64_t dim, int64_t k_token_stride, int64_t k_head_stride,
                      int64_t v_token_stride, int64_t v_head_stride, int64_t pages, int64_t page_size, int64_t page_stride,

@@ -6,6 +6,7 @@ import torch
 
 import paged_math as M
 from deuteron_b200 import native, ops
+from deuteron_b200.paged import PagedCache, PagesExhausted
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
@@ -411,3 +412,106 @@ def test_captured_graphs_share_no_workspace(cuda):
     for out, x in zip(outs, q):
         exact, bound = M.attend(x, k_pages, v_pages, tables, lens, 0.125)
         within(out, exact, bound)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_prompts_steps_forks_and_compaction_together(cuda, layout, dtype):
+    # a decoder's use: prompts, steps, a fork into three, a close, compaction, drafts that are taken back. Beside it every
+    # sequence's keys and values are kept whole, and every step's attention is held to the 64-bit form over them
+    layers, q_heads, kv_heads, dim, size = 2, 6, 2, 64, 8
+    cache = PagedCache(layers=layers, pages=30, page_size=size, kv_heads=kv_heads, head_dim=dim, max_sequences=6, max_pages_per_sequence=12, dtype=dtype)
+    cache.pool.fill_(float('nan'))
+    w, amplitude = ops.rotary_frequencies(48, scaling='yarn', factor=4.0, original_length=64)
+    g = torch.Generator(device='cuda').manual_seed(5)
+    kept = {}   # row: per layer a list of (key, value) rows
+
+    def step(rows, counts):
+        token_rows, positions = cache.extend(rows, counts)
+        n = token_rows.numel()
+        results = []
+        for layer in range(layers):
+            q, k, v = torch.randn(n, q_heads + 2 * kv_heads, dim, device='cuda', generator=g).to(dtype).split([q_heads, kv_heads, kv_heads], dim=1)
+            turned = cache.append(layer, k, v, token_rows, positions, frequencies=w, layout=layout, amplitude=amplitude, q=q)
+            keys = ops.rotary(k, positions, w, layout=layout, amplitude=amplitude)
+            assert torch.equal(turned, ops.rotary(q, positions, w, layout=layout, amplitude=amplitude))
+            for i, row in enumerate(token_rows.tolist()):
+                kept[row][layer].append((keys[i], v[i]))
+            results.append(turned)
+        return token_rows, results
+
+    def check(token_rows, queries):
+        last = {row: i for i, row in enumerate(token_rows.tolist())}
+        rows = sorted(last)
+        for layer in range(layers):
+            q = queries[layer][[last[row] for row in rows]]
+            y = cache.attend(layer, q, M.scale_of(dim), rows=torch.tensor(rows, dtype=torch.int32).cuda())
+            for i, row in enumerate(rows):
+                k = torch.stack([pair[0] for pair in kept[row][layer]]).transpose(0, 1)[None]
+                v = torch.stack([pair[1] for pair in kept[row][layer]]).transpose(0, 1)[None]
+                exact, bound = M.attend(q[i:i + 1], k, v, torch.zeros(1, 1, dtype=torch.int32).cuda(), [k.shape[2]], M.scale_of(dim))
+                within(y[i:i + 1], exact, bound)
+
+    a, b = cache.open(), cache.open()
+    kept[a], kept[b] = [[] for _ in range(layers)], [[] for _ in range(layers)]
+    check(*step([a, b], [13, 30]))
+    for _ in range(3):
+        check(*step([b, a], [1, 1]))
+    forks = [cache.fork(a) for _ in range(2)]
+    for row in forks:
+        kept[row] = [list(layer) for layer in kept[a]]
+    for _ in range(9):
+        check(*step([a, *forks], [1, 1, 1]))
+    cache.close(b)
+    del kept[b]
+    assert cache.compact() > 0
+    assert int(cache.tables[sorted(kept)].max()) < 30 - cache.book.free_pages
+    check(*step([forks[1], a], [1, 5]))
+    cache.truncate(a, 11)
+    kept[a] = [layer[:11] for layer in kept[a]]
+    check(*step([a, forks[0]], [2, 1]))
+    with pytest.raises(PagesExhausted):
+        cache.extend([a, *forks], [70, 70, 70])
+    with pytest.raises(ValueError):
+        cache.extend([a], [100])
+    check(*step([a, *forks], [1, 1, 1]))
+
+
+def test_a_captured_step_follows_the_cache(cuda):
+    cache = PagedCache(layers=1, pages=64, page_size=16, kv_heads=2, head_dim=64, max_sequences=4)
+    w, _ = ops.rotary_frequencies(64)
+    rows = [cache.open() for _ in range(3)]
+    token_rows, positions = cache.extend(rows, [40, 7, 100])
+    fill = torch.randn(147, 2, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    cache.append(0, fill, fill.flip(0), token_rows, positions, frequencies=w)
+    batch_rows = torch.full((4,), -1, dtype=torch.int32, device='cuda')       # one slot is padding
+    batch_positions = torch.zeros(4, dtype=torch.int32, device='cuda')
+    q, k, v = (torch.zeros(4, heads, 64, dtype=torch.float16, device='cuda') for heads in (8, 2, 2))
+
+    def body():
+        turned = cache.append(0, k, v, batch_rows, batch_positions, frequencies=w, q=q)
+        return cache.attend(0, turned, 0.125, rows=batch_rows)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        body()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = body()
+    for i in range(20):
+        if i == 10:
+            cache.close(rows[1])
+            rows[1] = cache.fork(rows[0])
+            cache.compact()
+        token_rows, positions = cache.extend(rows, [1, 1, 1])
+        batch_rows[:3], batch_positions[:3] = token_rows, positions
+        for n, x in enumerate((q, k, v)):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(10 * i + n)).half())
+        graph.replay()
+        eager = body()                                                        # writes the same keys and values again
+        assert torch.equal(captured, eager) and not captured[3].any()
+        turned = ops.rotary(q, batch_positions, w)
+        exact, bound = M.attend(turned[:3], cache.keys(0), cache.values(0), cache.tables, cache.lengths, 0.125, rows=rows)
+        within(captured[:3], exact, bound)

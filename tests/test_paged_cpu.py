@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from deuteron_b200 import native, ops
+from deuteron_b200.paged import PageBook, PagedCache, PagesExhausted
 
 
 def cache(dtype=torch.float16, pages=4, heads=2, size=8, dim=16):
@@ -201,3 +202,123 @@ def test_page_reports_have_their_own_error(monkeypatch):
     monkeypatch.setattr(native, 'device_status', lambda stream=0: 0x7100)
     with pytest.raises(native.DeviceWaitError, match='self-test'):
         native.raise_on_device_status(0)
+
+
+def check_book(book):
+    """Counts of references are what the tables say; a page is free or held; rows are free or open."""
+    held = [book.tables[row, :-(-int(book.lengths[row]) // book.page_size)].tolist() for row in range(len(book.lengths)) if book._open[row]]
+    counted = [0] * len(book.references)
+    for pages in held:
+        assert len(set(pages)) == len(pages)
+        for page in pages:
+            counted[page] += 1
+    assert counted == book.references.tolist()
+    assert sorted(book._free_pages) == [page for page, n in enumerate(counted) if n == 0] and book.free_pages == len(book._free_pages)
+    assert sorted(book._free_rows) == [row for row, is_open in enumerate(book._open) if not is_open]
+
+
+@pytest.mark.parametrize('seed', range(6))
+def test_the_book_keeps_every_sequence_whole(seed):
+    # a model: every sequence's tokens as a list, the pool as one; random calls, the copies applied as the device would
+    generator = random.Random(seed)
+    size = generator.choice([1, 3, 4, 16])
+    book = PageBook(pages=24, page_size=size, max_sequences=7, max_pages_per_sequence=9)
+    pool, tables, tokens, next_token = [[None] * size for _ in range(24)], [[0] * 9 for _ in range(7)], {}, 0
+    for _ in range(400):
+        call = generator.choice(['open', 'close', 'fork', 'extend', 'extend', 'extend', 'truncate', 'compact'])
+        copies, updates, written = [], [], []
+        state = (book.tables.copy(), book.lengths.copy(), book.references.copy(), sorted(book._free_pages))
+        try:
+            if call == 'open':
+                tokens[book.open()] = []
+            elif call == 'compact':
+                copies, updates = book.compact()
+                used = int((book.references > 0).sum())
+                assert not book.references[used:].any()
+            elif not tokens:
+                continue
+            elif call == 'close':
+                row = generator.choice(sorted(tokens))
+                book.close(row)
+                del tokens[row]
+            elif call == 'fork':
+                row = generator.choice(sorted(tokens))
+                new, updates = book.fork(row)
+                tokens[new] = list(tokens[row])
+            elif call == 'truncate':
+                row = generator.choice(sorted(tokens))
+                kept = generator.randint(0, len(tokens[row]))
+                book.truncate(row, kept)
+                del tokens[row][kept:]
+            else:
+                rows = generator.sample(sorted(tokens), generator.randint(1, len(tokens)))
+                counts = [generator.choice([0, 1, 1, 2, size, 2 * size + 1]) for _ in rows]
+                copies, updates = book.extend(rows, counts)
+                for row, count in zip(rows, counts):
+                    for _ in range(count):
+                        written.append((row, len(tokens[row]), next_token))
+                        tokens[row].append(next_token)
+                        next_token += 1
+        except (PagesExhausted, ValueError):
+            after = (book.tables.copy(), book.lengths.copy(), book.references.copy(), sorted(book._free_pages))
+            assert all((a == b).all() for a, b in zip(state[:3], after[:3])) and state[3] == after[3]
+            continue
+        destinations = [to for _, to in copies]
+        assert len(set(destinations)) == len(destinations) and not set(destinations) & {source for source, _ in copies}
+        for source, to in copies:
+            pool[to] = list(pool[source])
+        assert len({(row, column) for row, column, _ in updates}) == len(updates)
+        for row, column, page in updates:
+            tables[row][column] = page
+        for row, position, value in written:
+            pool[tables[row][position // size]][position % size] = value
+        check_book(book)
+        for row, expected in tokens.items():
+            assert int(book.lengths[row]) == len(expected)
+            assert [pool[tables[row][i // size]][i % size] for i in range(len(expected))] == expected, call
+            assert tables[row][:-(-len(expected) // size)] == book.tables[row, :-(-len(expected) // size)].tolist()
+
+
+def test_the_book_refuses():
+    for arguments in ((0, 4, 1, 1), (1, 0, 1, 1), (1, 4, 0, 1), (1, 4, 1, 0), (1, 4.0, 1, 1), (1, 2 ** 20, 1, 2 ** 11), (1, 1, 2 ** 20, 2 ** 11)):
+        with pytest.raises(ValueError):
+            PageBook(*arguments)
+    book = PageBook(pages=3, page_size=4, max_sequences=2, max_pages_per_sequence=3)
+    row = book.open()
+    for call in (lambda: book.close(1), lambda: book.fork(-1), lambda: book.extend([row, row], [1, 1]), lambda: book.extend([row], [-1]),
+                 lambda: book.extend([row], [1, 2]), lambda: book.extend([row], [13]), lambda: book.truncate(row, 1), lambda: book.truncate(row, -1)):
+        with pytest.raises(ValueError):
+            call()
+    book.extend([row], [6])
+    other, _ = book.fork(row)
+    with pytest.raises(PagesExhausted):
+        book.open()
+    with pytest.raises(PagesExhausted):
+        book.extend([row, other], [2, 3])     # a copy of the shared page is the last free one; a third page is missing
+    copies, _ = book.extend([row, other], [2, 2])
+    assert copies == [(1, 2)] and book.free_pages == 0
+    book.close(other)
+    with pytest.raises(ValueError):
+        book.close(other)
+    check_book(book)
+
+
+def test_the_cache_brings_the_device_up_to_date():
+    cache = PagedCache(layers=2, pages=6, page_size=4, kv_heads=2, head_dim=16, max_sequences=3, max_pages_per_sequence=4, device='cpu')
+    a, b = cache.open(), cache.open()
+    rows, positions = cache.extend([a, b], [5, 3])
+    assert rows.tolist() == [a] * 5 + [b] * 3 and positions.tolist() == [0, 1, 2, 3, 4, 0, 1, 2] and rows.dtype == positions.dtype == torch.int32
+    rows, positions = cache.extend([b, a], [0, 1])
+    assert rows.tolist() == [a] and positions.tolist() == [5]
+    assert [t.numel() for t in cache.extend([], [])] == [0, 0]
+    c = cache.fork(a)
+    cache.truncate(c, 4)
+    assert cache.lengths.tolist() == [6, 3, 4] and torch.equal(cache.tables, torch.from_numpy(cache.book.tables))
+    cache.close(b)
+    assert cache.lengths.tolist() == [6, 0, 4]
+    assert cache.keys(1).data_ptr() == cache.pool[1, 0].data_ptr() and cache.values(0).shape == (6, 2, 4, 16)
+    for changed in (dict(dtype=torch.float64), dict(head_dim=12), dict(head_dim=264), dict(layers=0), dict(kv_heads=-1)):
+        with pytest.raises(ValueError):
+            PagedCache(**{**dict(layers=2, pages=6, page_size=4, kv_heads=2, head_dim=16, max_sequences=3, device='cpu'), **changed})
+    with pytest.raises(ValueError, match='CUDA'):
+        cache.attend(0, torch.zeros(3, 2, 16, dtype=torch.float16), 1.0)
