@@ -59,7 +59,7 @@ struct PagedAttentionParams {
 };
 
 // Units for the end of an item: the teams' parts are added, the result written, the next query taken.
-constexpr int PA_ITEM_UNITS = 2;
+constexpr int PA_ITEM_UNITS = 3;
 constexpr int PA_JOIN = 16;
 
 // First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
@@ -369,20 +369,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * HB) : "memory");
   };
 
-  auto fill = [&]() {
-    if (ahead.left > 0) look_up();
-#pragma unroll 1
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (ahead.left > 0) {
-        copy(i);
-        ahead.step(p);
-        if (ahead.left > 0) look_up();
-      }
-      pa_commit();
-    }
-  };
-  fill();
-
   // -- queries ------------------------------------------------------------------------------------
   constexpr int STEPS_K = DP / 16;
   uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF && DP < 256 ? STEPS_K : 1][2];
@@ -392,25 +378,26 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
     // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
     const int h = head_of(block, member * 8 + g);
     const bool there = h < p.group;
-    const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)kv_head * p.group + (there ? h : 0)) * p.q_head_stride;
+    const T* q = static_cast<const T*>(p.q) + sequence * p.q_token_stride + ((int64_t)kv_head * p.group + (there ? h : 0)) * p.q_head_stride + 2 * t;
+    if (p.q_pairs && p.dim == DP) {
 #pragma unroll
-    for (int ks = 0; ks < STEPS_K; ++ks) {
+      for (int i = 0; i < 2 * STEPS_K; ++i) to[i / 2][i % 2] = there ? *reinterpret_cast<const uint32_t*>(q + i * 8) : 0u;
+    } else {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int d = ks * 16 + half * 8 + 2 * t;
+      for (int i = 0; i < 2 * STEPS_K; ++i) {
         uint32_t v = 0;
-        if (there && d < p.dim) {   // dim is even
+        if (there && i * 8 + 2 * t < p.dim) {   // dim is even
           if (p.q_pairs)
-            v = *reinterpret_cast<const uint32_t*>(q + d);
+            v = *reinterpret_cast<const uint32_t*>(q + i * 8);
           else
-            v = *reinterpret_cast<const uint16_t*>(q + d) | (uint32_t) * reinterpret_cast<const uint16_t*>(q + d + 1) << 16;
+            v = *reinterpret_cast<const uint16_t*>(q + i * 8) | (uint32_t) * reinterpret_cast<const uint16_t*>(q + i * 8 + 1) << 16;
         }
-        to[ks][half] = v;
+        to[i / 2][i % 2] = v;
       }
     }
   };
-  if (now.left <= 0) return;   // nothing but the ends of items
-  if constexpr (C::HALF && DP < 256) load_query(query_next, now.sequence, now.kv_head, now.block);
+  if constexpr (C::HALF && DP < 256)
+    if (now.left > 0) load_query(query_next, now.sequence, now.kv_head, now.block);
 
   // -- the pass over the tokens -------------------------------------------------------------------
   constexpr int COLUMNS = DP / 32;                 // FP32 storage: columns of V per lane
@@ -418,17 +405,23 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   constexpr int A = C::HALF ? DP / 16 : NH, B = C::HALF ? 4 : COLUMNS;
   float acc[A][B];                                 // numerators: 16 columns of V by 2 heads, or NH heads by COLUMNS
   bool fresh = true, exactly = false;
-  int start = 0, slot = 0;                         // the item's first tile here; the stage read next
+  int start = 0;                                   // the item's first tile here
+  int slot = 0, filling = STAGES - 1;              // the oldest stage; copies still to be issued before the first stage is read
 
+  if (ahead.left > 0) look_up();
   while (now.left > 0) {
     pa_wait<STAGES - 2>();
-    team_barrier();
+    team_barrier();   // the oldest stage is there, and the one before it has been read by all
     if (ahead.left > 0) {
-      copy(slot == 0 ? STAGES - 1 : slot - 1);
+      copy(filling > 0 ? STAGES - 1 - filling : (slot == 0 ? STAGES - 1 : slot - 1));
       ahead.step(p);
       if (ahead.left > 0) look_up();
     }
     pa_commit();
+    if (filling > 0) {
+      --filling;
+      continue;
+    }
 
     if (fresh) {
       fresh = false;
@@ -689,10 +682,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           now.left += now.tile - start;
           now.tile = start;
           ahead = now;
-          fill();
+          look_up();
           if constexpr (DP < 256) load_query(query_next, now.sequence, now.kv_head, now.block);
           exactly = fresh = true;
           slot = 0;
+          filling = STAGES - 1;
           continue;
         }
         exactly = false;
@@ -736,7 +730,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           weight_sum = fmaf(weight, s_sum[w][slot_head % 8], weight_sum);
         }
         if (whole) {
-          write(h, d, make_float4(y.x / weight_sum, y.y / weight_sum, y.z / weight_sum, y.w / weight_sum));
+          const float share = 1.f / weight_sum;
+          write(h, d, make_float4(y.x * share, y.y * share, y.z * share, y.w * share));
         } else {
           __stcg(reinterpret_cast<float4*>(part + slot_head * DP + d), y);
           if (d == 0) {
@@ -791,7 +786,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
                 sum_p = fmaf(weight, part_sum[j], sum_p);
               }
             }
-            write(h, d, make_float4(y.x / sum_p, y.y / sum_p, y.z / sum_p, y.w / sum_p));
+            const float share = 1.f / sum_p;
+            write(h, d, make_float4(y.x * share, y.y * share, y.z * share, y.w * share));
           }
         }
       }

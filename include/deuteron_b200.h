@@ -373,7 +373,7 @@ int dtn_paged_attention_workspace_bytes(size_t* bytes_out /* host */);
 
 /* How dtn_paged_attention cuts a batch among its blocks: host arithmetic only (the kernel does the same on the device from the
  * lengths). Sequence i has tiles[i] tiles of tokens for each of `heads` items (kv heads x blocks of query heads); an item has
- * a unit for each of its tiles and two for its end, none without tiles. The units, tile fastest, then item, then sequence, are
+ * a unit for each of its tiles and three for its end, none without tiles. The units, tile fastest, then item, then sequence, are
  * cut into *workers_out contiguous ranges [begin_out[c], begin_out[c + 1]), as many as `grid` allows with at least min_units
  * each. first_out / last_out (count * heads entries) are the blocks that hold an item's first and last tile (-1 without tiles);
  * the parts of an item are added in that order. Output pointers may be NULL; begin_out needs grid + 1 entries. */

@@ -158,7 +158,7 @@ def test_the_plan_covers_every_unit_once_and_names_its_owners():
         items = len(tiles) * heads
         begin, first, last, workers = ((ctypes.c_int64 * n)() for n in (grid + 1, items, items, 1))
         native.call('dtn_paged_attention_plan', (ctypes.c_int64 * len(tiles))(*tiles), len(tiles), heads, least, grid, begin, first, last, workers)
-        count, units = workers[0], sum(n + 2 for n in tiles if n) * heads
+        count, units = workers[0], sum(n + 3 for n in tiles if n) * heads
         if not units:
             assert count == 0 and set(first) == set(last) == {-1}
             continue
@@ -175,7 +175,7 @@ def test_the_plan_covers_every_unit_once_and_names_its_owners():
             assert (first[item], last[item]) == (owners[0], owners[-1]) and owners == list(range(owners[0], owners[-1] + 1))
             if len(owners) > 1:
                 started.append(first[item])
-            at = end + 2
+            at = end + 3
         assert len(set(started)) == len(started)          # one counter per block is enough: no two split items start in one block
     assert native.lib().dtn_paged_attention_plan((ctypes.c_int64 * 1)(-1), 1, 1, 1, 1, None, None, None, None) == native.ERR_INVALID
 
