@@ -51,7 +51,7 @@ struct PagedAttentionParams {
   float scale_log2e;
   int out_f32;
   int q_pairs, out_quads;               // neighbouring elements of q and out can be moved by two (4 bytes) and by four
-  int whole_sets;                       // the tokens of a set lie in one page, one after another, and fill their rows in shared memory
+  int whole_sets;                       // the tokens of a set lie in one page, one after another
   int min_units;                        // a block takes at least this many units
   int* counters;
   float* parts;
@@ -60,7 +60,7 @@ struct PagedAttentionParams {
 
 // Units for the end of an item: the teams' parts are added, the result written, the next query taken.
 constexpr int PA_ITEM_UNITS = 3;
-constexpr int PA_JOIN = 16;
+constexpr int PA_JOIN = 8;
 
 // First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
 __host__ __device__ __forceinline__ int64_t pa_share_begin(int64_t units, int64_t workers, int64_t c) { return units * c / workers; }
@@ -84,14 +84,14 @@ struct PaConfig {
   static constexpr int TEAMS = PA_WARPS / HB;
   static constexpr int ROW = DP * (int)sizeof(T);
   static constexpr int STAGE = 2 * CHUNK * ROW;          // keys, then values: 64 * DP * SETS bytes; at an item's end numerators of HB x 8 heads
-  static constexpr int RING = (DP == 256 ? 192 : 96) * 1024;
+  static constexpr int RING = (DP == 256 ? 192 : 64) * 1024;
   static constexpr int STAGES = RING / (TEAMS * STAGE);
   static constexpr int QUERY = HALF ? 0 : HB * NH * DP * 4;
   static constexpr int SMEM = RING + QUERY;
-  static constexpr int BLOCKS_PER_SM = DP == 256 ? 1 : 2;
+  static constexpr int BLOCKS_PER_SM = DP == 256 ? 1 : (HALF || HB == 1 ? 3 : 2);   // 168 registers and 64 KB for three
   static constexpr int HEADS = 8 * HB;                   // query heads of an item (the first NH of each 8 are looked at)
-  static constexpr int PART = HEADS * DP + 2 * HEADS;    // floats: numerators, maxima, sums
-  static_assert(STAGES >= 3 && STAGE >= HEADS * DP * 4, "a ring of three stages, numerators that fit one");
+  static constexpr int PART = HEADS * DP + 2 * HEADS;    // floats: numerators, then maximum and sum of each head
+  static_assert(STAGES >= 2 && STAGE >= HEADS * DP * 4, "a ring of two stages, numerators that fit one");
 };
 
 __device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src, int bytes) {
@@ -194,7 +194,7 @@ __device__ __forceinline__ int64_t pa_item_units(int tiles) { return tiles > 0 ?
 // A place in the order of the units, always a tile.
 template <int UNIT>
 struct PaCursor {
-  int64_t sequence;
+  int sequence;
   int left;                      // units of the share from here on
   int kv_head, block;            // block of query heads
   int tile, tiles;
@@ -234,6 +234,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   __shared__ __align__(16) float s_p[C::HALF ? 1 : PA_WARPS][C::HALF ? 1 : CHUNK][NH], s_alpha[C::HALF ? 1 : PA_WARPS][8];
   __shared__ int64_t s_scan[PA_WARPS];
   __shared__ int64_t s_start[2];
+  __shared__ int64_t s_plan[3];                    // units, workers and the share's end: for the end of an item, not worth registers
   __shared__ int s_last;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, team = warp / HB, member = warp % HB;
@@ -284,10 +285,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       at += here;
     }
   }
+  if (tid == 0) s_plan[0] = units, s_plan[1] = workers, s_plan[2] = end;
   __syncthreads();
   PaCursor<UNIT> now, ahead;
   now.left = (int)(end - begin);
-  now.sequence = s_start[0];
+  now.sequence = (int)s_start[0];
   now.enter(p);
   {
     const int item = (int)(s_start[1] / pa_item_units(now.tiles));
@@ -321,25 +323,40 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   };
   // Lane l copies vector l % LANES of rows l / LANES, + 32 / LANES, ...: their swizzled places differ by constants.
   const int lane_row = LANES <= 32 ? lane / LANES : 0, lane_column = LANES <= 32 ? lane % LANES : lane;
-  const uint8_t* const k_lane = static_cast<const uint8_t*>(p.k_pages) + lane_column * 16;
-  const uint8_t* const v_lane = static_cast<const uint8_t*>(p.v_pages) + lane_column * 16;
+  const uint8_t *k_pages = static_cast<const uint8_t*>(p.k_pages), *v_pages = static_cast<const uint8_t*>(p.v_pages);
   const uint32_t lane_place = (member * ROWS + lane_row) * ROW +
                               (C::HALF ? lane_column ^ ((member * ROWS + lane_row) & 7) : lane_column ^ (((member * ROWS + lane_row) & 1) << 2)) * 16;
   auto copy = [&](int slot) {
     const uint32_t seen_rows = __ballot_sync(0xffffffffu, offset >= 0);
     const uint32_t stage = ring_address + slot * C::STAGE;
     if (seen_rows == 0xffffffffu && p.whole_sets) {   // one page holds the rows of a set one after another: constant distances
-      constexpr int TOGETHER = ROWS < C::SUB ? ROWS : C::SUB;
+      constexpr int TOGETHER = ROWS < C::SUB ? ROWS : C::SUB, STEP = LANES <= 32 ? 32 / LANES : 1;   // rows between two copies of a lane
+      if (p.row_bytes == ROW) {
 #pragma unroll
-      for (int set = 0; set < ROWS / TOGETHER; ++set) {
-        const int64_t at = __shfl_sync(0xffffffffu, offset, set * TOGETHER) + lane_row * ROW;
+        for (int set = 0; set < ROWS / TOGETHER; ++set) {
+          const int64_t at = __shfl_sync(0xffffffffu, offset, set * TOGETHER) + (lane_row * ROW + lane_column * 16);
+          const uint8_t *k_at = k_pages + at, *v_at = v_pages + at;
 #pragma unroll
-        for (int j = 0; j < TOGETHER * LANES / 32; ++j) {
-          // rows between two copies of a lane; a row of 64 vectors takes two copies, 512 bytes apart
-          const int row = LANES <= 32 ? j * (LANES <= 32 ? 32 / LANES : 1) : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;
-          const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + (set * TOGETHER + row) * ROW + half;
-          pa_copy16(to, k_lane + at + row * ROW + half);
-          pa_copy16(to + CHUNK * ROW, v_lane + at + row * ROW + half);
+          for (int j = 0; j < TOGETHER * LANES / 32; ++j) {
+            const int row = LANES <= 32 ? j * STEP : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;   // a row of 64 vectors takes two copies
+            const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + (set * TOGETHER + row) * ROW + half;
+            pa_copy16(to, k_at + row * ROW + half);
+            pa_copy16(to + CHUNK * ROW, v_at + row * ROW + half);
+          }
+        }
+      } else {   // narrower rows: zeros in the columns past the head
+#pragma unroll
+        for (int set = 0; set < ROWS / TOGETHER; ++set) {
+          const int64_t at = __shfl_sync(0xffffffffu, offset, set * TOGETHER) + lane_row * p.row_bytes;
+#pragma unroll
+          for (int j = 0; j < TOGETHER * LANES / 32; ++j) {
+            const int row = LANES <= 32 ? j * STEP : j / 2, half = LANES <= 32 ? 0 : j % 2 * 512;
+            const uint32_t to = ((stage + lane_place) ^ (C::HALF ? (row & 7) << 4 : (row & 1) << 6)) + (set * TOGETHER + row) * ROW + half;
+            const int bytes = lane_column * 16 + half < p.row_bytes ? 16 : 0;
+            const int64_t from = bytes ? at + row * p.row_bytes + half + lane_column * 16 : 0;   // copies of nothing name the pool's start
+            pa_copy16(to, k_pages + from, bytes);
+            pa_copy16(to + CHUNK * ROW, v_pages + from, bytes);
+          }
         }
       }
       return;
@@ -358,8 +375,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       if (at == -2)   // keys of a page that does not exist are NaN, and so is all that sees them
         *reinterpret_cast<uint4*>(ring + (to - ring_address)) = make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
       else
-        pa_copy16(to, static_cast<const uint8_t*>(p.k_pages) + from, there ? 16 : 0);
-      pa_copy16(to + CHUNK * ROW, static_cast<const uint8_t*>(p.v_pages) + from, there ? 16 : 0);
+        pa_copy16(to, k_pages + from, there ? 16 : 0);
+      pa_copy16(to + CHUNK * ROW, v_pages + from, there ? 16 : 0);
     }
   };
   auto team_barrier = [&]() {
@@ -371,10 +388,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
 
   // -- queries ------------------------------------------------------------------------------------
   constexpr int STEPS_K = DP / 16;
-  uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF && DP < 256 ? STEPS_K : 1][2];
+  uint32_t query[C::HALF ? STEPS_K : 1][2], query_next[C::HALF && DP == 64 ? STEPS_K : 1][2];
   float* s_query = reinterpret_cast<float*>(smem + C::RING);
   auto head_of = [&](int block, int h) { return block * C::HEADS + h; };   // within the group
-  auto load_query = [&](uint32_t (&to)[C::HALF ? STEPS_K : 1][2], int64_t sequence, int kv_head, int block) {
+  auto load_query = [&](uint32_t (&to)[C::HALF ? STEPS_K : 1][2], int sequence, int kv_head, int block) {
     // 16-bit storage: columns 2t.. and 2t + 8.. of head g, per 16
     const int h = head_of(block, member * 8 + g);
     const bool there = h < p.group;
@@ -396,7 +413,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
     }
   };
-  if constexpr (C::HALF && DP < 256)
+  if constexpr (C::HALF && DP == 64)
     if (now.left > 0) load_query(query_next, now.sequence, now.kv_head, now.block);
 
   // -- the pass over the tokens -------------------------------------------------------------------
@@ -432,7 +449,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       for (int i = 0; i < A; ++i)
 #pragma unroll
         for (int j = 0; j < B; ++j) acc[i][j] = 0.f;
-      if constexpr (C::HALF && DP == 256) {
+      if constexpr (C::HALF && DP > 64) {
         load_query(query, now.sequence, now.kv_head, now.block);   // registers for one item's query only
       } else if constexpr (C::HALF) {
 #pragma unroll
@@ -464,6 +481,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};   // two chains of products
 #pragma unroll
           for (int ks = 0; ks < STEPS_K; ++ks) {
+            if (ks == STEPS_K * 3 / 4 && p.dim <= DP * 3 / 4) break;   // the last quarter is zeros
             uint32_t a[4];
             pa_ldmatrix(a, (k_place ^ (ks % 4 * 32)) + ks / 4 * 128 + set * 16 * ROW);
             pa_mma(ks % 2 ? s2 : s, a, query[ks][0], query[ks][1], T());
@@ -570,6 +588,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           const uint32_t v_place = stage + CHUNK * ROW + (lane % 8 + lane / 16 * 8) * ROW + ((lane / 8 % 2) ^ (lane % 8)) * 16;
 #pragma unroll
           for (int mt = 0; mt < DP / 16; ++mt) {
+            if (mt == DP / 16 * 3 / 4 && p.dim <= DP * 3 / 4) break;
             float y[4];
 #pragma unroll
             for (int set = 0; set < SETS; ++set) {
@@ -683,7 +702,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           now.tile = start;
           ahead = now;
           look_up();
-          if constexpr (DP < 256) load_query(query_next, now.sequence, now.kv_head, now.block);
+          if constexpr (DP == 64) load_query(query_next, now.sequence, now.kv_head, now.block);
           exactly = fresh = true;
           slot = 0;
           filling = STAGES - 1;
@@ -734,56 +753,55 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           write(h, d, make_float4(y.x * share, y.y * share, y.z * share, y.w * share));
         } else {
           __stcg(reinterpret_cast<float4*>(part + slot_head * DP + d), y);
-          if (d == 0) {
-            __stcg(part + C::HEADS * DP + slot_head, high);
-            __stcg(part + C::HEADS * DP + C::HEADS + slot_head, weight_sum);
-          }
+          if (d == 0) __stcg(reinterpret_cast<float2*>(part + C::HEADS * DP + 2 * slot_head), make_float2(high, weight_sum));
         }
       }
       if (!whole) {
-        const int64_t item = end - now.left - now.tile;   // the item's first unit
-        const int64_t first = pa_share_owner(units, workers, item), last = pa_share_owner(units, workers, item + now.tiles - 1);
+        const int64_t item = s_plan[2] - now.left - now.tile;   // the item's first unit
+        const int64_t first = pa_share_owner(s_plan[0], s_plan[1], item), last = pa_share_owner(s_plan[0], s_plan[1], item + now.tiles - 1);
         __syncthreads();
         if (tid == 0) s_last = pa_arrive(p.counters + first) == (int)(last - first);
         __syncthreads();
         if (s_last) {
           if (tid == 0) p.counters[first] = 0;
-          // the parts, added in the order of the blocks: the first block's second part, every other's first
-          const int count = (int)(last - first) + 1;
+          // The parts, added in the order of the blocks: the first block's second part, then every other's first, which lie at
+          // one distance; PA_JOIN of them requested at once.
+          const int count = (int)(last - first);
           const float* parts = p.parts + (first * 2 + 1) * C::PART;
-          auto part_of = [&](int n) { return parts + (n == 0 ? 0 : (int64_t)(2 * n - 1) * C::PART); };
 #pragma unroll 1
           for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
             const int slot_head = i / (DP / 4), d = i % (DP / 4) * 4, h = head_of(now.block, slot_head);
             if (h >= p.group || d >= p.dim) continue;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            float high = NONE, sum_p = 0.f;
+            const float* number = parts + slot_head * DP + d;
+            const float* state = parts + C::HEADS * DP + 2 * slot_head;   // maximum and sum
+            float4 y = __ldcg(reinterpret_cast<const float4*>(number));
+            const float2 started = __ldcg(reinterpret_cast<const float2*>(state));
+            float high = started.x, sum_p = started.y;
+            number += C::PART, state += C::PART;
 #pragma unroll 1
-            for (int n = 0; n < count; n += PA_JOIN) {   // PA_JOIN parts requested at once; past the last one nothing
+            for (int n = 0; n < count; n += PA_JOIN, number += 2 * PA_JOIN * C::PART, state += 2 * PA_JOIN * C::PART) {
               float4 x[PA_JOIN];
-              float part_high[PA_JOIN], part_sum[PA_JOIN], up = high;
+              float2 part[PA_JOIN];
+              float up = high;
 #pragma unroll
               for (int j = 0; j < PA_JOIN; ++j) {
-                part_high[j] = NONE;
-                part_sum[j] = 0.f;
+                part[j] = make_float2(NONE, 0.f);
                 x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (n + j < count) {
-                  const float* from = part_of(n + j);
-                  part_high[j] = __ldcg(from + C::HEADS * DP + slot_head);
-                  part_sum[j] = __ldcg(from + C::HEADS * DP + C::HEADS + slot_head);
-                  x[j] = __ldcg(reinterpret_cast<const float4*>(from + slot_head * DP + d));
+                  part[j] = __ldcg(reinterpret_cast<const float2*>(state + 2 * j * C::PART));
+                  x[j] = __ldcg(reinterpret_cast<const float4*>(number + 2 * j * C::PART));
                 }
               }
 #pragma unroll
-              for (int j = 0; j < PA_JOIN; ++j) up = fmaxf(up, part_high[j]);
+              for (int j = 0; j < PA_JOIN; ++j) up = fmaxf(up, part[j].x);
               const float around = up == NONE ? 0.f : up, before_weight = ex2_approx_ftz(high - around);
               high = up;
               y.x *= before_weight, y.y *= before_weight, y.z *= before_weight, y.w *= before_weight, sum_p *= before_weight;
 #pragma unroll
               for (int j = 0; j < PA_JOIN; ++j) {
-                const float weight = ex2_approx_ftz(part_high[j] - around);
+                const float weight = ex2_approx_ftz(part[j].x - around);
                 y.x = fmaf(weight, x[j].x, y.x), y.y = fmaf(weight, x[j].y, y.y), y.z = fmaf(weight, x[j].z, y.z), y.w = fmaf(weight, x[j].w, y.w);
-                sum_p = fmaf(weight, part_sum[j], sum_p);
+                sum_p = fmaf(weight, part[j].y, sum_p);
               }
             }
             const float share = 1.f / sum_p;
@@ -801,10 +819,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
 
 
 static size_t pa_workspace_bytes() {
-  // two parts per block of the largest forms: 32 heads of 128 and two blocks per SM, 32 heads of 256 and one
-  const size_t blocks = (size_t)sm_count();
-  const size_t small = 2 * blocks * 2 * PaConfig<float, 128, 4, 8>::PART, large = blocks * 2 * PaConfig<float, 256, 4, 8>::PART;
-  return PA_COUNTER_BYTES + (small > large ? small : large) * sizeof(float);
+  // two parts per block of the form with the most: 32 heads of 128, three blocks per SM
+  using Most = PaConfig<__half, 128, 4, 8>;
+  static_assert(Most::BLOCKS_PER_SM * Most::PART >= PaConfig<__half, 256, 4, 8>::PART && Most::BLOCKS_PER_SM >= PaConfig<float, 128, 4, 8>::BLOCKS_PER_SM, "largest");
+  return PA_COUNTER_BYTES + (size_t)sm_count() * Most::BLOCKS_PER_SM * 2 * Most::PART * sizeof(float);
 }
 
 template <typename T, int DP, int HB, int NH>
@@ -819,7 +837,7 @@ static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
   }
   p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
   p.heads = p.kv_heads * p.blocks;
-  p.whole_sets = p.page_size % C::SUB == 0 && p.window == 0 && p.row_bytes == C::ROW;
+  p.whole_sets = p.page_size % C::SUB == 0 && p.window == 0;
   int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
   const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;
