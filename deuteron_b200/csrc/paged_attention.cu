@@ -7,23 +7,36 @@
 //
 //   Shares. A unit is one tile of tokens (CHUNK per team of warps) of one item (sequence, kv head, block of query heads), and
 //   PA_ITEM_UNITS more stand at an item's end for what finishing it costs; the units of the whole batch, tile fastest, then
-//   head, then sequence, are cut into equal contiguous ranges, one per block of a grid that fills the card once. So the split over a sequence's length follows from the lengths on the device: no host
-//   copy of them, one launch, any raggedness, and a captured launch follows lengths that change.
-//   Pipeline. Each team keeps a ring of stages in shared memory filled by 16-byte asynchronous copies, several stages ahead
+//   head, then sequence, are cut into equal contiguous ranges, one per block of a grid that fills the card once. So the split
+//   over a sequence's length follows from the lengths on the device: no host copy of them, one launch, any raggedness, and a
+//   captured launch follows lengths that change.
+//   Pipeline. Each team keeps a ring of stages in shared memory filled by 16-byte asynchronous copies, ahead of the products
 //   and across the ends of sequences; a token's row is looked up through the page table one stage before its copies are
-//   issued. Nothing but the stage's own warps waits for a stage.
+//   issued. Nothing but the stage's own warps waits for a stage. Where a set of tokens lies in one page its rows follow one
+//   another and the copies' addresses differ by constants. Three blocks of four warps per SM with two stages each read faster
+//   than two with three stages (245 against 254 us below): what is short is not bytes in flight but warps whose chains of
+//   dependent instructions overlap.
 //   Products, 16-bit storage. mma.sync m16n8k16 with the tokens as the 16 rows and the query heads as the 8 columns:
 //   scores = K Q^T, numerators = V^T P^T, so that a group of up to 8 heads wastes nothing and the probabilities turn from
-//   result to operand layout with one movmatrix per 8 x 8. (tcgen05 would need 64 or 128 rows of heads or a round trip of P
-//   through shared memory; at 2 g products per element the tensor pipe idles either way.) P is split into two f16 or three
-//   bf16 terms, which keeps the products with V exact to about 2^-23, and a chunk's product starts from zero and is added
-//   to the FP32 numerator apart: the tensor core's own accumulator truncates.
+//   result to operand layout with one movmatrix per 8 x 8. At the copy rate 8 heads need 80 TFLOP/s of products; tcgen05
+//   would need 64 or 128 rows of heads, or P through shared memory. P is split into two f16 or three bf16 terms, which keeps
+//   the products with V exact to about 2^-23, and a chunk's product starts from zero and is added to the FP32 numerator
+//   apart: the tensor core's own accumulator truncates.
 //   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
 //   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
-//   heads are split into blocks that read the keys again.
+//   heads are split into blocks that read the keys again. From 16 heads on the products, not the bytes, set the time.
 //   Join. A block that holds a whole item writes it. Otherwise it leaves (m, sum, numerators) in the workspace and counts
 //   itself in; the last to arrive adds the parts in the order of the blocks, so the result does not depend on who was last.
 //   It leaves the counter at zero for the next launch.
+//
+// No form may use local memory: a build in which registers spilled read wrong addresses at head sizes above 128.
+//
+// Measured (kernel in a graph of 30 calls on three sets of inputs in turn, fraction of the 6540 GB/s of a copy):
+//   96 users, 17..8192 tokens, 32 heads on 8, 128, f16, 1.62 GB: 244 us (1.01); 16 users, 1..4096, 137 MB: 30 us (0.69, of
+//   which 3 us are the launch and the clearing of the counters); one user of 131071, bf16, 537 MB: 91 us (0.90; 55 blocks
+//   share each head, joining them costs 4 us, the slowest SM is 8 % behind the mean); 9 users, FP32, 16 heads of 64, 124 MB:
+//   29 us (0.65); 37 tokens of one user: 6 us. Head 64, 32 on 8: 0.88; head 80: 0.82; head 256: 0.82; groups of 16: 0.67, of
+//   32: 0.51; 256 users of 128..256 tokens: 0.70.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -58,9 +71,10 @@ struct PagedAttentionParams {
   int* status;
 };
 
-// Units for the end of an item: the teams' parts are added, the result written, the next query taken.
+// Units for the end of an item: the teams' parts are added, the result written, the next query taken (0, 1, 2, 3 and 5 units on
+// the 16 users: 35.3, 32.5, 32.1, 31.5 and 31.5 us; on 64 long ones 3 is still free).
 constexpr int PA_ITEM_UNITS = 3;
-constexpr int PA_JOIN = 8;
+constexpr int PA_JOIN = 8;                 // parts requested at once where they are joined
 
 // First unit of block c of `workers`, and the block that holds a unit: units * c / workers <= unit.
 __host__ __device__ __forceinline__ int64_t pa_share_begin(int64_t units, int64_t workers, int64_t c) { return units * c / workers; }
@@ -931,8 +945,10 @@ int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   const int64_t capacity = pages_per_sequence * page_size, most = (1LL << 31) - (1 << 16);
   PagedAttentionParams p = {};
   p.q = q;
-  p.k_pages = pages ? k_pages : q;   // an empty pool is never read, but copies of no bytes name an address
-  p.v_pages = pages ? v_pages : q;
+  // an empty pool is never read, but copies of no bytes name an aligned address
+  const void* nothing = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(q) & ~(uintptr_t)15);
+  p.k_pages = pages ? k_pages : nothing;
+  p.v_pages = pages ? v_pages : nothing;
   p.out = out;
   p.tables = tables;
   p.lengths = lengths;

@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t page_offset(const RotaryParams& p, int64_t to
 
 constexpr int R_MAX_DIM = 1024;
 constexpr int R_THREADS = 256;
-constexpr int R_FILL = 8192;   // threads per SM wanted of a launch
+constexpr int R_FILL = 8192;   // threads per SM wanted of a launch: 54 us at 16384 x 40 x 128, 59 with 4096, 62 with 16384
 
 // V elements in one access.
 template <int BYTES> struct Access;
@@ -91,8 +91,9 @@ template <> struct Access<2> { using type = uint16_t; };
 // issued before the angles are formed and before a key or value's page is looked up.
 //
 // Bound by memory. V is the widest that divides the head, its strides and addresses and, in the half layout, the number of
-// pairs: 16 bytes in practice, one element for an odd number of pairs. Measured (one element against a form that staged heads
-// in shared memory by 16-byte vectors): see the launch below.
+// pairs: 16 bytes in practice. 16384 tokens x 40 heads x 128 bf16 (336 MB): 54 us, 0.95 of the copy rate; 4095 x 20 x 96 FP32
+// interleaved (63 MB): 12 us, 0.80; append of 16000 tokens, 32 + 8 + 8 heads (393 MB): 61.5 us, 0.98; one token: 2 us. (A
+// form with the angles in shared memory and a unit per thread and head took 61, 15.7 and 112 us: its index arithmetic.)
 template <typename T, bool TWO, int V>
 __global__ void __launch_bounds__(R_THREADS) rotary_kernel(const RotaryParams p, const int interleaved, const int units, const int tokens_per_block,
                                                            const int heads_per_thread, const int q_slices, const int k_slices) {
@@ -193,6 +194,8 @@ static int rotary_launch_v(const RotaryParams& p, int interleaved, cudaStream_t 
 // halves of its elements' pairs from shared memory, where every thread of the head puts its vector: two vectors, out of
 // which OFF = pairs % V elements are shifted (a constant, so the shift costs no instruction or one per word). Between two
 // barriers all loads of R_SHARED heads precede their stores, and a head's threads are in one block, so out may be x itself.
+// 16384 x 40 x 128 bf16 with 37 pairs: 92 us against 161 with one element per access; with 38 pairs 92 against 111 with two;
+// with 36 pairs 89 against 96 with four. What it pays over whole vectors is twice the angles, one per element.
 constexpr int R_SHARED = 4, R_FILL_SHARED = 4096;
 
 template <typename T, int OFF>
