@@ -173,14 +173,16 @@ __device__ __forceinline__ int pa_arrive(int* counter) {
   return before;
 }
 
-// What is seen of a sequence: its row of the tables, its first token that is seen and how many.
+// What is seen of a sequence: its row of the tables and tokens first + skip .. first + seen. A window's tiles start at a
+// multiple of SUB tokens, so that sets of tokens lie in one page where they can; the skip tokens before it are not seen.
 struct PaSequence {
   int64_t table;
-  int first, seen;
+  int first, skip, seen;
 };
 
+template <int SUB>
 __device__ __forceinline__ PaSequence pa_sequence(const PagedAttentionParams& p, int64_t i) {
-  PaSequence s = {0, 0, 0};
+  PaSequence s = {0, 0, 0, 0};
   const int64_t row = p.rows ? (int64_t)p.rows[i] : i;
   if (row < 0) return s;
   if (row >= p.sequences) {
@@ -194,7 +196,9 @@ __device__ __forceinline__ PaSequence pa_sequence(const PagedAttentionParams& p,
   }
   if (length <= 0) return s;
   s.table = row * p.table_stride;
-  s.first = p.window > 0 && p.window < length ? length - (int)p.window : 0;
+  const int begin = p.window > 0 && p.window < length ? length - (int)p.window : 0;
+  s.skip = begin % SUB;
+  s.first = begin - s.skip;
   s.seen = length - s.first;
   return s;
 }
@@ -206,7 +210,7 @@ __device__ __forceinline__ int pa_tiles(int seen) { return seen <= 0 ? 0 : (seen
 __device__ __forceinline__ int64_t pa_item_units(int tiles) { return tiles > 0 ? (int64_t)tiles + PA_ITEM_UNITS : 0; }
 
 // A place in the order of the units, always a tile.
-template <int UNIT>
+template <int UNIT, int SUB>
 struct PaCursor {
   int sequence;
   int left;                      // units of the share from here on
@@ -215,7 +219,7 @@ struct PaCursor {
   PaSequence s;
 
   __device__ __forceinline__ void enter(const PagedAttentionParams& p) {
-    s = pa_sequence(p, sequence);
+    s = pa_sequence<SUB>(p, sequence);
     tiles = pa_tiles<UNIT>(s.seen);
   }
   __device__ __forceinline__ void next_item(const PagedAttentionParams& p) {   // from the first unit behind this item's tiles
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   // -- the share of this block: thread i adds up a contiguous part of the sequences ---------------
   const int64_t per = (p.count + THREADS - 1) / THREADS, mine = tid * per, mine_end = mine + per < p.count ? mine + per : p.count;
   int64_t sum = 0;
-  for (int64_t i = mine; i < mine_end; ++i) sum += pa_item_units(pa_tiles<UNIT>(pa_sequence(p, i).seen));
+  for (int64_t i = mine; i < mine_end; ++i) sum += pa_item_units(pa_tiles<UNIT>(pa_sequence<C::SUB>(p, i).seen));
   int64_t before = sum;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   }
   before -= sum;
   for (int64_t i = blockIdx.x; i < p.count; i += gridDim.x) {   // rows that see nothing
-    if (pa_sequence(p, i).seen > 0) continue;
+    if (pa_sequence<C::SUB>(p, i).seen > 0) continue;
     for (int j = tid; j < p.q_heads * p.dim; j += THREADS) {
       const int64_t to = i * p.out_token_stride + j / p.dim * p.out_head_stride + j % p.dim;
       if (p.out_f32)
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   if (begin >= before * p.heads && begin < (before + sum) * p.heads) {
     int64_t at = before * p.heads;
     for (int64_t i = mine; i < mine_end; ++i) {
-      const int64_t here = pa_item_units(pa_tiles<UNIT>(pa_sequence(p, i).seen)) * p.heads;
+      const int64_t here = pa_item_units(pa_tiles<UNIT>(pa_sequence<C::SUB>(p, i).seen)) * p.heads;
       if (begin < at + here) {
         s_start[0] = i;
         s_start[1] = begin - at;
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   }
   if (tid == 0) s_plan[0] = units, s_plan[1] = workers, s_plan[2] = end;
   __syncthreads();
-  PaCursor<UNIT> now, ahead;
+  PaCursor<UNIT, C::SUB> now, ahead;
   now.left = (int)(end - begin);
   now.sequence = (int)s_start[0];
   now.enter(p);
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   auto look_up = [&]() {
     const int token = (ahead.tile * TEAMS + team) * CHUNK + member * ROWS + lane % ROWS;
     offset = -1;
-    if (token < ahead.s.seen) {
+    if (token < ahead.s.seen && token >= ahead.s.skip) {
       const int position = ahead.s.first + token;
       const int index = (int)(((uint64_t)(uint32_t)position * p.divide_mul) >> p.divide_shift);
       const int page = p.tables[ahead.s.table + index];
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       } else if constexpr (C::HALF) {
 #pragma unroll
         for (int ks = 0; ks < STEPS_K; ++ks) query[ks][0] = query_next[ks][0], query[ks][1] = query_next[ks][1];
-        PaCursor<UNIT> next = now;   // the next item's, a whole item ahead
+        PaCursor<UNIT, C::SUB> next = now;   // the next item's, a whole item ahead
         next.left -= now.tiles - now.tile;
         next.next_item(p);
         if (next.left > 0) load_query(query_next, next.sequence, next.kv_head, next.block);
@@ -539,10 +543,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
 #pragma unroll
       for (int n = 0; n < EIGHTS; ++n) x[n][0] *= p.scale_log2e, x[n][1] *= p.scale_log2e;
-      if (base + CHUNK > seen) {
+      if (base + CHUNK > seen || base < now.s.skip) {
 #pragma unroll
         for (int n = 0; n < EIGHTS; ++n)
-          if (base + g + 8 * n >= seen) x[n][0] = x[n][1] = NONE;
+          if (base + g + 8 * n >= seen || base + g + 8 * n < now.s.skip) x[n][0] = x[n][1] = NONE;
       }
       // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
       // neither f16 terms nor FP32 sums mind, and nothing is exchanged or rescaled.
@@ -851,7 +855,7 @@ static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
   }
   p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
   p.heads = p.kv_heads * p.blocks;
-  p.whole_sets = p.page_size % C::SUB == 0 && p.window == 0;
+  p.whole_sets = p.page_size % C::SUB == 0;
   int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
   const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;

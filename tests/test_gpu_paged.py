@@ -216,6 +216,20 @@ def test_attention_of_the_last_tokens(cuda, window, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('size', [8, 16, 24, 64])
+def test_what_lies_before_the_window_does_not_matter(cuda, size, dtype):
+    lengths, window = [300, 41, 77, 16, 100], 40
+    k_pages, v_pages, tables, lens = M.a_cache(lengths, 2, 64, dtype, size, 'cuda')
+    q = normal((5, 8, 64), dtype, 2)
+    exact, bound = M.attend(q, k_pages, v_pages, tables, lens, 0.125, window=window)
+    for row, length in enumerate(lengths):
+        for position in range(max(0, length - window)):
+            page = int(tables[row, position // size])
+            k_pages[page, :, position % size], v_pages[page, :, position % size] = float('nan'), float('-inf')
+    within(ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.125, window=window), exact, bound)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('heads', [(8, 8), (8, 2), (12, 1), (32, 1)])
 def test_long_ragged_batches_are_joined(cuda, heads, dtype):
     attend_both([5000, 1, 0, 777, 12_345, 64], *heads, 64, dtype, 16)
