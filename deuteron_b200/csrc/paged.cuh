@@ -14,10 +14,10 @@ constexpr int PAGED_STATUS_ATTENTION = 0x6100;
 constexpr int PAGED_STATUS_APPEND = 0x6200;
 constexpr int PAGED_STATUS_COPY = 0x6300;
 
-static inline bool paged_storage_known(int storage) {
+static inline bool paged_storage_known(int64_t storage) {
   return storage == DTN_STORAGE_F32 || storage == DTN_STORAGE_F16 || storage == DTN_STORAGE_BF16;
 }
-static inline int paged_storage_bytes(int storage) { return storage == DTN_STORAGE_F32 ? 4 : 2; }
+static inline int paged_storage_bytes(int64_t storage) { return storage == DTN_STORAGE_F32 ? 4 : 2; }
 
 #ifdef __CUDACC__
 

@@ -919,85 +919,82 @@ int dtn_paged_attention_plan(const int64_t* tiles, int64_t count, int64_t heads,
   return DTN_OK;
 }
 
-int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
-                        void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
-                        int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
-                        int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
-                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+int dtn_paged_attention(const dtn_paged_attention_args* args, void* stream) {
   using namespace dtn;
-  DTN_REQUIRE(count >= 0 && q_heads >= 0 && kv_heads >= 0 && dim >= 0 && pages >= 0 && sequences >= 0 && pages_per_sequence >= 0 && window >= 0,
+  DTN_REQUIRE(args != nullptr, DTN_ERR_INVALID, "paged attention: no arguments");
+  const dtn_paged_attention_args& a = *args;
+  DTN_REQUIRE(a.count >= 0 && a.q_heads >= 0 && a.kv_heads >= 0 && a.dim >= 0 && a.pages >= 0 && a.sequences >= 0 && a.pages_per_sequence >= 0 && a.window >= 0,
               DTN_ERR_INVALID, "paged attention: negative extent");
-  DTN_REQUIRE(page_size >= 1 && page_size < (1LL << 31), DTN_ERR_INVALID, "paged attention: page size %lld", (long long)page_size);
-  DTN_REQUIRE(paged_storage_known(storage), DTN_ERR_INVALID, "paged attention: unknown storage %d", storage);
-  if (count == 0 || q_heads == 0 || dim == 0) return DTN_OK;
-  DTN_REQUIRE(kv_heads > 0 && q_heads % kv_heads == 0, DTN_ERR_INVALID, "paged attention: query heads must be a multiple of kv heads");
-  DTN_REQUIRE(dim <= 256, DTN_ERR_UNSUPPORTED, "paged attention: heads of at most 256 elements");
-  const int64_t element = paged_storage_bytes(storage);
-  DTN_REQUIRE(dim * element % 16 == 0 && page_stride * element % 16 == 0 && page_head_stride * element % 16 == 0 && aligned_to(k_pages, 16) &&
-                  aligned_to(v_pages, 16),
+  DTN_REQUIRE(a.page_size >= 1 && a.page_size < (1LL << 31), DTN_ERR_INVALID, "paged attention: page size %lld", (long long)a.page_size);
+  DTN_REQUIRE(paged_storage_known(a.storage), DTN_ERR_INVALID, "paged attention: unknown storage %lld", (long long)a.storage);
+  if (a.count == 0 || a.q_heads == 0 || a.dim == 0) return DTN_OK;
+  DTN_REQUIRE(a.kv_heads > 0 && a.q_heads % a.kv_heads == 0, DTN_ERR_INVALID, "paged attention: query heads must be a multiple of kv heads");
+  DTN_REQUIRE(a.dim <= 256, DTN_ERR_UNSUPPORTED, "paged attention: heads of at most 256 elements");
+  const int64_t element = paged_storage_bytes(a.storage);
+  DTN_REQUIRE(a.dim * element % 16 == 0 && a.page_stride * element % 16 == 0 && a.page_head_stride * element % 16 == 0 && aligned_to(a.k_pages, 16) &&
+                  aligned_to(a.v_pages, 16),
               DTN_ERR_INVALID, "paged attention: the heads of the pools must start on 16-byte boundaries and have a multiple of 16 bytes");
-  DTN_REQUIRE(q && out && (lengths || sequences == 0) && (rows || count <= sequences), DTN_ERR_INVALID, "paged attention: null pointer");
-  DTN_REQUIRE((k_pages && v_pages) || pages == 0, DTN_ERR_INVALID, "paged attention: null pool");
-  DTN_REQUIRE(sequences == 0 || tables || pages_per_sequence == 0, DTN_ERR_INVALID, "paged attention: null tables");
-  DTN_REQUIRE(pages < (1LL << 31) && count < (1LL << 31) && q_heads < (1LL << 20) && pages_per_sequence < (1LL << 31), DTN_ERR_UNSUPPORTED,
+  DTN_REQUIRE(a.q && a.out && (a.lengths || a.sequences == 0) && (a.rows || a.count <= a.sequences), DTN_ERR_INVALID, "paged attention: null pointer");
+  DTN_REQUIRE((a.k_pages && a.v_pages) || a.pages == 0, DTN_ERR_INVALID, "paged attention: null pool");
+  DTN_REQUIRE(a.sequences == 0 || a.tables || a.pages_per_sequence == 0, DTN_ERR_INVALID, "paged attention: null tables");
+  DTN_REQUIRE(a.pages < (1LL << 31) && a.count < (1LL << 31) && a.q_heads < (1LL << 20) && a.pages_per_sequence < (1LL << 31), DTN_ERR_UNSUPPORTED,
               "paged attention: too many rows or pages for one launch");
-  DTN_REQUIRE(workspace && workspace_bytes >= pa_workspace_bytes(), DTN_ERR_WORKSPACE, "paged attention: %zu bytes of workspace, %zu needed", workspace_bytes,
-              pa_workspace_bytes());
-  DTN_REQUIRE(aligned_to(workspace, 16), DTN_ERR_WORKSPACE, "paged attention: the workspace must be 16-byte aligned");
+  DTN_REQUIRE(a.workspace && a.workspace_bytes >= (int64_t)pa_workspace_bytes(), DTN_ERR_WORKSPACE,
+              "paged attention: %lld bytes of workspace, %zu needed", (long long)a.workspace_bytes, pa_workspace_bytes());
+  DTN_REQUIRE(aligned_to(a.workspace, 16), DTN_ERR_WORKSPACE, "paged attention: the workspace must be 16-byte aligned");
   cudaStream_t s = as_stream(stream);
-  const int64_t capacity = pages_per_sequence * page_size, most = (1LL << 31) - (1 << 16);
+  const int64_t capacity = a.pages_per_sequence * a.page_size, most = (1LL << 31) - (1 << 16);
   PagedAttentionParams p = {};
-  p.q = q;
+  p.q = a.q;
   // an empty pool is never read, but copies of no bytes name an aligned address
-  const void* nothing = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(q) & ~(uintptr_t)15);
-  p.k_pages = pages ? k_pages : nothing;
-  p.v_pages = pages ? v_pages : nothing;
-  p.out = out;
-  p.tables = tables;
-  p.lengths = lengths;
-  p.rows = rows;
-  p.count = count;
-  p.sequences = sequences;
-  p.pages = pages;
-  p.table_stride = table_stride;
+  const void* nothing = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(a.q) & ~(uintptr_t)15);
+  p.k_pages = a.pages ? a.k_pages : nothing;
+  p.v_pages = a.pages ? a.v_pages : nothing;
+  p.out = a.out;
+  p.tables = a.tables;
+  p.lengths = a.lengths;
+  p.rows = a.rows;
+  p.count = a.count;
+  p.sequences = a.sequences;
+  p.pages = a.pages;
+  p.table_stride = a.table_stride;
   p.capacity = (int)(capacity < most ? capacity : most);
-  p.q_token_stride = q_token_stride;
-  p.q_head_stride = q_head_stride;
-  p.out_token_stride = out_token_stride;
-  p.out_head_stride = out_head_stride;
-  p.page_stride = page_stride * element;
-  p.page_head_stride = page_head_stride * element;
-  p.kv_heads = (int)kv_heads;
-  p.q_heads = (int)q_heads;
-  p.group = (int)(q_heads / kv_heads);
-  p.dim = (int)dim;
-  p.page_size = (int)page_size;
-  p.row_bytes = (int)(dim * element);
-  p.window = window;
-  p.scale_log2e = scale * 1.4426950408889634f;
-  p.out_f32 = out_f32;
-  p.q_pairs = element == 2 && aligned_to(q, 4) && q_token_stride % 2 == 0 && q_head_stride % 2 == 0;
-  const int64_t out_element = out_f32 ? 4 : element;
-  p.out_quads = aligned_to(out, 4 * out_element) && out_token_stride % 4 == 0 && out_head_stride % 4 == 0;
+  p.q_token_stride = a.q_token_stride;
+  p.q_head_stride = a.q_head_stride;
+  p.out_token_stride = a.out_token_stride;
+  p.out_head_stride = a.out_head_stride;
+  p.page_stride = a.page_stride * element;
+  p.page_head_stride = a.page_head_stride * element;
+  p.kv_heads = (int)a.kv_heads;
+  p.q_heads = (int)a.q_heads;
+  p.group = (int)(a.q_heads / a.kv_heads);
+  p.dim = (int)a.dim;
+  p.page_size = (int)a.page_size;
+  p.row_bytes = (int)(a.dim * element);
+  p.window = a.window;
+  p.scale_log2e = (float)(a.scale * 1.4426950408889634);
+  p.out_f32 = a.out_f32 != 0;
+  p.q_pairs = element == 2 && aligned_to(a.q, 4) && a.q_token_stride % 2 == 0 && a.q_head_stride % 2 == 0;
+  const int64_t out_element = a.out_f32 ? 4 : element;
+  p.out_quads = aligned_to(a.out, 4 * out_element) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
   p.min_units = 1 + PA_ITEM_UNITS;
   // position / page_size for positions below 2^31: mul = floor(2^(31 + s) / d) + 1 with 2^s >= d exceeds 2^(31 + s) / d by at
   // most 1, so the product exceeds the quotient by less than 2^31 / 2^(31 + s) <= 1 / d: the floor is exact. mul <= 2^32 - 1
   // needs d > 1; for d = 1 the multiplier is 1 and the shift 0.
-  if (page_size == 1) {
+  if (a.page_size == 1) {
     p.divide_mul = 1;
     p.divide_shift = 0;
   } else {
     int bits = 1;
-    while ((1LL << bits) < page_size) ++bits;
+    while ((1LL << bits) < a.page_size) ++bits;
     p.divide_shift = 31 + bits;
-    p.divide_mul = (uint32_t)((1ULL << (31 + bits)) / (uint64_t)page_size + 1);
+    p.divide_mul = (uint32_t)((1ULL << (31 + bits)) / (uint64_t)a.page_size + 1);
   }
-  p.counters = static_cast<int*>(workspace);
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + PA_COUNTER_BYTES);
+  p.counters = static_cast<int*>(a.workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + PA_COUNTER_BYTES);
   p.status = device_status_word_unless_capturing(s);
-  if (storage == DTN_STORAGE_F32) return paged_attention_launch<float>(p, s);
-  if (storage == DTN_STORAGE_F16) return paged_attention_launch<__half>(p, s);
+  if (a.storage == DTN_STORAGE_F32) return paged_attention_launch<float>(p, s);
+  if (a.storage == DTN_STORAGE_F16) return paged_attention_launch<__half>(p, s);
   return paged_attention_launch<__nv_bfloat16>(p, s);
 }
 

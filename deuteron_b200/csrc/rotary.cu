@@ -343,80 +343,79 @@ static int rotary_launch(const RotaryParams& p, int interleaved, int storage, cu
 
 extern "C" {
 
-int dtn_rotary(const void* x, void* out, const void* positions, int positions_64, const double* frequencies, int64_t tokens, int64_t heads,
-               int64_t dim, int64_t pairs, int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride, int64_t out_head_stride,
-               int interleaved, int transpose, float amplitude, int storage, void* stream) {
+int dtn_rotary(const dtn_rotary_args* args, void* stream) {
   using namespace dtn;
-  DTN_REQUIRE(tokens >= 0 && heads >= 0 && dim >= 0 && pairs >= 0, DTN_ERR_INVALID, "rotary: negative extent");
-  DTN_REQUIRE(paged_storage_known(storage), DTN_ERR_INVALID, "rotary: unknown storage %d", storage);
-  DTN_REQUIRE(2 * pairs <= dim, DTN_ERR_INVALID, "rotary: %lld pairs do not fit a head of %lld", (long long)pairs, (long long)dim);
-  DTN_REQUIRE(dim <= R_MAX_DIM && heads < (1 << 20) && tokens < (1LL << 31), DTN_ERR_UNSUPPORTED,
+  DTN_REQUIRE(args != nullptr, DTN_ERR_INVALID, "rotary: no arguments");
+  const dtn_rotary_args& a = *args;
+  DTN_REQUIRE(a.tokens >= 0 && a.heads >= 0 && a.dim >= 0 && a.pairs >= 0, DTN_ERR_INVALID, "rotary: negative extent");
+  DTN_REQUIRE(paged_storage_known(a.storage), DTN_ERR_INVALID, "rotary: unknown storage %lld", (long long)a.storage);
+  DTN_REQUIRE(a.dim <= R_MAX_DIM && a.heads < (1 << 20) && a.tokens < (1LL << 31), DTN_ERR_UNSUPPORTED,
               "rotary: heads of at most %d elements, fewer than 2^31 tokens", R_MAX_DIM);
-  if (tokens == 0 || heads == 0 || dim == 0) return DTN_OK;
-  DTN_REQUIRE(x && out && positions && (frequencies || pairs == 0), DTN_ERR_INVALID, "rotary: null pointer");
+  DTN_REQUIRE(a.pairs <= a.dim / 2, DTN_ERR_INVALID, "rotary: %lld pairs do not fit a head of %lld", (long long)a.pairs, (long long)a.dim);
+  if (a.tokens == 0 || a.heads == 0 || a.dim == 0) return DTN_OK;
+  DTN_REQUIRE(a.x && a.out && a.positions && (a.frequencies || a.pairs == 0), DTN_ERR_INVALID, "rotary: null pointer");
   RotaryParams p = {};
-  p.q = {x, x_token_stride, x_head_stride, (int)heads};
-  p.q_out = out;
-  p.q_out_token_stride = out_token_stride;
-  p.q_out_head_stride = out_head_stride;
-  p.positions = positions;
-  p.positions_64 = positions_64;
-  p.frequencies = frequencies;
-  p.pairs = (int)pairs;
-  p.dim = (int)dim;
-  p.amplitude = amplitude;
-  p.sign = transpose ? -1.f : 1.f;
-  p.tokens = tokens;
-  return rotary_launch(p, interleaved, storage, as_stream(stream));
+  p.q = {a.x, a.x_token_stride, a.x_head_stride, (int)a.heads};
+  p.q_out = a.out;
+  p.q_out_token_stride = a.out_token_stride;
+  p.q_out_head_stride = a.out_head_stride;
+  p.positions = a.positions;
+  p.positions_64 = a.positions_64 != 0;
+  p.frequencies = a.frequencies;
+  p.pairs = (int)a.pairs;
+  p.dim = (int)a.dim;
+  p.amplitude = (float)a.amplitude;
+  p.sign = a.transpose ? -1.f : 1.f;
+  p.tokens = a.tokens;
+  return rotary_launch(p, a.interleaved != 0, (int)a.storage, as_stream(stream));
 }
 
-int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int* tables, const int* rows, const void* positions,
-                     int positions_64, int64_t tokens, int64_t kv_heads, int64_t dim, int64_t k_token_stride, int64_t k_head_stride,
-                     int64_t v_token_stride, int64_t v_head_stride, int64_t pages, int64_t page_size, int64_t page_stride,
-                     int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence, int64_t table_stride, const double* frequencies,
-                     int64_t pairs, int interleaved, float amplitude, const void* q, void* q_out, int64_t q_heads, int64_t q_token_stride,
-                     int64_t q_head_stride, int64_t q_out_token_stride, int64_t q_out_head_stride, int storage, void* stream) {
+int dtn_paged_append(const dtn_paged_append_args* args, void* stream) {
   using namespace dtn;
-  DTN_REQUIRE(tokens >= 0 && kv_heads >= 0 && dim >= 0 && pairs >= 0 && q_heads >= 0 && pages >= 0 && sequences >= 0 && pages_per_sequence >= 0,
+  DTN_REQUIRE(args != nullptr, DTN_ERR_INVALID, "paged append: no arguments");
+  const dtn_paged_append_args& a = *args;
+  DTN_REQUIRE(a.tokens >= 0 && a.kv_heads >= 0 && a.dim >= 0 && a.pairs >= 0 && a.q_heads >= 0 && a.pages >= 0 && a.sequences >= 0 &&
+                  a.pages_per_sequence >= 0,
               DTN_ERR_INVALID, "paged append: negative extent");
-  DTN_REQUIRE(page_size >= 1 && page_size < (1LL << 31), DTN_ERR_INVALID, "paged append: page size %lld", (long long)page_size);
-  DTN_REQUIRE(paged_storage_known(storage), DTN_ERR_INVALID, "paged append: unknown storage %d", storage);
-  DTN_REQUIRE(2 * pairs <= dim, DTN_ERR_INVALID, "paged append: %lld pairs do not fit a head of %lld", (long long)pairs, (long long)dim);
-  DTN_REQUIRE(dim <= R_MAX_DIM && kv_heads < (1 << 20) && q_heads < (1 << 20) && tokens < (1LL << 31) && pages < (1LL << 31), DTN_ERR_UNSUPPORTED,
-              "paged append: heads of at most %d elements, fewer than 2^31 tokens and pages", R_MAX_DIM);
-  if (tokens == 0 || dim == 0 || kv_heads + q_heads == 0) return DTN_OK;
-  DTN_REQUIRE(k && v && rows && positions && (frequencies || pairs == 0), DTN_ERR_INVALID, "paged append: null pointer");
-  DTN_REQUIRE((k_pages && v_pages) || pages == 0, DTN_ERR_INVALID, "paged append: null pool");
-  DTN_REQUIRE(tables || sequences == 0 || pages_per_sequence == 0, DTN_ERR_INVALID, "paged append: null tables");
-  DTN_REQUIRE(q_heads == 0 || (q && q_out), DTN_ERR_INVALID, "paged append: null queries");
+  DTN_REQUIRE(a.page_size >= 1 && a.page_size < (1LL << 31), DTN_ERR_INVALID, "paged append: page size %lld", (long long)a.page_size);
+  DTN_REQUIRE(paged_storage_known(a.storage), DTN_ERR_INVALID, "paged append: unknown storage %lld", (long long)a.storage);
+  DTN_REQUIRE(a.dim <= R_MAX_DIM && a.kv_heads < (1 << 20) && a.q_heads < (1 << 20) && a.tokens < (1LL << 31) && a.pages < (1LL << 31) &&
+                  a.pages_per_sequence < (1LL << 31),
+              DTN_ERR_UNSUPPORTED, "paged append: heads of at most %d elements, fewer than 2^31 tokens and pages", R_MAX_DIM);
+  DTN_REQUIRE(a.pairs <= a.dim / 2, DTN_ERR_INVALID, "paged append: %lld pairs do not fit a head of %lld", (long long)a.pairs, (long long)a.dim);
+  if (a.tokens == 0 || a.dim == 0 || a.kv_heads + a.q_heads == 0) return DTN_OK;
+  DTN_REQUIRE(a.k && a.v && a.rows && a.positions && (a.frequencies || a.pairs == 0), DTN_ERR_INVALID, "paged append: null pointer");
+  DTN_REQUIRE((a.k_pages && a.v_pages) || a.pages == 0, DTN_ERR_INVALID, "paged append: null pool");
+  DTN_REQUIRE(a.tables || a.sequences == 0 || a.pages_per_sequence == 0, DTN_ERR_INVALID, "paged append: null tables");
+  DTN_REQUIRE(a.q_heads == 0 || (a.q && a.q_out), DTN_ERR_INVALID, "paged append: null queries");
   RotaryParams p = {};
-  p.q = {q, q_token_stride, q_head_stride, (int)q_heads};
-  p.k = {k, k_token_stride, k_head_stride, (int)kv_heads};
-  p.v = {v, v_token_stride, v_head_stride, (int)kv_heads};
-  p.q_out = q_out;
-  p.q_out_token_stride = q_out_token_stride;
-  p.q_out_head_stride = q_out_head_stride;
-  p.k_pages = k_pages;
-  p.v_pages = v_pages;
-  p.page_stride = page_stride;
-  p.page_head_stride = page_head_stride;
-  p.tables = tables;
-  p.table_stride = table_stride;
-  p.rows = rows;
-  p.sequences = sequences;
-  p.pages = pages;
-  p.capacity = pages_per_sequence * page_size;
-  p.page_size = (int)page_size;
-  p.positions = positions;
-  p.positions_64 = positions_64;
-  p.frequencies = frequencies;
-  p.pairs = (int)pairs;
-  p.dim = (int)dim;
-  p.amplitude = amplitude;
+  p.q = {a.q, a.q_token_stride, a.q_head_stride, (int)a.q_heads};
+  p.k = {a.k, a.k_token_stride, a.k_head_stride, (int)a.kv_heads};
+  p.v = {a.v, a.v_token_stride, a.v_head_stride, (int)a.kv_heads};
+  p.q_out = a.q_out;
+  p.q_out_token_stride = a.q_out_token_stride;
+  p.q_out_head_stride = a.q_out_head_stride;
+  p.k_pages = a.k_pages;
+  p.v_pages = a.v_pages;
+  p.page_stride = a.page_stride;
+  p.page_head_stride = a.page_head_stride;
+  p.tables = a.tables;
+  p.table_stride = a.table_stride;
+  p.rows = a.rows;
+  p.sequences = a.sequences;
+  p.pages = a.pages;
+  p.capacity = a.pages_per_sequence * a.page_size;
+  p.page_size = (int)a.page_size;
+  p.positions = a.positions;
+  p.positions_64 = a.positions_64 != 0;
+  p.frequencies = a.frequencies;
+  p.pairs = (int)a.pairs;
+  p.dim = (int)a.dim;
+  p.amplitude = (float)a.amplitude;
   p.sign = 1.f;
-  p.tokens = tokens;
+  p.tokens = a.tokens;
   p.status = device_status_word_unless_capturing(as_stream(stream));
-  return rotary_launch(p, interleaved, storage, as_stream(stream));
+  return rotary_launch(p, a.interleaved != 0, (int)a.storage, as_stream(stream));
 }
 
 }  // extern "C"

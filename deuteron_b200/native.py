@@ -6,6 +6,7 @@ module's `lib()` raises. There is no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes as ct
+import struct
 import threading
 from pathlib import Path
 
@@ -35,6 +36,10 @@ class DeviceWaitError(RuntimeError):
 class PageError(IndexError):
     """A kernel met a page number, position, row or length that a paged cache's pool or tables do not cover."""
 
+
+# Argument structures of the operators of a decode step (dtn_rotary_args, dtn_paged_append_args, dtn_paged_attention_args): pointers
+# and 64-bit integers in the header's order, then a double. One packed object costs a third of as many ctypes arguments.
+ROTARY_ARGS, PAGED_APPEND_ARGS, PAGED_ATTENTION_ARGS = struct.Struct('16qd'), struct.Struct('33qd'), struct.Struct('27qd')
 
 _I64, _P, _F, _I = ct.c_int64, ct.c_void_p, ct.c_float, ct.c_int
 _SIGNATURES = {
@@ -66,11 +71,9 @@ _SIGNATURES = {
     'dtn_attention_f32': [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _F, _P],
     'dtn_gqa_fwd': [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _I, _I64, _I64, _P],
     'dtn_gqa_set_variant': [_I],
-    'dtn_rotary': [_P, _P, _P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _F, _I, _P],
-    'dtn_paged_append': [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-                         _I64, _P, _I64, _I, _F, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P],
-    'dtn_paged_attention': [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
-                            _I64, _I64, _F, _I64, _I, _I, _P, ct.c_size_t, _P],
+    'dtn_rotary': [ct.c_char_p, _P],
+    'dtn_paged_append': [ct.c_char_p, _P],
+    'dtn_paged_attention': [ct.c_char_p, _P],
     'dtn_paged_attention_workspace_bytes': [ct.POINTER(ct.c_size_t)],
     'dtn_paged_attention_plan': [ct.POINTER(ct.c_int64), _I64, _I64, _I64, _I64, ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64),
                                  ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64)],

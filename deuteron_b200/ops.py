@@ -492,9 +492,9 @@ def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> tor
     if out.data_ptr() == x.data_ptr() and (out_token_stride, out_head_stride) != (token_stride, head_stride):
         raise ValueError('out must be x itself or lie elsewhere')
     _on_current_device(x, positions, frequencies, out)
-    native.call('dtn_rotary', x.data_ptr(), out.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(),
-                tokens, heads, dim, pairs, token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose,
-                float(amplitude), _STORAGE_OF[x.dtype], _stream())
+    native.call('dtn_rotary', native.ROTARY_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), positions.dtype is torch.int64, tokens, heads, dim, pairs,
+        token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose, _STORAGE_OF[x.dtype], float(amplitude)), _stream())
     return out
 
 
@@ -562,11 +562,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             raise ValueError('q_out must be q itself or lie elsewhere')
         _on_current_device(q, q_out)
     _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, k if frequencies is None else frequencies)
-    native.call('dtn_paged_append', k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(),
-                positions.data_ptr(), positions.dtype == torch.int64, tokens, kv_heads, dim, k_token, k_head, v_token, v_head, pages, page_size,
-                page_stride, page_head_stride, sequences, width, table_stride, frequencies.data_ptr() if pairs else None, pairs,
-                _LAYOUTS[layout], float(amplitude), q.data_ptr() if q_heads else None, q_out.data_ptr() if q_heads else None, q_heads,
-                q_token, q_head, q_out_token, q_out_head, _STORAGE_OF[k.dtype], _stream())
+    native.call('dtn_paged_append', native.PAGED_APPEND_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(), positions.data_ptr(),
+        frequencies.data_ptr() if pairs else 0, q.data_ptr() if q_heads else 0, q_out.data_ptr() if q_heads else 0,
+        positions.dtype is torch.int64, tokens, kv_heads, dim, k_token, k_head, v_token, v_head, pages, page_size, page_stride,
+        page_head_stride, sequences, width, table_stride, pairs, _LAYOUTS[layout], q_heads, q_token, q_head, q_out_token, q_out_head,
+        _STORAGE_OF[k.dtype], float(amplitude)), _stream())
     return q_out
 
 
@@ -621,8 +622,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _index(rows, 'rows', count)
     elif count > sequences:
         raise ValueError(f'{count} queries but {sequences} sequences')
-    if type(window) is not int or window < 0:
+    if type(window) is not int or not 0 <= window < 1 << 63:
         raise ValueError(f'window must be a non-negative integer, got {window!r}')
+    scale = float(scale)
     if out is None:
         out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)
     _tensors(out)
@@ -630,9 +632,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError('out must have the shape of q and dtype float32 or that of q')
     out_token, out_head = _heads(out, 'out', written=True)
     _on_current_device(q, k_pages, v_pages, tables, lengths, lengths if rows is None else rows, out)
-    native.call('dtn_paged_attention', q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
-                None if rows is None else rows.data_ptr(), out.data_ptr(), count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head,
-                pages, page_size, page_stride, page_head_stride, sequences, width, table_stride, float(scale), window, _STORAGE_OF[q.dtype], out.dtype == torch.float32, *_paged_workspace(q, stream := _stream()), stream)
+    stream = _stream()
+    workspace, workspace_bytes = _paged_workspace(q, stream)
+    native.call('dtn_paged_attention', native.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(), 0 if rows is None else rows.data_ptr(),
+        out.data_ptr(), workspace, workspace_bytes, count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head, pages, page_size,
+        page_stride, page_head_stride, sequences, width, table_stride, window, _STORAGE_OF[q.dtype], out.dtype is torch.float32, scale), stream)
     return out
 
 

@@ -325,16 +325,27 @@ int dtn_gqa_fwd(const void* q, const void* k, const void* v, float* out, int64_t
  * No reference counterpart. */
 int dtn_gqa_set_variant(int variant);
 
-/* Rotary positions: out[t, h] = x[t, h] with pair i of its first 2 * pairs elements turned by the angle
+/* The operators of a decode step take their arguments in a structure of pointers (device), 64-bit integers and doubles that the
+ * call reads before it returns.
+ *
+ * Rotary positions: out[t, h] = x[t, h] with pair i of its first 2 * pairs elements turned by the angle
  * positions[t] * frequencies[i] and scaled by `amplitude`; the other elements are copied. Pair i is (i, i + pairs), or
  * (2 i, 2 i + 1) when `interleaved` is non-zero. A non-zero `transpose` turns the other way: the gradient of x from that of
  * out. x and out are [tokens, heads, dim] of `storage` with the given strides in elements and dense heads (out may be x
  * itself, with the same strides); positions are int32, or int64 when `positions_64` is non-zero; frequencies are FP64 radians
  * per position. The angle is formed and reduced in FP64, the rotation computed in FP32 and rounded once. dim <= 1024. Any
  * alignment of whole elements; 16-byte aligned heads are moved faster. No reference counterpart. */
-int dtn_rotary(const void* x, void* out, const void* positions, int positions_64, const double* frequencies, int64_t tokens, int64_t heads,
-               int64_t dim, int64_t pairs, int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride,
-               int64_t out_head_stride, int interleaved, int transpose, float amplitude, int storage, void* stream);
+typedef struct {
+  const void* x;
+  void* out;
+  const void* positions;
+  const double* frequencies;
+  int64_t positions_64, tokens, heads, dim, pairs;
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  int64_t interleaved, transpose, storage;
+  double amplitude;
+} dtn_rotary_args;
+int dtn_rotary(const dtn_rotary_args* args /* host */, void* stream);
 
 /* Appends tokens to a paged key-value cache, with the rotation of dtn_rotary on the way (pairs = 0: none).
  * Pools: k_pages and v_pages are [pages, kv_heads, page_size, dim] of `storage` with the same page_stride and
@@ -344,12 +355,24 @@ int dtn_rotary(const void* x, void* out, const void* positions, int positions_64
  * the same positions into q_out, which may be q itself. A row >= sequences, a position outside the tables or a page number
  * outside the pool stores nothing and is reported by dtn_device_status (not where the first call on a device is being captured:
  * the status word is allocated outside captures). Two tokens for one place: either may stay. */
-int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int* tables, const int* rows, const void* positions,
-                     int positions_64, int64_t tokens, int64_t kv_heads, int64_t dim, int64_t k_token_stride, int64_t k_head_stride,
-                     int64_t v_token_stride, int64_t v_head_stride, int64_t pages, int64_t page_size, int64_t page_stride,
-                     int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence, int64_t table_stride, const double* frequencies,
-                     int64_t pairs, int interleaved, float amplitude, const void* q, void* q_out, int64_t q_heads, int64_t q_token_stride,
-                     int64_t q_head_stride, int64_t q_out_token_stride, int64_t q_out_head_stride, int storage, void* stream);
+typedef struct {
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  const int *tables, *rows;
+  const void* positions;
+  const double* frequencies;
+  const void* q;
+  void* q_out;
+  int64_t positions_64, tokens, kv_heads, dim;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t pages, page_size, page_stride, page_head_stride;
+  int64_t sequences, pages_per_sequence, table_stride;
+  int64_t pairs, interleaved;
+  int64_t q_heads, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+  int64_t storage;
+  double amplitude;
+} dtn_paged_append_args;
+int dtn_paged_append(const dtn_paged_append_args* args /* host */, void* stream);
 
 /* Attention of one new token per sequence over a paged cache (pools and tables as above):
  * out[i, h] = sum over t of softmax_t(scale * q[i, h] . k[t]) v[t], t over the last `window` (0: all) of the first lengths[r]
@@ -361,12 +384,18 @@ int dtn_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
  * dtn_paged_attention_workspace_bytes bytes, 16-byte aligned, and is zeroed once before its first call; every call leaves its
  * first 4096 bytes (counters) zero again. Calls that can overlap on the GPU need a workspace each. Same result on every
  * run of the same call. */
-int dtn_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* tables, const int* lengths, const int* rows,
-                        void* out, int64_t count, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t q_token_stride,
-                        int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int64_t pages, int64_t page_size,
-                        int64_t page_stride, int64_t page_head_stride, int64_t sequences, int64_t pages_per_sequence,
-                        int64_t table_stride, float scale, int64_t window, int storage, int out_f32, void* workspace,
-                        size_t workspace_bytes, void* stream);
+typedef struct {
+  const void *q, *k_pages, *v_pages;
+  const int *tables, *lengths, *rows;
+  void *out, *workspace;
+  int64_t workspace_bytes, count, q_heads, kv_heads, dim;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t pages, page_size, page_stride, page_head_stride;
+  int64_t sequences, pages_per_sequence, table_stride;
+  int64_t window, storage, out_f32;
+  double scale;
+} dtn_paged_attention_args;
+int dtn_paged_attention(const dtn_paged_attention_args* args /* host */, void* stream);
 
 /* Bytes of workspace that serve any dtn_paged_attention call on the current device. */
 int dtn_paged_attention_workspace_bytes(size_t* bytes_out /* host */);

@@ -101,53 +101,69 @@ def test_copies_refuse():
             ops.copy_pages(*arguments)
 
 
-def test_the_c_entries_check_before_any_cuda_call():
+ONE = 1 << 20
+# pointers and integers in the order of the header's structures, then the double
+ROTARY = [ONE] * 4 + [0, 1, 1, 8, 4, 8, 8, 8, 8, 0, 0, 0, 1.0]
+APPEND = [ONE] * 10 + [0, 1, 1, 8, 8, 8, 8, 8, 4, 8, 64, 64, 1, 1, 1, 4, 0, 1, 8, 8, 8, 8, 0, 1.0]
+ATTENTION = [ONE] * 8 + [1 << 30, 1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 0, 0, 1, 1.0]
+
+
+def status_of(name, good, changes):
+    arguments = list(good)
+    for place, value in changes.items():
+        arguments[place] = value
     library = native.lib()
-    one = 1 << 20
-    rotary = [one, one, one, 0, one, 1, 1, 8, 4, 8, 8, 8, 8, 0, 0, 1.0, 0, None]
-    append = [one] * 7 + [0, 1, 1, 8, 8, 8, 8, 8, 4, 8, 64, 64, 1, 1, 1, one, 4, 0, 1.0, one, one, 1, 8, 8, 8, 8, 0, None]
-    attention = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 0, 1, one, 1 << 30, None]
-    copies = [one, 1, 64, 4, 64, 64, one, one, 1, None]
+    if name == 'dtn_copy_pages':
+        return library.dtn_copy_pages(*arguments)
+    packer = {'dtn_rotary': native.ROTARY_ARGS, 'dtn_paged_append': native.PAGED_APPEND_ARGS, 'dtn_paged_attention': native.PAGED_ATTENTION_ARGS}[name]
+    return getattr(library, name)(packer.pack(*arguments), None)
+
+
+def test_the_structures_are_those_of_the_header():
+    header = (native.LIBRARY_PATH.parent.parent / 'include' / 'deuteron_b200.h').read_text()
+    for name, packer in (('dtn_rotary_args', native.ROTARY_ARGS), ('dtn_paged_append_args', native.PAGED_APPEND_ARGS), ('dtn_paged_attention_args', native.PAGED_ATTENTION_ARGS)):
+        body = header[:header.index('} ' + name)].rsplit('typedef struct {', 1)[1]
+        declarations = [line.strip() for line in body.split(';') if line.strip()]
+        fields = sum(len(line.split(',')) for line in declarations)
+        assert packer.size == 8 * fields and declarations[-1].startswith('double') and len(declarations[-1].split(',')) == 1
+        assert all('*' in line or line.startswith('int64_t') for line in declarations[:-1])
+
+
+def test_the_c_entries_check_before_any_cuda_call():
+    copies = [ONE, 1, 64, 4, 64, 64, ONE, ONE, 1, None]
+    for name in ('dtn_rotary', 'dtn_paged_append', 'dtn_paged_attention'):
+        assert getattr(native.lib(), name)(None, None) == native.ERR_INVALID
     for name, good, bad in (
-            ('dtn_rotary', rotary, {0: None, 1: None, 2: None, 4: None, 5: -1, 6: -1, 7: -1, 8: 5, 16: 3}),
-            ('dtn_paged_append', append, {0: None, 1: None, 2: None, 3: None, 4: None, 5: None, 6: None, 8: -1, 9: -1, 10: -1, 15: -1, 16: 0, 19: -1, 20: -1, 22: None,
-                                          23: 5, 26: None, 27: None, 28: -1, 33: -1}),
-            ('dtn_paged_attention', attention, {0: None, 1: None, 2: None, 3: None, 4: None, 6: None, 7: -1, 8: 3, 9: 2 ** 40, 15: -1, 16: 0, 19: -1, 20: -1, 23: -1, 24: 5}),
+            ('dtn_rotary', ROTARY, {0: 0, 1: 0, 2: 0, 3: 0, 5: -1, 6: -1, 7: -1, 8: 5, 15: 3}),
+            ('dtn_paged_append', APPEND, {0: 0, 1: 0, 2: 0, 3: 0, 4: 0, 5: 0, 6: 0, 7: 0, 8: 0, 9: 0, 11: -1, 12: -1, 13: -1, 18: -1, 19: 0, 22: -1, 23: -1,
+                                          25: 5, 27: -1, 32: -1}),
+            ('dtn_paged_attention', ATTENTION, {0: 0, 1: 0, 2: 0, 3: 0, 4: 0, 6: 0, 9: -1, 10: 3, 11: 0, 17: -1, 18: 0, 21: -1, 22: -1, 24: -1, 25: 5}),
             ('dtn_copy_pages', copies, {0: None, 1: -1, 3: -1, 5: -1, 6: None, 7: None, 8: -1})):
         for place, value in bad.items():
-            arguments = list(good)
-            arguments[place] = value
-            if name == 'dtn_paged_attention' and place == 8:
-                arguments[9] = 2                                  # three query heads over two kv heads
-            assert getattr(library, name)(*arguments) == native.ERR_INVALID, (name, place)
+            changes = {place: value}
+            if name == 'dtn_paged_attention' and place == 10:
+                changes[11] = 2                                   # three query heads over two kv heads
+            assert status_of(name, good, changes) == native.ERR_INVALID, (name, place)
             assert native.last_error()
-    for name, good, changes in (('dtn_rotary', rotary, {7: 1025}), ('dtn_rotary', rotary, {5: 2 ** 31}), ('dtn_paged_append', append, {10: 1025}),
-                                ('dtn_paged_attention', attention, {10: 257}), ('dtn_copy_pages', copies, {8: 2 ** 31})):
-        arguments = list(good)
-        for place, value in changes.items():
-            arguments[place] = value
-        assert getattr(library, name)(*arguments) == native.ERR_UNSUPPORTED, (name, changes)
+    for name, good, changes in (('dtn_rotary', ROTARY, {7: 1025}), ('dtn_rotary', ROTARY, {5: 2 ** 31}), ('dtn_paged_append', APPEND, {13: 1025}),
+                                ('dtn_paged_append', APPEND, {23: 2 ** 31}), ('dtn_paged_attention', ATTENTION, {12: 264}), ('dtn_copy_pages', copies, {8: 2 ** 31})):
+        assert status_of(name, good, changes) == native.ERR_UNSUPPORTED, (name, changes)
     # nothing to do is no error, and needs no pointer and no device
-    for name, good, changes in (('dtn_rotary', rotary, {0: None, 5: 0}), ('dtn_rotary', rotary, {1: None, 6: 0}), ('dtn_paged_append', append, {0: None, 8: 0}),
-                                ('dtn_paged_attention', attention, {0: None, 7: 0}), ('dtn_copy_pages', copies, {0: None, 8: 0})):
-        arguments = list(good)
-        for place, value in changes.items():
-            arguments[place] = value
-        assert getattr(library, name)(*arguments) == native.OK, (name, changes)
+    for name, good, changes in (('dtn_rotary', ROTARY, {0: 0, 5: 0}), ('dtn_rotary', ROTARY, {1: 0, 6: 0}), ('dtn_paged_append', APPEND, {0: 0, 11: 0}),
+                                ('dtn_paged_attention', ATTENTION, {0: 0, 9: 0}), ('dtn_copy_pages', copies, {0: None, 8: 0})):
+        assert status_of(name, good, changes) == native.OK, (name, changes)
 
 
 def test_attention_entry_refuses_alignment_and_workspace():
-    library, one = native.lib(), 1 << 20
-    good = [one] * 7 + [1, 2, 1, 8, 16, 8, 16, 8, 4, 8, 64, 64, 1, 1, 1, 1.0, 0, 1, 1, one, 1 << 30, None]
     size = ctypes.c_size_t(0)
     native.call('dtn_paged_attention_workspace_bytes', ctypes.byref(size))
     assert 4096 < size.value < 16 << 20
-    for place, value, status, text in ((1, one + 8, native.ERR_INVALID, '16-byte'), (2, one + 2, native.ERR_INVALID, '16-byte'), (10, 12, native.ERR_INVALID, '16-byte'),
-                                       (17, 60, native.ERR_INVALID, '16-byte'), (18, 4, native.ERR_INVALID, '16-byte'), (26, None, native.ERR_WORKSPACE, 'workspace'),
-                                       (27, size.value - 1, native.ERR_WORKSPACE, 'needed'), (26, one + 4, native.ERR_WORKSPACE, 'aligned')):
-        arguments = list(good)
-        arguments[place] = value
-        assert library.dtn_paged_attention(*arguments) == status and text in native.last_error(), (place, native.last_error())
+    for place, value, status, text in ((1, ONE + 8, native.ERR_INVALID, '16-byte'), (2, ONE + 2, native.ERR_INVALID, '16-byte'), (12, 12, native.ERR_INVALID, '16-byte'),
+                                       (19, 60, native.ERR_INVALID, '16-byte'), (20, 4, native.ERR_INVALID, '16-byte'), (7, 0, native.ERR_WORKSPACE, 'workspace'),
+                                       (8, size.value - 1, native.ERR_WORKSPACE, 'needed'), (8, -1, native.ERR_WORKSPACE, 'needed'), (7, ONE + 4, native.ERR_WORKSPACE, 'aligned')):
+        good = list(ATTENTION)
+        good[25] = 1
+        assert status_of('dtn_paged_attention', good, {place: value}) == status and text in native.last_error(), (place, native.last_error())
 
 
 def test_the_plan_covers_every_unit_once_and_names_its_owners():
