@@ -354,7 +354,7 @@ _LAYOUTS = {'half': 0, 'interleaved': 1}
 
 def _on_current_device(*tensors: torch.Tensor) -> None:
     current = torch.cuda.current_device() if tensors[0].is_cuda else None
-    for tensor in tensors:
+    for tensor in tensors:   # -1 for a tensor of the CPU
         if tensor.get_device() != current:
             if not tensor.is_cuda:
                 raise ValueError('deuteron_b200 operators take CUDA tensors')
@@ -560,8 +560,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         q_out_token, q_out_head = _heads(q_out, 'q_out', written=True)
         if q_out.data_ptr() == q.data_ptr() and (q_out_token, q_out_head) != (q_token, q_head):
             raise ValueError('q_out must be q itself or lie elsewhere')
-        _on_current_device(q, q_out)
-    _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, k if frequencies is None else frequencies)
+    _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, *([] if frequencies is None else [frequencies]),
+                       *([] if q is None else [q, q_out]))
     native.call('dtn_paged_append', native.PAGED_APPEND_ARGS.pack(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(), positions.data_ptr(),
         frequencies.data_ptr() if pairs else 0, q.data_ptr() if q_heads else 0, q_out.data_ptr() if q_heads else 0,
@@ -650,10 +650,16 @@ def copy_pages(pages: torch.Tensor, sources: torch.Tensor, destinations: torch.T
     """
     _tensors(pages, sources, destinations)
     shape = pages.shape
-    if not 4 <= len(shape) <= 6:
+    if len(shape) == 5:
+        planes, count, heads, size, dim = shape
+    elif len(shape) == 4:
+        planes, (count, heads, size, dim) = 1, shape
+    elif len(shape) == 6:
+        layers, kinds, count, heads, size, dim = shape
+        planes = layers * kinds
+    else:
         raise ValueError('pages must be a [pages, kv_heads, page_size, dim] tensor, or one with one or two leading dimensions')
-    count, heads, size, dim = shape[-4:]
-    dense, planes = heads * size * dim, math.prod(shape[:-4])
+    dense = heads * size * dim
     page_stride, plane_stride = dense, count * dense
     if not pages.is_contiguous():
         strides = pages.stride()
