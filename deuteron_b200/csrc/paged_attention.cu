@@ -33,8 +33,8 @@
 //
 // Measured (kernel in a graph of 30 calls on three sets of inputs in turn, fraction of the 6540 GB/s of a copy):
 //   96 users, 17..8192 tokens, 32 heads on 8, 128, f16, 1.62 GB: 244 us (1.01); 16 users, 1..4096, 137 MB: 30 us (0.69, of
-//   which 3 us are the launch and the clearing of the counters); one user of 131071, bf16, 537 MB: 91 us (0.90; 55 blocks
-//   share each head, joining them costs 4 us, the slowest SM is 8 % behind the mean); 9 users, FP32, 16 heads of 64, 124 MB:
+//   which 3 us are the launch and the clearing of the counters); one user of 131071, bf16, 537 MB: 88.6 us (0.93; 37 blocks
+//   share each head, joining them costs 3 us, the slowest SM is 8 % behind the mean); 9 users, FP32, 16 heads of 64, 124 MB:
 //   29 us (0.65); 37 tokens of one user: 6 us. Head 64, 32 on 8: 0.88; head 80: 0.82; head 256: 0.82; groups of 16: 0.67, of
 //   32: 0.51; 256 users of 128..256 tokens: 0.70.
 #include <type_traits>
@@ -856,7 +856,11 @@ static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
   p.blocks = (p.group + C::HEADS - 1) / C::HEADS;
   p.heads = p.kv_heads * p.blocks;
   p.whole_sets = p.page_size % C::SUB == 0;
-  int64_t grid = (int64_t)sm_count() * C::BLOCKS_PER_SM;
+  // Two blocks per SM are enough to read, and where few items are shared by many blocks the fewer parts to join count more:
+  // 8 items 88.6 us against 91.4 with three (131071 tokens each) and 32.7 against 33.7 (32768); 16 items equal; 24 items 70.1
+  // against 68.9, 32 items 44.9 against 43.8.
+  const int64_t per_sm = C::BLOCKS_PER_SM > 2 && p.count <= 16 && p.count * p.heads <= 16 ? 2 : C::BLOCKS_PER_SM;
+  int64_t grid = (int64_t)sm_count() * per_sm;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;
   const int64_t unit = C::CHUNK * C::TEAMS, most_tiles = p.capacity > unit ? (p.capacity + unit - 1) / unit : 1;
   DTN_REQUIRE((double)p.count * p.heads * (double)(most_tiles + PA_ITEM_UNITS) < 2147483648.0 * (double)grid, DTN_ERR_UNSUPPORTED,
