@@ -484,14 +484,17 @@ def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> tor
     _index(positions, 'positions', tokens, wide=True)
     pairs = _rotation(frequencies, layout, dim)
     if out is None:
+        _on_current_device(x, positions, frequencies)
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _tensors(out)
-    if out.dtype != x.dtype or out.shape != x.shape:
-        raise ValueError('out must have the shape and dtype of x')
-    out_token_stride, out_head_stride = _heads(out, 'out', written=True)
-    if out.data_ptr() == x.data_ptr() and (out_token_stride, out_head_stride) != (token_stride, head_stride):
-        raise ValueError('out must be x itself or lie elsewhere')
-    _on_current_device(x, positions, frequencies, out)
+        out_token_stride, out_head_stride = heads * dim, dim
+    else:
+        _tensors(out)
+        if out.dtype != x.dtype or out.shape != x.shape:
+            raise ValueError('out must have the shape and dtype of x')
+        out_token_stride, out_head_stride = _heads(out, 'out', written=True)
+        if out.data_ptr() == x.data_ptr() and (out_token_stride, out_head_stride) != (token_stride, head_stride):
+            raise ValueError('out must be x itself or lie elsewhere')
+        _on_current_device(x, positions, frequencies, out)
     native.call('dtn_rotary', native.ROTARY_ARGS.pack(
         x.data_ptr(), out.data_ptr(), positions.data_ptr(), frequencies.data_ptr(), positions.dtype is torch.int64, tokens, heads, dim, pairs,
         token_stride, head_stride, out_token_stride, out_head_stride, _LAYOUTS[layout], transpose, _STORAGE_OF[x.dtype], float(amplitude)), _stream())
@@ -533,7 +536,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _tensors(k, v, k_pages, v_pages, tables, rows, positions)
     if k.dtype not in _STORAGE_OF or v.dtype != k.dtype or k_pages.dtype != k.dtype:
         raise ValueError('k, v and the pools must share dtype float32, float16 or bfloat16')
-    (k_token, k_head), (v_token, v_head) = _heads(k, 'k'), _heads(v, 'v')
+    k_token, k_head = _heads(k, 'k')
+    v_token, v_head = (k_token, k_head) if v.stride() == k.stride() and v.shape == k.shape else _heads(v, 'v')
     pages, pool_heads, page_size, pool_dim, page_stride, page_head_stride, sequences, width, table_stride = _pools(k_pages, v_pages, tables)
     tokens, kv_heads, dim = k.shape
     if v.shape != k.shape or pool_heads != kv_heads or pool_dim != dim:
@@ -552,16 +556,17 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         q_heads = q.shape[1]
         if q.dtype != k.dtype or q.shape[0] != tokens or q.shape[2] != dim:
             raise ValueError('q must be a [tokens, q_heads, dim] tensor of the dtype of k')
-        if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        _tensors(q_out)
-        if q_out.dtype != q.dtype or q_out.shape != q.shape:
-            raise ValueError('q_out must have the shape and dtype of q')
-        q_out_token, q_out_head = _heads(q_out, 'q_out', written=True)
-        if q_out.data_ptr() == q.data_ptr() and (q_out_token, q_out_head) != (q_token, q_head):
-            raise ValueError('q_out must be q itself or lie elsewhere')
-    _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, *([] if frequencies is None else [frequencies]),
-                       *([] if q is None else [q, q_out]))
+        if q_out is not None:
+            _tensors(q_out)
+            if q_out.dtype != q.dtype or q_out.shape != q.shape:
+                raise ValueError('q_out must have the shape and dtype of q')
+            q_out_token, q_out_head = _heads(q_out, 'q_out', written=True)
+            if q_out.data_ptr() == q.data_ptr() and (q_out_token, q_out_head) != (q_token, q_head):
+                raise ValueError('q_out must be q itself or lie elsewhere')
+    _on_current_device(k, v, k_pages, v_pages, tables, rows, positions, *[x for x in (frequencies, q, q_out) if x is not None])
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_out_token, q_out_head = q_heads * dim, dim
     native.call('dtn_paged_append', native.PAGED_APPEND_ARGS.pack(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), rows.data_ptr(), positions.data_ptr(),
         frequencies.data_ptr() if pairs else 0, q.data_ptr() if q_heads else 0, q_out.data_ptr() if q_heads else 0,
@@ -625,13 +630,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if type(window) is not int or not 0 <= window < 1 << 63:
         raise ValueError(f'window must be a non-negative integer, got {window!r}')
     scale = float(scale)
+    if out is not None:
+        _tensors(out)
+        if out.shape != q.shape or out.dtype not in (torch.float32, q.dtype):
+            raise ValueError('out must have the shape of q and dtype float32 or that of q')
+        out_token, out_head = _heads(out, 'out', written=True)
+    _on_current_device(q, k_pages, v_pages, tables, lengths, *[x for x in (rows, out) if x is not None])
     if out is None:
         out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)
-    _tensors(out)
-    if out.shape != q.shape or out.dtype not in (torch.float32, q.dtype):
-        raise ValueError('out must have the shape of q and dtype float32 or that of q')
-    out_token, out_head = _heads(out, 'out', written=True)
-    _on_current_device(q, k_pages, v_pages, tables, lengths, lengths if rows is None else rows, out)
+        out_token, out_head = q_heads * dim, dim
     stream = _stream()
     workspace, workspace_bytes = _paged_workspace(q, stream)
     native.call('dtn_paged_attention', native.PAGED_ATTENTION_ARGS.pack(

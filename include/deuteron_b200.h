@@ -84,7 +84,9 @@ int dtn_version(void);
 int dtn_last_error(char* buf, size_t n);
 
 /* Reads and clears the device-side status word that kernels with bounded waits write
- * when a wait runs out. This call synchronises `stream`. *status_out = 0 when clean.
+ * when a wait runs out, and the operators of a paged cache when they meet a page number, row, position or length that the
+ * pool or the tables do not cover (0x61nn attention, 0x62nn append, 0x63nn copies; nn the block). This call synchronises
+ * `stream`. *status_out = 0 when clean.
  * No reference counterpart (its kernels have no device-side waits on async units). */
 int dtn_device_status(int* status_out /* host */, void* stream);
 
