@@ -21,6 +21,8 @@ LIBRARY = PACKAGE / 'libdeuteron_b200.so'
 OBJECTS = CSRC / 'build'
 ARCH_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a']
 COMMON_FLAGS = ['-O3', '-std=c++17', '-lineinfo', '-Xcompiler', '-fPIC', '--expt-relaxed-constexpr']
+# Sources that must not use local memory (a build with spilled registers read wrong addresses): the assembler's warning is an error.
+SOURCE_FLAGS = {'paged_attention.cu': ['-Xptxas', '-warn-lmem-usage,-Werror']}
 
 
 def nvcc() -> str:
@@ -48,7 +50,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         obj = OBJECTS / (source.stem + '.o')
         stale = force or not obj.exists() or obj.stat().st_mtime < max(source.stat().st_mtime, header_time)
         if stale:
-            command = [compiler, *ARCH_FLAGS, *COMMON_FLAGS, '-c', str(source), '-o', str(obj)]
+            command = [compiler, *ARCH_FLAGS, *COMMON_FLAGS, *SOURCE_FLAGS.get(source.name, []), '-c', str(source), '-o', str(obj)]
             if verbose:
                 command.insert(1, '-Xptxas=-v')
             jobs.append(command)
