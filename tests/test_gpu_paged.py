@@ -398,6 +398,28 @@ def test_tensors_of_the_cpu_and_streams(cuda):
     assert all(torch.equal(y, expected) for y in results)
 
 
+def test_host_threads_on_their_own_streams(cuda):
+    import threading
+    k_pages, v_pages, tables, lens = M.a_cache([3000, 70], 2, 64, torch.float16, 16, 'cuda')
+    q = normal((2, 8, 64), torch.float16)
+    expected = ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.125)
+    torch.cuda.synchronize()
+    results = {}
+
+    def work(number):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results[number] = [ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.125) for _ in range(50)]
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(number,)) for number in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert all(torch.equal(y, expected) for number in range(4) for y in results[number])
+
+
 def test_captured_graphs_share_no_workspace(cuda):
     k_pages, v_pages, tables, lens = M.a_cache([5000, 170], 2, 64, torch.float16, 16, 'cuda')
     q = [normal((2, 8, 64), torch.float16, seed) for seed in range(2)]
