@@ -24,7 +24,8 @@
 //   apart: the tensor core's own accumulator truncates.
 //   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
 //   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
-//   heads are split into blocks that read the keys again. From 16 heads on the products, not the bytes, set the time.
+//   heads are split into blocks that read the keys again. From 16 heads on the products and the instructions around them, not the bytes, set
+//   the time.
 //   Join. A block that holds a whole item writes it. Otherwise it leaves (m, sum, numerators) in the workspace and counts
 //   itself in; the last to arrive adds the parts in the order of the blocks, so the result does not depend on who was last.
 //   It leaves the counter at zero for the next launch.
