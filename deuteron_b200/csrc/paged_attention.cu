@@ -19,9 +19,15 @@
 //   Products, 16-bit storage. mma.sync m16n8k16 with the tokens as the 16 rows and the query heads as the 8 columns:
 //   scores = K Q^T, numerators = V^T P^T, so that a group of up to 8 heads wastes nothing and the probabilities turn from
 //   result to operand layout with one movmatrix per 8 x 8. At the copy rate 8 heads need 80 TFLOP/s of products; tcgen05
-//   would need 64 or 128 rows of heads, or P through shared memory. P is split into two f16 or three bf16 terms, which keeps
-//   the products with V exact to about 2^-23, and a chunk's product starts from zero and is added to the FP32 numerator
-//   apart: the tensor core's own accumulator truncates.
+//   would need 64 or 128 rows of heads, or P through shared memory. P is split into terms of the storage type, and a chunk's
+//   product starts from zero and is added to the FP32 numerator apart: the tensor core's own accumulator truncates. Three
+//   bf16 terms leave 2^-24 of a probability. f16 has too few exponents for that: 2^-24 is its smallest step. So its
+//   probabilities are 2^BIAS times larger (the factor is in the sums as well and cancels), which puts the largest at 2^15, and
+//   the second of two terms is 2^REST times what the first leaves, with a product of its own that is scaled back when it is
+//   added. That leaves 2^-23 of a probability, or 2^-44 of 1 where that is more: 2^-44 is 2^-(25 + BIAS + REST), half a step
+//   of the second term; 1 is a token whose score is the maximum that the block keeps. (Two terms of one scale left 2^-25 of 1: 48
+//   tokens, one of them with a zero value and all but 1e-6 of the mass, were off by 1e-3, now by 5e-7. Neither form is
+//   slower than the other anywhere: the 96 users 247.3 and 247.3 us, groups of 16 98.9 and 98.9, head size 80 69.8 and 70.1.)
 //   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
 //   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
 //   heads are split into blocks that read the keys again. From 16 heads on the products and the instructions around them, not the bytes, set
@@ -118,6 +124,11 @@ __device__ __forceinline__ void pa_copy16(uint32_t dst, const void* src) {
 // Two FP32 sums in one instruction.
 __device__ __forceinline__ void pa_add2(float& a0, float& a1, float b0, float b1) {
   asm("{ .reg .b64 a, b; mov.b64 a, {%0, %1}; mov.b64 b, {%2, %3}; add.rn.f32x2 a, a, b; mov.b64 {%0, %1}, a; }" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+// a += b * c for two.
+__device__ __forceinline__ void pa_fma2(float& a0, float& a1, float b0, float b1, float c) {
+  asm("{ .reg .b64 a, b, c; mov.b64 a, {%0, %1}; mov.b64 b, {%2, %3}; mov.b64 c, {%4, %4}; fma.rn.f32x2 a, b, c, a; mov.b64 {%0, %1}, a; }"
+      : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1), "f"(c));
 }
 __device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -248,6 +259,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   constexpr int CHUNK = C::CHUNK, SETS = C::SETS, TEAMS = C::TEAMS, ROW = C::ROW, STAGES = C::STAGES, UNIT = CHUNK * TEAMS, THREADS = PA_WARPS * 32;
   constexpr int LANES = ROW / 16;                  // 16-byte vectors of a row
   constexpr float NONE = -INFINITY;
+  constexpr bool SPLIT = std::is_same_v<T, __half>;   // probabilities in two terms of different scales
+  constexpr float REST = 4096.f;                      // half a step of the first term, at most 2^3, stays below f16's largest value
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_max[PA_WARPS][8], s_sum[PA_WARPS][8];
   __shared__ __align__(16) float s_p[C::HALF ? 1 : PA_WARPS][C::HALF ? 1 : CHUNK][NH], s_alpha[C::HALF ? 1 : PA_WARPS][8];
@@ -550,8 +563,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           if (base + g + 8 * n >= seen || base + g + 8 * n < now.s.skip) x[n][0] = x[n][1] = NONE;
       }
       // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
-      // neither f16 terms nor FP32 sums mind, and nothing is exchanged or rescaled.
-      constexpr float GROWTH = 8.f;
+      // FP32 sums do not mind and f16 terms have room for (2^(GROWTH + BIAS) = 2^15), and nothing is exchanged or rescaled.
+      constexpr float GROWTH = 8.f, BIAS = SPLIT ? 7.f : 0.f;
       bool higher = false;
 #pragma unroll
       for (int n = 0; n < EIGHTS; ++n) higher |= x[n][0] > top[0] + GROWTH || x[n][1] > top[1] + GROWTH;
@@ -587,7 +600,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float around = top[i] == NONE ? 0.f : top[i];   // every score -inf so far: the exponentials are zeros, not NaN
+        const float around = top[i] == NONE ? 0.f : top[i] - BIAS;   // every score -inf so far: the exponentials are zeros, not NaN
 #pragma unroll
         for (int n = 0; n < EIGHTS; ++n) {
           x[n][i] = ex2_approx_ftz(x[n][i] - around);
@@ -596,30 +609,65 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
       if constexpr (C::HALF) {
         if (!exactly) {
-          constexpr int TERMS = std::is_same_v<T, __half> ? 2 : 3;
+          constexpr int TERMS = SPLIT ? 2 : 3;
           uint32_t b[SETS][TERMS][2];
 #pragma unroll
           for (int set = 0; set < SETS; ++set)
 #pragma unroll
             for (int n = 0; n < TERMS; ++n)
 #pragma unroll
-              for (int half = 0; half < 2; ++half) b[set][n][half] = pa_transpose(pa_take(x[2 * set + half][0], x[2 * set + half][1], T()));
+              for (int half = 0; half < 2; ++half) {
+                float &p0 = x[2 * set + half][0], &p1 = x[2 * set + half][1];
+                if (SPLIT && n == 1) p0 *= REST, p1 *= REST;
+                b[set][n][half] = pa_transpose(pa_take(p0, p1, T()));
+              }
           const uint32_t v_place = stage + CHUNK * ROW + (lane % 8 + lane / 16 * 8) * ROW + ((lane / 8 % 2) ^ (lane % 8)) * 16;
+          auto load_values = [&](uint32_t(&a)[4], int mt, int set) { pa_ldmatrix_t(a, (v_place ^ (mt % 4 * 32)) + mt / 4 * 128 + set * 16 * ROW); };
+          // Registers for one product only: the small terms' is scaled back and goes on as the large ones', which reads the values again.
+          constexpr bool TWICE = SPLIT && DP == 256 && SETS > 1;
 #pragma unroll
           for (int mt = 0; mt < DP / 16; ++mt) {
             if (mt == DP / 16 * 3 / 4 && p.dim <= DP * 3 / 4) break;
             float y[4];
+            if constexpr (TWICE) {
+#pragma unroll
+              for (int set = 0; set < SETS; ++set) {
+                uint32_t a[4];
+                load_values(a, mt, set);
+                if (set == 0)
+                  pa_mma_first(y, a, b[set][1][0], b[set][1][1], T());
+                else
+                  pa_mma(y, a, b[set][1][0], b[set][1][1], T());
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] *= 1.f / REST;
+            }
+            float rest[4];
 #pragma unroll
             for (int set = 0; set < SETS; ++set) {
               uint32_t a[4];
-              pa_ldmatrix_t(a, (v_place ^ (mt % 4 * 32)) + mt / 4 * 128 + set * 16 * ROW);
+              load_values(a, mt, set);
+              if constexpr (SPLIT) {
+                if (set == 0 && !TWICE) {
+                  pa_mma_first(rest, a, b[set][1][0], b[set][1][1], T());
+                  pa_mma_first(y, a, b[set][0][0], b[set][0][1], T());
+                } else {
+                  if (!TWICE) pa_mma(rest, a, b[set][1][0], b[set][1][1], T());
+                  pa_mma(y, a, b[set][0][0], b[set][0][1], T());
+                }
+              } else {
 #pragma unroll
-              for (int n = TERMS - 1; n >= 0; --n) {   // small terms first
-                if (set == 0 && n == TERMS - 1)
-                  pa_mma_first(y, a, b[set][n][0], b[set][n][1], T());
-                else
-                  pa_mma(y, a, b[set][n][0], b[set][n][1], T());
+                for (int n = TERMS - 1; n >= 0; --n) {   // small terms first
+                  if (set == 0 && n == TERMS - 1)
+                    pa_mma_first(y, a, b[set][n][0], b[set][n][1], T());
+                  else
+                    pa_mma(y, a, b[set][n][0], b[set][n][1], T());
+                }
               }
+            }
+            if constexpr (SPLIT && !TWICE) {
+              pa_fma2(acc[mt][0], acc[mt][1], rest[0], rest[1], 1.f / REST);
+              pa_fma2(acc[mt][2], acc[mt][3], rest[2], rest[3], 1.f / REST);
             }
             pa_add2(acc[mt][0], acc[mt][1], y[0], y[1]);
             pa_add2(acc[mt][2], acc[mt][3], y[2], y[3]);

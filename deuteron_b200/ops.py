@@ -606,7 +606,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     them). rows: int32 [n], the sequence of each query (None: query i is sequence i); a negative row (padding of a captured
     batch) and a length of zero give zeros. window > 0 keeps the last `window` tokens only. Query head h reads kv head
     h // (q_heads // kv_heads). Heads have a multiple of 16 bytes (at most 256 elements) and start on 16-byte boundaries in the
-    pools. Storage float32 / float16 / bfloat16, softmax and sums in FP32; `out` is float32 by default, as
+    pools. Storage float32 / float16 / bfloat16, softmax and sums in FP32 (float16: a probability counts to 2^-23 of itself or 2^-44
+    of the largest, whichever is more); `out` is float32 by default, as
     `gqa_attention` returns it, or a given tensor of float32 or of q's dtype. The values in a page behind a sequence's end do
     not matter, NaN included. A row or length outside the tables, or a page number outside the pool, makes
     `check_device_status` raise PageError; a sequence with such a page gets NaN.

@@ -382,6 +382,7 @@ int dtn_paged_append(const dtn_paged_append_args* args /* host */, void* stream)
  * length of zero gives zeros. out is FP32, or of `storage` when out_f32 is zero. A row >= sequences or a length beyond the tables is
  * reported by dtn_device_status (the length is cut), and so is a page number outside the pool, which makes the sequence's
  * output NaN; nothing outside the pools is read. What lies in the pools behind a sequence's end is not used, whatever it holds.
+ * Softmax and sums are FP32; with f16 storage a probability counts to 2^-23 of itself or 2^-44 of the largest, whichever is more.
  * Heads of the pools have a multiple of 16 bytes (at most 256 elements) and start on 16-byte boundaries. `workspace` has
  * dtn_paged_attention_workspace_bytes bytes, 16-byte aligned, and is zeroed once before its first call; every call leaves its
  * first 4096 bytes (counters) zero again. Calls that can overlap on the GPU need a workspace each. Same result on every
