@@ -260,6 +260,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   constexpr int LANES = ROW / 16;                  // 16-byte vectors of a row
   constexpr float NONE = -INFINITY;
   constexpr bool SPLIT = std::is_same_v<T, __half>;   // probabilities in two terms of different scales
+  // Probabilities are held 2^BIAS times larger than against the maximum, in the second pass over an item 2^AGAIN times.
+  constexpr float BIAS = SPLIT ? 7.f : 0.f, AGAIN = SPLIT ? BIAS : -23.f;
   constexpr float REST = 4096.f;                      // half a step of the first term, at most 2^3, stays below f16's largest value
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_max[PA_WARPS][8], s_sum[PA_WARPS][8];
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   float top[2] = {NONE, NONE}, total_p[2] = {0.f, 0.f};   // of heads 2t, 2t + 1
   constexpr int A = C::HALF ? DP / 16 : NH, B = C::HALF ? 4 : COLUMNS;
   float acc[A][B];                                 // numerators: 16 columns of V by 2 heads, or NH heads by COLUMNS
-  bool fresh = true, exactly = false;
+  bool fresh = true, again = false;
   int start = 0;                                   // the item's first tile here
   int slot = 0, filling = STAGES - 1;              // the oldest stage; copies still to be issued before the first stage is read
 
@@ -564,10 +566,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
       // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
       // FP32 sums do not mind and f16 terms have room for (2^(GROWTH + BIAS) = 2^15), and nothing is exchanged or rescaled.
-      constexpr float GROWTH = 8.f, BIAS = SPLIT ? 7.f : 0.f;
+      constexpr float GROWTH = 8.f;
+      const float growth = SPLIT || !again ? GROWTH : 0.f;
       bool higher = false;
 #pragma unroll
-      for (int n = 0; n < EIGHTS; ++n) higher |= x[n][0] > top[0] + GROWTH || x[n][1] > top[1] + GROWTH;
+      for (int n = 0; n < EIGHTS; ++n) higher |= x[n][0] > top[0] + growth || x[n][1] > top[1] + growth;
       if (__any_sync(0xffffffffu, higher)) {
         float alpha[2];
 #pragma unroll
@@ -600,15 +603,19 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float around = top[i] == NONE ? 0.f : top[i] - BIAS;   // every score -inf so far: the exponentials are zeros, not NaN
+        const float around = top[i] == NONE ? 0.f : top[i] - (again ? AGAIN : BIAS);   // every score -inf so far: the exponentials are zeros, not NaN
+        if (SPLIT || !again) {
 #pragma unroll
-        for (int n = 0; n < EIGHTS; ++n) {
-          x[n][i] = ex2_approx_ftz(x[n][i] - around);
-          total_p[i] += x[n][i];
+          for (int n = 0; n < EIGHTS; ++n) x[n][i] = ex2_approx_ftz(x[n][i] - around);
+        } else {   // as far down as the first pass: results below 2^-126 too
+#pragma unroll
+          for (int n = 0; n < EIGHTS; ++n) x[n][i] = ex2_approx(x[n][i] - around);
         }
+#pragma unroll
+        for (int n = 0; n < EIGHTS; ++n) total_p[i] += x[n][i];
       }
       if constexpr (C::HALF) {
-        if (!exactly) {
+        if (!again) {
           constexpr int TERMS = SPLIT ? 2 : 3;
           uint32_t b[SETS][TERMS][2];
 #pragma unroll
@@ -729,7 +736,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
         if (g == 0) {
-          s_max[warp][2 * t + i] = top[i];
+          s_max[warp][2 * t + i] = top[i] == NONE ? NONE : top[i] - (again ? AGAIN : BIAS);   // what the part's exponents are relative to
           s_sum[warp][2 * t + i] = total_p[i];
         }
       }
@@ -749,18 +756,17 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
             numerators[h * DP + (d ^ ((h / 2) << 3))] = acc[h][j];
           }
       }
-      if constexpr (!C::HALF) {
-        __syncthreads();
-      } else {
-        // Everybody's part is there behind this barrier. An infinite value times one term of a probability, negative or zero, is
-        // not what it is times the probability: where a numerator is not finite the block goes over its tiles of the item once
-        // more, with whole probabilities.
+      {
+        // Everybody's part is there behind this barrier. Where a numerator is not finite the block goes over its tiles of the item
+        // once more. 16-bit storage takes whole probabilities then: an infinite value times one term of a probability, negative
+        // or zero, is not what it is times the probability. And where values can be so large that their sum, but not their mean,
+        // passes FP32 (bf16 and FP32), the probabilities are 2^-23 at most: 2^23 tokens of the largest value can be added.
         float probe = 0.f;
-        if (!exactly) {
+        if (!again) {
 #pragma unroll
-          for (int mt = 0; mt < DP / 16; ++mt)
+          for (int i = 0; i < A; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) probe = fmaf(acc[mt][j], 0.f, probe);
+            for (int j = 0; j < B; ++j) probe = fmaf(acc[i][j], 0.f, probe);
         }
         if (__syncthreads_or(probe != 0.f)) {
           pa_wait<0>();
@@ -769,13 +775,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           now.tile = start;
           ahead = now;
           look_up();
-          if constexpr (DP == 64) load_query(query_next, now.sequence, now.kv_head, now.block);
-          exactly = fresh = true;
+          if constexpr (C::HALF && DP == 64) load_query(query_next, now.sequence, now.kv_head, now.block);
+          again = fresh = true;
           slot = 0;
           filling = STAGES - 1;
           continue;
         }
-        exactly = false;
+        again = false;
       }
       const bool whole = start == 0 && to_end;
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + (start == 0 ? 1 : 0)) * C::PART;
@@ -809,7 +815,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
 #pragma unroll
         for (int m = 0; m < TEAMS; ++m) {
           const int w = m * HB + slot_head / 8;
-          const float weight = ex2_approx_ftz(s_max[w][slot_head % 8] - around);
+          const float weight = ex2_approx_ftz(s_max[w][slot_head % 8] - around) * (1.f / TEAMS);   // finite parts have a finite sum
           const float* from = reinterpret_cast<const float*>(smem + (m * STAGES + slot) * C::STAGE);
           const float4 x = *reinterpret_cast<const float4*>(from + slot_head * DP + (d ^ (((slot_head % 8) / 2) << 3)));
           y.x = fmaf(weight, x.x, y.x), y.y = fmaf(weight, x.y, y.y), y.z = fmaf(weight, x.z, y.z), y.w = fmaf(weight, x.w, y.w);
@@ -834,6 +840,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           // The parts, added in the order of the blocks: the first block's second part, then every other's first, which lie at
           // one distance; PA_JOIN of them requested at once.
           const int count = (int)(last - first);
+          constexpr float SHARED = 1.f / PA_MAX_BLOCKS;   // finite parts have a finite sum
           const float* parts = p.parts + (first * 2 + 1) * C::PART;
 #pragma unroll 1
           for (int i = tid; i < C::HEADS * DP / 4; i += THREADS) {
@@ -843,7 +850,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
             const float* state = parts + C::HEADS * DP + 2 * slot_head;   // maximum and sum
             float4 y = __ldcg(reinterpret_cast<const float4*>(number));
             const float2 started = __ldcg(reinterpret_cast<const float2*>(state));
-            float high = started.x, sum_p = started.y;
+            float high = started.x, sum_p = started.y * SHARED;
+            y.x *= SHARED, y.y *= SHARED, y.z *= SHARED, y.w *= SHARED;
             number += C::PART, state += C::PART;
 #pragma unroll 1
             for (int n = 0; n < count; n += PA_JOIN, number += 2 * PA_JOIN * C::PART, state += 2 * PA_JOIN * C::PART) {
@@ -866,7 +874,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
               y.x *= before_weight, y.y *= before_weight, y.z *= before_weight, y.w *= before_weight, sum_p *= before_weight;
 #pragma unroll
               for (int j = 0; j < PA_JOIN; ++j) {
-                const float weight = ex2_approx_ftz(part[j].x - around);
+                const float weight = ex2_approx_ftz(part[j].x - around) * SHARED;
                 y.x = fmaf(weight, x[j].x, y.x), y.y = fmaf(weight, x[j].y, y.y), y.z = fmaf(weight, x[j].z, y.z), y.w = fmaf(weight, x[j].w, y.w);
                 sum_p = fmaf(weight, part[j].y, sum_p);
               }

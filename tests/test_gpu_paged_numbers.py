@@ -71,3 +71,43 @@ def test_small_probabilities_in_every_form(cuda, dim, heads, dtype):
 @pytest.mark.parametrize('dtype', TYPES)
 def test_a_long_tail_of_one_sign(cuda, dtype):
     within(*tail_below_a_sink(30_000, (8, 8), 64, dtype, 64, 18, 4))        # 2^-26 each
+
+
+# -- values near the end of the type's range -----------------------------------------------------
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads', [(1, 1), (4, 1), (8, 1), (12, 1), (32, 1)])
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_the_largest_values_have_a_finite_mean(cuda, dim, heads, dtype):
+    # their sum passes FP32, the result does not. The second pass adds 23 to a score's distance from the maximum: below 64, it
+    # rounds to 2^-19, in numerators and denominators. Every column has one sign, so the sum of magnitudes is the result's
+    lengths = [40, 1, 700, 0, 5000]
+    k_pages, v_pages, tables, lens = M.a_cache(lengths, heads[1], dim, dtype, 16, 'cuda', seed=4)
+    largest = torch.finfo(dtype).max
+    sign = torch.where(torch.arange(dim, device='cuda') % 2 == 0, 1.0, -1.0)
+    v_pages.copy_(((0.5 + 0.49 * torch.rand(v_pages.shape, generator=torch.Generator().manual_seed(6)).cuda()).double() * largest * sign).to(dtype))
+    q = torch.randn(5, heads[0], dim, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    for window in (0, 100):
+        exact, bound = M.attend(q, k_pages, v_pages, tables, lens, M.scale_of(dim), window=window)
+        y = ops.paged_attention(q, k_pages, v_pages, tables, lens, M.scale_of(dim), window=window)
+        empty = lens == 0
+        assert not y[empty].any()
+        within(y[~empty], exact[~empty], (bound + 2.0 ** -18 * exact.abs())[~empty])
+        narrow = ops.paged_attention(q, k_pages, v_pages, tables, lens, M.scale_of(dim), window=window, out=torch.empty_like(q))
+        assert narrow.isfinite().all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_infinite_values_of_a_small_probability(cuda, dtype):
+    # e^-76 is above 2^-126: the result is infinite, in the column and the query heads that see it only
+    k_pages, v_pages, tables, lens = M.a_cache([50, 50], 1, 64, dtype, 16, 'cuda')
+    k_pages.zero_()
+    page = int(tables[0, 1])
+    k_pages[page, 0, 3, 0] = -76.0
+    v_pages[page, 0, 3, 7] = float('-inf')
+    q = torch.zeros(2, 4, 64, dtype=dtype, device='cuda')
+    q[..., 0] = 1.0
+    y = ops.paged_attention(q, k_pages, v_pages, tables, lens, 1.0)
+    assert torch.isneginf(y[0, :, 7]).all()
+    y[0, :, 7] = 0.0
+    assert y.isfinite().all()
