@@ -33,8 +33,12 @@ class PageBook:
     """Which sequence owns which pages: tables, lengths, reference counts and free pages, all on the host.
 
     Methods that move or hand out pages return `(copies, updates)`: pairs (source page, destination page) to be copied
-    before anything is written, and entries (row, column, page) of the tables that changed.
+    before anything is written, and entries (row, column, page) of the tables that changed; those that take pages away return
+    `updates`. An entry that a sequence does not hold is NO_PAGE, a number outside every pool: the operators store nothing there
+    and report it.
     """
+
+    NO_PAGE = -1
 
     def __init__(self, pages: int, page_size: int, max_sequences: int, max_pages_per_sequence: int):
         for label, value in (('pages', pages), ('page_size', page_size), ('max_sequences', max_sequences),
@@ -44,7 +48,7 @@ class PageBook:
         if max_pages_per_sequence * page_size >= 1 << 31 or max_sequences * max_pages_per_sequence >= 1 << 31:
             raise ValueError('a sequence holds fewer than 2^31 tokens, the tables fewer than 2^31 entries')
         self.page_size = page_size
-        self.tables = np.zeros((max_sequences, max_pages_per_sequence), dtype=np.int32)
+        self.tables = np.full((max_sequences, max_pages_per_sequence), self.NO_PAGE, dtype=np.int32)
         self.lengths = np.zeros(max_sequences, dtype=np.int32)
         self.references = np.zeros(pages, dtype=np.int32)
         self._free_pages = list(range(pages))             # heaps: the lowest number first
@@ -63,11 +67,15 @@ class PageBook:
     def _held(self, row: int) -> int:
         return -(-int(self.lengths[row]) // self.page_size)
 
-    def _release(self, pages: np.ndarray) -> None:
-        for page in pages.tolist():
+    def _release(self, row: int, kept: int) -> list[tuple[int, int, int]]:
+        """Takes the pages from column `kept` on away from a row: updates."""
+        held = self._held(row)
+        for page in self.tables[row, kept:held].tolist():
             self.references[page] -= 1
             if self.references[page] == 0:
                 heapq.heappush(self._free_pages, page)
+        self.tables[row, kept:held] = self.NO_PAGE
+        return [(row, column, self.NO_PAGE) for column in range(kept, held)]
 
     def open(self) -> int:
         """A row for a new, empty sequence."""
@@ -77,13 +85,14 @@ class PageBook:
         self._open[row] = True
         return row
 
-    def close(self, row: int) -> None:
-        """Frees a sequence: its row, and the pages that no fork shares."""
+    def close(self, row: int) -> list[tuple[int, int, int]]:
+        """Frees a sequence: its row, and the pages that no fork shares: updates."""
         row = self._row(row)
-        self._release(self.tables[row, :self._held(row)])
+        updates = self._release(row, 0)
         self.lengths[row] = 0
         self._open[row] = False
         heapq.heappush(self._free_rows, row)
+        return updates
 
     def fork(self, row: int) -> tuple[int, list[tuple[int, int, int]]]:
         """A new sequence with the tokens of `row`, sharing its pages: (new row, updates)."""
@@ -137,14 +146,14 @@ class PageBook:
         self.references[page] = 1
         return page
 
-    def truncate(self, row: int, length: int) -> None:
-        """Forgets the tokens of `row` from `length` on (drafts that were not accepted)."""
+    def truncate(self, row: int, length: int) -> list[tuple[int, int, int]]:
+        """Forgets the tokens of `row` from `length` on (drafts that were not accepted): updates."""
         row = self._row(row)
         if not 0 <= length <= self.lengths[row]:
             raise ValueError(f'row {row} holds {self.lengths[row]} tokens, cannot keep {length!r}')
-        kept = -(-int(length) // self.page_size)
-        self._release(self.tables[row, kept:self._held(row)])
+        updates = self._release(row, -(-int(length) // self.page_size))
         self.lengths[row] = length
+        return updates
 
     def compact(self) -> tuple[list[tuple[int, int]], list[tuple[int, int, int]]]:
         """Moves the pages in use to the lowest numbers: (copies, updates). Sources and destinations are disjoint."""
@@ -170,7 +179,9 @@ class PagedCache:
     """Keys and values of all layers in pages, with the operators of `ops` on them.
 
     `pool` is [layers, 2, pages, kv_heads, page_size, head_dim]; `tables` and `lengths` are the device's copies of the book's,
-    changed in place, so a captured step keeps reading the current ones.
+    changed in place, so a captured step keeps reading the current ones. Entries of `tables` that no sequence holds are negative: an
+    append to a closed row, or to a page that was not extended to or was given back, stores nothing and is reported. Within the pages
+    that a row holds the positions of `extend` are the caller's to keep: a page may be shared with a fork.
     """
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, max_sequences: int,
@@ -185,7 +196,7 @@ class PagedCache:
         self.book = PageBook(pages, page_size, max_sequences, pages if max_pages_per_sequence is None else max_pages_per_sequence)
         device = torch.device('cuda' if device is None else device)
         self.pool = torch.empty((layers, 2, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
-        self.tables = torch.zeros(self.book.tables.shape, dtype=torch.int32, device=device)
+        self.tables = torch.full(self.book.tables.shape, PageBook.NO_PAGE, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(max_sequences, dtype=torch.int32, device=device)
         if self.pool.is_cuda:
             with torch.cuda.device(self.pool.device):
@@ -220,8 +231,7 @@ class PagedCache:
 
     def close(self, row: int) -> None:
         """Frees a sequence: its row, and the pages that no fork shares."""
-        self.book.close(row)
-        self._apply([], [], [row])
+        self._apply([], self.book.close(row), [row])
 
     def fork(self, row: int) -> int:
         """A new sequence with the tokens of `row`. Its pages are shared until one of the two writes."""
@@ -242,8 +252,7 @@ class PagedCache:
 
     def truncate(self, row: int, length: int) -> None:
         """Forgets the tokens of `row` from `length` on."""
-        self.book.truncate(row, length)
-        self._apply([], [], [row])
+        self._apply([], self.book.truncate(row, length), [row])
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers, in one launch; returns how many moved."""

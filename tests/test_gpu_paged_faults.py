@@ -1,0 +1,42 @@
+"""Calls of the paged operators that must be reported or must not disturb others."""
+import pytest
+import torch
+
+from deuteron_b200 import native, ops
+from deuteron_b200.paged import PagedCache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    native.device_status(0)
+    yield
+    ops.check_device_status()
+
+
+def test_appends_outside_what_a_row_holds_are_reported(cuda):
+    cache = PagedCache(layers=1, pages=8, page_size=4, kv_heads=2, head_dim=64, max_sequences=4, max_pages_per_sequence=5)
+    cache.pool.fill_(3.0)
+    closed, kept, cut, fresh = (cache.open() for _ in range(4))
+    cache.extend([closed, cut], [6, 10])
+    cache.close(closed)
+    cache.extend([kept], [12])                       # takes the pages of the closed row
+    cache.truncate(cut, 3)
+    before = cache.pool.clone()
+    k = torch.ones(1, 2, 64, dtype=torch.float16, device='cuda')
+    for row, position in ((closed, 0), (closed, 5), (cut, 4), (cut, 9), (cut, 12), (fresh, 0), (kept, 12)):
+        cache.append(0, k, k, torch.tensor([row], dtype=torch.int32).cuda(), torch.tensor([position], dtype=torch.int32).cuda())
+        with pytest.raises(native.PageError, match='paged append'):
+            ops.check_device_status()
+        assert torch.equal(cache.pool, before), (row, position)
+    reopened = cache.open()                          # the closed row's number
+    assert reopened == closed
+    cache.append(0, k, k, torch.tensor([reopened], dtype=torch.int32).cuda(), torch.tensor([0], dtype=torch.int32).cuda())
+    with pytest.raises(native.PageError, match='paged append'):
+        ops.check_device_status()
+    assert torch.equal(cache.pool, before)
+    rows, positions = cache.extend([kept], [1])
+    cache.append(0, k, k, rows, positions)
+    ops.check_device_status()
+    assert not torch.equal(cache.pool, before)
