@@ -94,6 +94,14 @@ int dtn_device_status(int* status_out, void* stream) {
   return DTN_OK;
 }
 
+int dtn_device_status_prepare(void* stream) {
+  if (dtn::device_status_word_unless_capturing(dtn::as_stream(stream)) != nullptr) return DTN_OK;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  DTN_CUDA_CHECK(cudaStreamIsCapturing(dtn::as_stream(stream), &capturing));
+  DTN_REQUIRE(capturing != cudaStreamCaptureStatusNone, DTN_ERR_CUDA, "dtn_device_status_prepare: no status word on this device");
+  return DTN_OK;
+}
+
 int dtn_capture_begin(void* stream) {
   cudaStream_t s = dtn::as_stream(stream);
   DTN_REQUIRE(s != nullptr, DTN_ERR_INVALID, "dtn_capture_begin: a stream of its own is needed (not the default stream)");

@@ -46,6 +46,7 @@ _SIGNATURES = {
     'dtn_version': [],
     'dtn_last_error': [ct.c_char_p, ct.c_size_t],
     'dtn_device_status': [ct.POINTER(ct.c_int), _P],
+    'dtn_device_status_prepare': [_P],
     'dtn_selftest_wait_timeout': [ct.c_longlong, _P],
     'dtn_copy_block': [_P, ct.c_size_t, _P, ct.c_size_t, ct.c_size_t, ct.c_size_t, _I, _P],
     'dtn_capture_begin': [_P],

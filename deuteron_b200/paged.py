@@ -200,7 +200,7 @@ class PagedCache:
         self.lengths = torch.zeros(max_sequences, dtype=torch.int32, device=device)
         if self.pool.is_cuda:
             with torch.cuda.device(self.pool.device):
-                native.device_status()   # the word that reports go to exists before any capture
+                native.call('dtn_device_status_prepare', torch.cuda.current_stream().cuda_stream)   # the word that reports go to exists before any capture
 
     def keys(self, layer: int) -> torch.Tensor:
         return self.pool[layer, 0]

@@ -90,6 +90,11 @@ int dtn_last_error(char* buf, size_t n);
  * No reference counterpart (its kernels have no device-side waits on async units). */
 int dtn_device_status(int* status_out /* host */, void* stream);
 
+/* Makes the status word of the current device, where it is not there yet and `stream` is not being captured (the word is
+ * allocated outside captures only: an operator of a paged cache that is captured before it exists reports nothing). What the word
+ * holds stays. No reference counterpart. */
+int dtn_device_status_prepare(void* stream);
+
 /* What the kernels of a call cost, for result records that carry those fields (benchmark.py:218-220 of the
  * reference reads them from its one PTX entry with cuFuncGetAttribute). dtn_capture_begin puts `stream` (not the
  * default stream) into capture; the caller then makes the library calls it wants described, which are recorded, not

@@ -40,3 +40,26 @@ def test_appends_outside_what_a_row_holds_are_reported(cuda):
     cache.append(0, k, k, rows, positions)
     ops.check_device_status()
     assert not torch.equal(cache.pool, before)
+
+
+def test_a_new_cache_leaves_reports_standing(cuda):
+    pool = torch.zeros(1, 1, 4, 64, dtype=torch.float16, device='cuda')
+    one = torch.tensor([1], dtype=torch.int32).cuda()
+    ops.copy_pages(pool, one, one)                   # a page outside the pool
+    torch.cuda.synchronize()
+    PagedCache(layers=1, pages=2, page_size=4, kv_heads=1, head_dim=64, max_sequences=1)
+    with pytest.raises(native.PageError, match='copy of pages'):
+        ops.check_device_status()
+    native.call('dtn_selftest_wait_timeout', 1000, torch.cuda.current_stream().cuda_stream)   # a wait with a budget that runs out
+    torch.cuda.synchronize()
+    PagedCache(layers=1, pages=2, page_size=4, kv_heads=1, head_dim=64, max_sequences=1)
+    with pytest.raises(native.DeviceWaitError, match='self-test'):
+        ops.check_device_status()
+
+
+def test_a_cache_made_in_a_capture(cuda):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache = PagedCache(layers=1, pages=2, page_size=4, kv_heads=1, head_dim=64, max_sequences=2)
+    graph.replay()
+    assert bool((cache.tables == -1).all()) and not cache.lengths.any()
