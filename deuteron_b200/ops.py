@@ -580,10 +580,11 @@ _paged_workspaces: dict[tuple[int, int], tuple[torch.Tensor, int, int]] = {}
 _PAGED_COUNTER_BYTES = 4096
 
 
-def _paged_workspace(q: torch.Tensor, stream: int) -> tuple[int, int]:
-    """Address and size of the parts and counters of `paged_attention`, one workspace per device and stream. Its counters are zeroed
-    here once; every call leaves them zero. A call that is captured gets one of its own from the graph's memory, zeroed by each
-    replay: replays may run beside one another and beside eager calls."""
+def _paged_workspace(q: torch.Tensor, stream: int) -> tuple[torch.Tensor, int, int]:
+    """The parts and counters of `paged_attention`, its address and size: one workspace per device and stream (15 MB, kept as the
+    products' are). Its counters are zeroed here once; every call leaves them zero. A call that is captured gets one of its own from
+    the graph's memory, zeroed by each replay: replays may run beside one another and beside eager calls. The caller holds the
+    tensor until its launch is queued; of threads that make a stream's first call at once all get the workspace of one."""
     capturing = torch.cuda.is_current_stream_capturing()
     key = (q.get_device(), stream)
     held = None if capturing else _paged_workspaces.get(key)
@@ -594,8 +595,8 @@ def _paged_workspace(q: torch.Tensor, stream: int) -> tuple[int, int]:
         workspace[:_PAGED_COUNTER_BYTES].zero_()
         held = workspace, workspace.data_ptr(), size.value
         if not capturing:
-            _paged_workspaces[key] = held
-    return held[1:]
+            held = _paged_workspaces.setdefault(key, held)
+    return held
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, scale: float,
@@ -641,7 +642,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)
         out_token, out_head = q_heads * dim, dim
     stream = _stream()
-    workspace, workspace_bytes = _paged_workspace(q, stream)
+    held, workspace, workspace_bytes = _paged_workspace(q, stream)
     native.call('dtn_paged_attention', native.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), lengths.data_ptr(), 0 if rows is None else rows.data_ptr(),
         out.data_ptr(), workspace, workspace_bytes, count, q_heads, kv_heads, dim, q_token, q_head, out_token, out_head, pages, page_size,

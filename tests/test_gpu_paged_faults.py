@@ -1,7 +1,10 @@
 """Calls of the paged operators that must be reported or must not disturb others."""
+import threading
+
 import pytest
 import torch
 
+import paged_math as M
 from deuteron_b200 import native, ops
 from deuteron_b200.paged import PagedCache
 
@@ -63,3 +66,25 @@ def test_a_cache_made_in_a_capture(cuda):
         cache = PagedCache(layers=1, pages=2, page_size=4, kv_heads=1, head_dim=64, max_sequences=2)
     graph.replay()
     assert bool((cache.tables == -1).all()) and not cache.lengths.any()
+
+
+def test_threads_call_first_on_one_shared_stream(cuda):
+    k_pages, v_pages, tables, lens = M.a_cache([3000, 70], 2, 64, torch.float16, 16, 'cuda')
+    q = torch.randn(2, 8, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    expected = ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.125)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    results, meeting = {}, threading.Barrier(6)
+
+    def work(number):
+        with torch.cuda.stream(stream):
+            meeting.wait(30)
+            results[number] = [ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.125) for _ in range(20)]
+
+    threads = [threading.Thread(target=work, args=(number,)) for number in range(6)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, expected) for number in range(6) for y in results[number])

@@ -1,8 +1,10 @@
 """Calls of the paged cache that go wrong on the host's side; no GPU."""
+import threading
+
 import pytest
 import torch
 
-from deuteron_b200 import ops
+from deuteron_b200 import native, ops
 from deuteron_b200.paged import PageBook, PagedCache
 
 
@@ -45,3 +47,34 @@ def test_the_book_names_what_it_takes_away():
     book.extend([row], [7])
     assert book.truncate(row, 5) == [(row, 3, -1)] and book.truncate(row, 5) == []
     assert book.close(row) == [(row, 0, -1), (row, 1, -1), (row, 2, -1)] and book.free_pages == 4
+
+
+def test_threads_that_call_first_on_one_stream_share_its_workspace(monkeypatch):
+    # both threads are held inside the creation until the other is there
+    meeting = threading.Barrier(2)
+
+    def call(name, size):
+        assert name == 'dtn_paged_attention_workspace_bytes'
+        size._obj.value = 8192
+        meeting.wait(10)
+
+    monkeypatch.setattr(native, 'call', call)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(ops, '_paged_workspaces', {})
+    results = []
+    threads = [threading.Thread(target=lambda: results.append(ops._paged_workspace(torch.zeros(1), 7))) for _ in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert len(results) == 2 and results[0][-2:] == results[1][-2:]
+    kept, = ops._paged_workspaces.values()
+    assert kept[0].data_ptr() == results[0][-2] and not kept[0][:4096].any()
+
+
+def test_a_captured_call_holds_its_workspace(monkeypatch):
+    monkeypatch.setattr(native, 'call', lambda name, size: setattr(size._obj, 'value', 8192))
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    monkeypatch.setattr(ops, '_paged_workspaces', {})
+    first, second = (ops._paged_workspace(torch.zeros(1), 7) for _ in range(2))
+    assert isinstance(first[0], torch.Tensor) and first[0].data_ptr() == first[1] != second[1] and not ops._paged_workspaces
