@@ -54,6 +54,21 @@ constexpr int PA_WARPS = 4;
 constexpr int PA_MAX_BLOCKS = 1024;        // counters in the workspace
 constexpr int PA_COUNTER_BYTES = PA_MAX_BLOCKS * 4;
 
+// position / divisor as a multiplication, for positions below 2^31 and divisors from 1 to 2^31 - 1: mul = floor(2^(31 + s) / d) + 1
+// with 2^s >= d exceeds 2^(31 + s) / d by at most 1, so the product exceeds the quotient by less than 2^31 / 2^(31 + s) <= 1 / d:
+// the floor is exact. mul <= 2^32 - 1 needs d > 1; for d = 1 the multiplier is 1 and the shift 0.
+struct PaDivider {
+  uint32_t mul;
+  int shift;
+  __host__ __device__ __forceinline__ int operator()(int position) const { return (int)(((uint64_t)(uint32_t)position * mul) >> shift); }
+};
+static PaDivider pa_divider(int64_t divisor) {
+  if (divisor == 1) return {1, 0};
+  int bits = 1;
+  while ((1LL << bits) < divisor) ++bits;
+  return {(uint32_t)((1ULL << (31 + bits)) / (uint64_t)divisor + 1), 31 + bits};
+}
+
 struct PagedAttentionParams {
   const void *q, *k_pages, *v_pages;
   void* out;
@@ -66,8 +81,7 @@ struct PagedAttentionParams {
   int heads, kv_heads;                  // items per sequence: kv heads x blocks of query heads
   int blocks;                           // blocks of query heads per kv head
   int q_heads, group, dim, page_size, row_bytes;
-  uint32_t divide_mul;                  // position / page_size = (position * divide_mul) >> divide_shift
-  int divide_shift;
+  PaDivider pages_of;                   // position / page_size
   float scale_log2e;
   int out_f32;
   int q_pairs, out_quads;               // neighbouring elements of q and out can be moved by two (4 bytes) and by four
@@ -348,7 +362,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
     offset = -1;
     if (token < ahead.s.seen && token >= ahead.s.skip) {
       const int position = ahead.s.first + token;
-      const int index = (int)(((uint64_t)(uint32_t)position * p.divide_mul) >> p.divide_shift);
+      const int index = p.pages_of(position);
       const int page = p.tables[ahead.s.table + index];
       offset = -2;
       if (page >= 0 && page < p.pages)
@@ -980,6 +994,18 @@ int dtn_paged_attention_plan(const int64_t* tiles, int64_t count, int64_t heads,
   return DTN_OK;
 }
 
+int dtn_paged_attention_pages(const int* positions, int64_t count, int64_t page_size, int* pages_out) {
+  using namespace dtn;
+  DTN_REQUIRE(count >= 0 && (count == 0 || (positions && pages_out)), DTN_ERR_INVALID, "paged attention pages: null pointer or negative count");
+  DTN_REQUIRE(page_size >= 1 && page_size < (1LL << 31), DTN_ERR_INVALID, "paged attention pages: page size %lld", (long long)page_size);
+  const PaDivider pages_of = pa_divider(page_size);
+  for (int64_t i = 0; i < count; ++i) {
+    DTN_REQUIRE(positions[i] >= 0, DTN_ERR_INVALID, "paged attention pages: negative position");
+    pages_out[i] = pages_of(positions[i]);
+  }
+  return DTN_OK;
+}
+
 int dtn_paged_attention(const dtn_paged_attention_args* args, void* stream) {
   using namespace dtn;
   DTN_REQUIRE(args != nullptr, DTN_ERR_INVALID, "paged attention: no arguments");
@@ -1039,18 +1065,7 @@ int dtn_paged_attention(const dtn_paged_attention_args* args, void* stream) {
   const int64_t out_element = a.out_f32 ? 4 : element;
   p.out_quads = aligned_to(a.out, 4 * out_element) && a.out_token_stride % 4 == 0 && a.out_head_stride % 4 == 0;
   p.min_units = 1 + PA_ITEM_UNITS;
-  // position / page_size for positions below 2^31: mul = floor(2^(31 + s) / d) + 1 with 2^s >= d exceeds 2^(31 + s) / d by at
-  // most 1, so the product exceeds the quotient by less than 2^31 / 2^(31 + s) <= 1 / d: the floor is exact. mul <= 2^32 - 1
-  // needs d > 1; for d = 1 the multiplier is 1 and the shift 0.
-  if (a.page_size == 1) {
-    p.divide_mul = 1;
-    p.divide_shift = 0;
-  } else {
-    int bits = 1;
-    while ((1LL << bits) < a.page_size) ++bits;
-    p.divide_shift = 31 + bits;
-    p.divide_mul = (uint32_t)((1ULL << (31 + bits)) / (uint64_t)a.page_size + 1);
-  }
+  p.pages_of = pa_divider(a.page_size);
   p.counters = static_cast<int*>(a.workspace);
   p.parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + PA_COUNTER_BYTES);
   p.status = device_status_word_unless_capturing(s);

@@ -78,6 +78,7 @@ _SIGNATURES = {
     'dtn_paged_attention_workspace_bytes': [ct.POINTER(ct.c_size_t)],
     'dtn_paged_attention_plan': [ct.POINTER(ct.c_int64), _I64, _I64, _I64, _I64, ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64),
                                  ct.POINTER(ct.c_int64), ct.POINTER(ct.c_int64)],
+    'dtn_paged_attention_pages': [ct.POINTER(ct.c_int), _I64, _I64, ct.POINTER(ct.c_int)],
     'dtn_copy_pages': [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P],
 }
 

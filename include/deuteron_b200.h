@@ -418,6 +418,10 @@ int dtn_paged_attention_plan(const int64_t* tiles /* host */, int64_t count, int
                              int64_t* begin_out /* host */, int64_t* first_out /* host */, int64_t* last_out /* host */,
                              int64_t* workers_out /* host */);
 
+/* pages_out[i] = positions[i] / page_size as dtn_paged_attention computes it, by a multiplication: host arithmetic only, the kernel's
+ * own function. Positions are below 2^31. */
+int dtn_paged_attention_pages(const int* positions /* host */, int64_t count, int64_t page_size, int* pages_out /* host */);
+
 /* Copies page sources[i] onto page destinations[i] in each of `planes` planes of a pool (a layer's keys or values each),
  * i < pairs. Strides and page_bytes in bytes; a page's bytes are dense. No destination may be a source or occur twice. A
  * page number outside [0, pages) copies nothing for its pair and is reported by dtn_device_status. */

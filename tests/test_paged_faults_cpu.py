@@ -1,4 +1,6 @@
 """Calls of the paged cache that go wrong on the host's side; no GPU."""
+import ctypes
+import random
 import threading
 
 import pytest
@@ -78,3 +80,19 @@ def test_a_captured_call_holds_its_workspace(monkeypatch):
     monkeypatch.setattr(ops, '_paged_workspaces', {})
     first, second = (ops._paged_workspace(torch.zeros(1), 7) for _ in range(2))
     assert isinstance(first[0], torch.Tensor) and first[0].data_ptr() == first[1] != second[1] and not ops._paged_workspaces
+
+
+def test_the_kernels_own_division_of_positions_is_exact():
+    generator = random.Random(5)
+    most = 2 ** 31 - 1
+    sizes = [1, 2, 3, 5, 7, 8, 16, 24, 50, 64, 1000, 2 ** 16, 2 ** 16 + 1, 2 ** 20 - 1, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, most - 1, most]
+    for size in sizes + [generator.randint(1, most) for _ in range(300)] + [generator.randint(1, 4096) for _ in range(300)]:
+        near = [generator.randint(0, most // size) * size + step for _ in range(60) for step in (-1, 0, 1)]   # around multiples
+        ends = [most // size * size + step for step in (-1, 0, 1)] + [most - i for i in range(20)] + [size - 1, size, size + 1]
+        positions = [n for n in near + ends + [0, 1] + [generator.randint(0, most) for _ in range(50)] if 0 <= n <= most]
+        found = (ctypes.c_int * len(positions))()
+        native.call('dtn_paged_attention_pages', (ctypes.c_int * len(positions))(*positions), len(positions), size, found)
+        assert list(found) == [n // size for n in positions], size
+    one = (ctypes.c_int * 1)(-1)
+    for arguments in ((one, 1, 8, one), (one, 1, 0, one), (one, 1, 2 ** 31, one), (one, -1, 8, one), (None, 1, 8, one), (one, 1, 8, None)):
+        assert native.lib().dtn_paged_attention_pages(*arguments) == native.ERR_INVALID
