@@ -274,8 +274,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   constexpr int LANES = ROW / 16;                  // 16-byte vectors of a row
   constexpr float NONE = -INFINITY;
   constexpr bool SPLIT = std::is_same_v<T, __half>;   // probabilities in two terms of different scales
-  // Probabilities are held 2^BIAS times larger than against the maximum, in the second pass over an item 2^AGAIN times.
-  constexpr float BIAS = SPLIT ? 7.f : 0.f, AGAIN = SPLIT ? BIAS : -23.f;
+  constexpr float BIAS = SPLIT ? 7.f : 0.f;           // probabilities are held 2^BIAS times larger than against the maximum
+  constexpr float FEWER = SPLIT ? 0.f : 23.f, FEW = SPLIT ? 1.f : 1.f / 8388608.f;   // and 2^FEWER times smaller in a second pass
+  constexpr float GROWTH = 8.f;
   constexpr float REST = 4096.f;                      // half a step of the first term, at most 2^3, stays below f16's largest value
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_max[PA_WARPS][8], s_sum[PA_WARPS][8];
@@ -469,6 +470,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
   float top[2] = {NONE, NONE}, total_p[2] = {0.f, 0.f};   // of heads 2t, 2t + 1
   constexpr int A = C::HALF ? DP / 16 : NH, B = C::HALF ? 4 : COLUMNS;
   float acc[A][B];                                 // numerators: 16 columns of V by 2 heads, or NH heads by COLUMNS
+  float growth = GROWTH;                           // how far scores may pass the maximum before it moves
   bool fresh = true, again = false;
   int start = 0;                                   // the item's first tile here
   int slot = 0, filling = STAGES - 1;              // the oldest stage; copies still to be issued before the first stage is read
@@ -580,8 +582,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
       // The maximum moves only when a score passes it by more than GROWTH: until then probabilities reach 2^GROWTH, which
       // FP32 sums do not mind and f16 terms have room for (2^(GROWTH + BIAS) = 2^15), and nothing is exchanged or rescaled.
-      constexpr float GROWTH = 8.f;
-      const float growth = SPLIT || !again ? GROWTH : 0.f;
       bool higher = false;
 #pragma unroll
       for (int n = 0; n < EIGHTS; ++n) higher |= x[n][0] > top[0] + growth || x[n][1] > top[1] + growth;
@@ -617,16 +617,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float around = top[i] == NONE ? 0.f : top[i] - (again ? AGAIN : BIAS);   // every score -inf so far: the exponentials are zeros, not NaN
-        if (SPLIT || !again) {
+        const float around = top[i] == NONE ? 0.f : top[i] - BIAS;   // every score -inf so far: the exponentials are zeros, not NaN
 #pragma unroll
-          for (int n = 0; n < EIGHTS; ++n) x[n][i] = ex2_approx_ftz(x[n][i] - around);
-        } else {   // as far down as the first pass: results below 2^-126 too
-#pragma unroll
-          for (int n = 0; n < EIGHTS; ++n) x[n][i] = ex2_approx(x[n][i] - around);
+        for (int n = 0; n < EIGHTS; ++n) {
+          x[n][i] = ex2_approx_ftz(x[n][i] - around);
+          total_p[i] += x[n][i];
         }
+      }
+      if (!SPLIT && again) {
 #pragma unroll
-        for (int n = 0; n < EIGHTS; ++n) total_p[i] += x[n][i];
+        for (int n = 0; n < EIGHTS; ++n) x[n][0] *= FEW, x[n][1] *= FEW;
       }
       if constexpr (C::HALF) {
         if (!again) {
@@ -750,8 +750,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) total_p[i] += __shfl_xor_sync(0xffffffffu, total_p[i], o);
         if (g == 0) {
-          s_max[warp][2 * t + i] = top[i] == NONE ? NONE : top[i] - (again ? AGAIN : BIAS);   // what the part's exponents are relative to
-          s_sum[warp][2 * t + i] = total_p[i];
+          s_max[warp][2 * t + i] = again ? top[i] + FEWER : top[i];   // a part is relative to 2^(this - BIAS)
+          s_sum[warp][2 * t + i] = again ? total_p[i] * FEW : total_p[i];
         }
       }
       team_barrier();   // every member has read the stage
@@ -791,11 +791,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaConfig<T, DP, HB, NH>::BLOCKS
           look_up();
           if constexpr (C::HALF && DP == 64) load_query(query_next, now.sequence, now.kv_head, now.block);
           again = fresh = true;
+          if (!SPLIT) growth = 0.f;
           slot = 0;
           filling = STAGES - 1;
           continue;
         }
         again = false;
+        growth = GROWTH;
       }
       const bool whole = start == 0 && to_end;
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + (start == 0 ? 1 : 0)) * C::PART;
