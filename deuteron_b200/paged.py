@@ -18,6 +18,7 @@ that change the book outside captures; `append` and `attend` may be captured.
 from __future__ import annotations
 
 import heapq
+import operator
 
 import numpy as np
 import torch
@@ -27,6 +28,13 @@ from . import native, ops
 
 class PagesExhausted(RuntimeError):
     """There are not enough free pages; nothing was changed."""
+
+
+def _whole(value, label: str) -> int:
+    try:
+        return operator.index(value)
+    except TypeError:
+        raise ValueError(f'{label} must be an integer, got {value!r}') from None
 
 
 class PageBook:
@@ -60,9 +68,10 @@ class PageBook:
         return len(self._free_pages)
 
     def _row(self, row: int) -> int:
+        row = _whole(row, 'a row')
         if not 0 <= row < len(self._open) or not self._open[row]:
             raise ValueError(f'row {row!r} is not an open sequence')
-        return int(row)
+        return row
 
     def _held(self, row: int) -> int:
         return -(-int(self.lengths[row]) // self.page_size)
@@ -106,7 +115,7 @@ class PageBook:
 
     def extend(self, rows, counts) -> tuple[list[tuple[int, int]], list[tuple[int, int, int]]]:
         """Makes room for counts[i] more tokens of rows[i] (each row once) and counts them in: (copies, updates)."""
-        rows, counts = [self._row(row) for row in rows], [int(count) for count in counts]
+        rows, counts = [self._row(row) for row in rows], [_whole(count, 'a count') for count in counts]
         if len(rows) != len(counts) or len(set(rows)) != len(rows) or any(count < 0 for count in counts):
             raise ValueError('extend takes one non-negative count for each of different rows')
         capacity = self.tables.shape[1] * self.page_size
@@ -148,10 +157,10 @@ class PageBook:
 
     def truncate(self, row: int, length: int) -> list[tuple[int, int, int]]:
         """Forgets the tokens of `row` from `length` on (drafts that were not accepted): updates."""
-        row = self._row(row)
+        row, length = self._row(row), _whole(length, 'a length')
         if not 0 <= length <= self.lengths[row]:
             raise ValueError(f'row {row} holds {self.lengths[row]} tokens, cannot keep {length!r}')
-        updates = self._release(row, -(-int(length) // self.page_size))
+        updates = self._release(row, -(-length // self.page_size))
         self.lengths[row] = length
         return updates
 
@@ -244,10 +253,10 @@ class PagedCache:
         nothing, where pages are missing. Returns rows and positions of the new tokens (int32, in that order) for `append`.
         A shared page that would be written is copied first."""
         rows, counts = list(rows), list(counts)
-        before = [int(self.book.lengths[row]) if 0 <= row < len(self.book.lengths) else 0 for row in rows]
         copies, updates = self.book.extend(rows, counts)
-        token_rows = np.repeat(np.array(rows, dtype=np.int32), np.array(counts, dtype=np.int64))
-        positions = np.concatenate([np.arange(start, start + count, dtype=np.int32) for start, count in zip(before, counts)] or [np.zeros(0, np.int32)])
+        rows, counts = np.array(rows, dtype=np.int64), np.array(counts, dtype=np.int64)
+        token_rows = np.repeat(rows, counts)
+        positions = np.arange(len(token_rows)) + np.repeat(self.book.lengths[rows] - np.cumsum(counts), counts)   # the last token's is its row's length - 1
         return self._apply(copies, updates, rows, (token_rows, positions))
 
     def truncate(self, row: int, length: int) -> None:

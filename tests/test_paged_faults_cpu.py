@@ -3,6 +3,7 @@ import ctypes
 import random
 import threading
 
+import numpy as np
 import pytest
 import torch
 
@@ -96,3 +97,17 @@ def test_the_kernels_own_division_of_positions_is_exact():
     one = (ctypes.c_int * 1)(-1)
     for arguments in ((one, 1, 8, one), (one, 1, 0, one), (one, 1, 2 ** 31, one), (one, -1, 8, one), (None, 1, 8, one), (one, 1, 8, None)):
         assert native.lib().dtn_paged_attention_pages(*arguments) == native.ERR_INVALID
+
+
+def test_rows_counts_and_lengths_are_whole_numbers():
+    cache = a_cache()
+    a, b = cache.open(), cache.open()
+    cache.extend([np.int64(a), torch.tensor(b)], [np.int32(3), torch.tensor(2)])
+    state = cache.tables.clone(), cache.lengths.tolist(), cache.book.lengths.tolist(), cache.book.free_pages
+    for call in (lambda: cache.extend([a], [1.5]), lambda: cache.extend([a], [2.0]), lambda: cache.extend([float(a)], [1]), lambda: cache.extend(['0'], [1]),
+                 lambda: cache.truncate(a, 1.5), lambda: cache.close(0.0), lambda: cache.fork(None), lambda: cache.extend([a, b], [1, '1'])):
+        with pytest.raises(ValueError, match='integer'):
+            call()
+        assert torch.equal(cache.tables, state[0]) and (cache.lengths.tolist(), cache.book.lengths.tolist(), cache.book.free_pages) == state[1:]
+    rows, positions = cache.extend([a, b], [2, 1])
+    assert rows.tolist() == [a, a, b] and positions.tolist() == [3, 4, 2]
