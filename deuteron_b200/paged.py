@@ -227,12 +227,18 @@ class PagedCache:
         numbers = torch.from_numpy(np.concatenate([np.asarray(part, dtype=np.int32) for part in lists])).to(self.pool.device, non_blocking=True)   # pageable memory is staged before the call returns
         sources, destinations, places, pages, changed, lengths, *tokens = numbers.split(sizes)
         if copies:
-            ops.copy_pages(self.pool, sources, destinations)
+            with torch.cuda.device_of(self.pool):   # the book has changed already: also where another device is current
+                ops.copy_pages(self.pool, sources, destinations)
         if updates:
             self.tables.view(-1).index_copy_(0, places.long(), pages)
         if len(rows):
             self.lengths.index_copy_(0, changed.long(), lengths)
         return tuple(tokens)
+
+    def _outside_captures(self) -> None:
+        """The book would change once, its copy to the device be repeated by every replay."""
+        if self.pool.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('a cache is closed, forked, extended, truncated and compacted outside captures; append and attend may be captured')
 
     def open(self) -> int:
         """A row for a new, empty sequence."""
@@ -240,10 +246,12 @@ class PagedCache:
 
     def close(self, row: int) -> None:
         """Frees a sequence: its row, and the pages that no fork shares."""
+        self._outside_captures()
         self._apply([], self.book.close(row), [row])
 
     def fork(self, row: int) -> int:
         """A new sequence with the tokens of `row`. Its pages are shared until one of the two writes."""
+        self._outside_captures()
         new, updates = self.book.fork(row)
         self._apply([], updates, [new])
         return new
@@ -252,6 +260,7 @@ class PagedCache:
         """Makes room for counts[i] more tokens of rows[i] (each row once) and counts them in; raises PagesExhausted, and changes
         nothing, where pages are missing. Returns rows and positions of the new tokens (int32, in that order) for `append`.
         A shared page that would be written is copied first."""
+        self._outside_captures()
         rows, counts = list(rows), list(counts)
         copies, updates = self.book.extend(rows, counts)
         rows, counts = np.array(rows, dtype=np.int64), np.array(counts, dtype=np.int64)
@@ -261,10 +270,12 @@ class PagedCache:
 
     def truncate(self, row: int, length: int) -> None:
         """Forgets the tokens of `row` from `length` on."""
+        self._outside_captures()
         self._apply([], self.book.truncate(row, length), [row])
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest numbers, in one launch; returns how many moved."""
+        self._outside_captures()
         copies, updates = self.book.compact()
         if copies:
             self._apply(copies, updates, [])

@@ -88,3 +88,23 @@ def test_threads_call_first_on_one_shared_stream(cuda):
         thread.join()
     torch.cuda.synchronize()
     assert all(torch.equal(y, expected) for number in range(6) for y in results[number])
+
+
+def test_the_book_does_not_change_inside_a_capture(cuda):
+    cache = PagedCache(layers=1, pages=8, page_size=4, kv_heads=1, head_dim=64, max_sequences=3)
+    a = cache.open()
+    cache.extend([a], [6])
+    fork = cache.fork(a)
+    state = cache.tables.tolist(), cache.lengths.tolist(), cache.book.tables.tolist(), cache.book.references.tolist()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.extend([a], [1]), lambda: cache.extend([fork], [0]), lambda: cache.close(a), lambda: cache.fork(a), lambda: cache.truncate(a, 2),
+                     cache.compact):
+            with pytest.raises(RuntimeError, match='outside captures'):
+                call()
+        graph_only = torch.zeros(1, device='cuda')
+    graph.replay()
+    assert not graph_only.any()
+    assert (cache.tables.tolist(), cache.lengths.tolist(), cache.book.tables.tolist(), cache.book.references.tolist()) == state
+    cache.extend([a, fork], [1, 1])
+    assert torch.equal(cache.tables.cpu(), torch.from_numpy(cache.book.tables)) and cache.lengths.tolist()[:2] == [7, 7]
