@@ -475,8 +475,30 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
     return torch.tensor(frequencies, dtype=torch.float64, device='cuda' if device is None else device), amplitude
 
 
+class _Turned(torch.autograd.Function):
+    """`rotary` and `rotary_backward` where a gradient is recorded: each is the other's."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, layout, amplitude, transpose):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.rest = layout, amplitude, 1 - transpose
+        return _rotary(x, positions, frequencies, layout, amplitude, None, transpose)
+
+    @staticmethod
+    def backward(ctx, grad):
+        if grad.shape[-1] > 1 and grad.stride(-1) != 1:   # a sum's gradient is one value expanded
+            grad = grad.contiguous()
+        return _rotary(grad, *ctx.saved_tensors, *ctx.rest[:2], None, ctx.rest[2]), None, None, None, None, None
+
+
 def _rotary(x, positions, frequencies, layout, amplitude, out, transpose) -> torch.Tensor:
     _tensors(x, positions, frequencies)
+    if (x.requires_grad or frequencies.requires_grad) and torch.is_grad_enabled():
+        if frequencies.requires_grad:
+            raise ValueError('frequencies have no gradient')
+        if out is not None:
+            raise ValueError('a result in `out` has no gradient: call without it, or under torch.no_grad()')
+        return _Turned.apply(x, positions, frequencies, layout, amplitude, transpose)
     if x.dtype not in _STORAGE_OF:
         raise ValueError(f'x must have dtype float32, float16 or bfloat16, got {x.dtype}')
     token_stride, head_stride = _heads(x, 'x')
@@ -508,7 +530,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     x: [tokens, heads, dim], float32 / float16 / bfloat16, any token and head strides, dense heads (a slice of a fused
     projection); positions: int32 or int64 [tokens]; frequencies: float64 [pairs] from `rotary_frequencies`. Pair i is
     (i, i + pairs) in the 'half' layout, (2i, 2i + 1) in the 'interleaved' one; elements from 2 * pairs on are copied. The
-    angle is formed in 64 bits, the result rounded once. `out` may be x itself; otherwise it must not overlap x.
+    angle is formed in 64 bits and reduced to a fraction of a turn; its sine and cosine and the rotation are FP32 (2^-21 of a pair's
+    magnitude), the result is rounded once. `out` may be x itself; otherwise it must not overlap x. The gradient of x is recorded
+    where x requires one (`rotary_backward`); positions and frequencies have none.
     """
     return _rotary(x, positions, frequencies, layout, amplitude, out, 0)
 
@@ -516,7 +540,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
 def rotary_backward(grad: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = 'half', amplitude: float = 1.0,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of `rotary`'s x from the gradient of its result: the transposed map (each pair turned back, times `amplitude`).
-    Same arguments; positions and frequencies have no gradient."""
+    Same arguments."""
     return _rotary(grad, positions, frequencies, layout, amplitude, out, 1)
 
 
@@ -531,7 +555,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     positions[t] % page_size. With `frequencies` the keys are rotated as `rotary` does, and so is `q` [tokens, q_heads, dim],
     which is returned (in `q_out`, which may be q itself, or a new tensor); values are stored as they are. A row, position or
     page number outside the tables or the pool stores nothing and makes `check_device_status` raise PageError. No two
-    tokens of a call may have the same place.
+    tokens of a call may have the same place. Nothing is recorded for gradients.
     """
     _tensors(k, v, k_pages, v_pages, tables, rows, positions)
     if k.dtype not in _STORAGE_OF or v.dtype != k.dtype or k_pages.dtype != k.dtype:
@@ -611,7 +635,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     of the largest, whichever is more); `out` is float32 by default, as
     `gqa_attention` returns it, or a given tensor of float32 or of q's dtype. The values in a page behind a sequence's end do
     not matter, NaN included. A row or length outside the tables, or a page number outside the pool, makes
-    `check_device_status` raise PageError; a sequence with such a page gets NaN.
+    `check_device_status` raise PageError; a sequence with such a page gets NaN. Nothing is recorded for gradients.
     """
     _tensors(q, k_pages, v_pages, tables, lengths)
     if q.dtype not in _STORAGE_OF or k_pages.dtype != q.dtype:

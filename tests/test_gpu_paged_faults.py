@@ -108,3 +108,52 @@ def test_the_book_does_not_change_inside_a_capture(cuda):
     assert (cache.tables.tolist(), cache.lengths.tolist(), cache.book.tables.tolist(), cache.book.references.tolist()) == state
     cache.extend([a, fork], [1, 1])
     assert torch.equal(cache.tables.cpu(), torch.from_numpy(cache.book.tables)) and cache.lengths.tolist()[:2] == [7, 7]
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+def test_the_gradient_of_rotary_is_recorded(cuda, layout, dtype):
+    g = torch.Generator().manual_seed(2)
+    projected = torch.randn(7, 6, 64, generator=g).to(dtype).cuda().requires_grad_()
+    positions = torch.randint(0, 5000, (7,), generator=g).cuda()
+    w, amplitude = ops.rotary_frequencies(48, scaling='yarn', factor=4.0, original_length=64)
+    weight = torch.randn(7, 4, 64, generator=g).to(dtype).cuda()
+    x = projected[:, 1:5]
+    y = ops.rotary(x, positions, w, layout=layout, amplitude=amplitude)
+    with torch.no_grad():
+        plain = ops.rotary(x, positions, w, layout=layout, amplitude=amplitude)
+    assert y.requires_grad and not plain.requires_grad and torch.equal(y, plain)
+    y.backward(weight)
+    expected = torch.zeros_like(projected)
+    expected[:, 1:5] = ops.rotary_backward(weight, positions, w, layout=layout, amplitude=amplitude)
+    assert torch.equal(projected.grad, expected)
+    projected.grad = None
+    ops.rotary(projected, positions, w, layout=layout).sum().backward()          # the gradient arrives as one expanded value
+    assert torch.equal(projected.grad, ops.rotary_backward(torch.ones_like(projected), positions, w, layout=layout).detach())
+    back = ops.rotary_backward(x, positions, w, layout=layout)
+    gradient, = torch.autograd.grad(back, projected, weight, create_graph=True)
+    assert torch.equal(gradient[:, 1:5], ops.rotary(weight, positions, w, layout=layout))
+    # of the gradient as a function of what it is applied to: the map is linear
+    leaf = weight.clone().requires_grad_()
+    first, = torch.autograd.grad(ops.rotary(x, positions, w, layout=layout), projected, leaf, create_graph=True)
+    second, = torch.autograd.grad(first[:, 1:5], leaf, weight)
+    assert torch.equal(second, ops.rotary(weight, positions, w, layout=layout))
+
+
+def test_rotary_records_on_streams_and_in_captures(cuda):
+    x = torch.randn(9, 3, 32, generator=torch.Generator().manual_seed(3)).cuda().requires_grad_()
+    positions, (w, _) = torch.arange(9, device='cuda'), ops.rotary_frequencies(32)
+    expected = ops.rotary_backward(torch.ones(9, 3, 32, device='cuda'), positions, w)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            gradient, = torch.autograd.grad(ops.rotary(x, positions, w).sum(), x)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(gradient, expected)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured, = torch.autograd.grad(ops.rotary(x, positions, w).sum(), x)
+    captured.zero_()
+    graph.replay()
+    assert torch.equal(captured, expected)

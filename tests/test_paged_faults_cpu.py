@@ -111,3 +111,14 @@ def test_rows_counts_and_lengths_are_whole_numbers():
         assert torch.equal(cache.tables, state[0]) and (cache.lengths.tolist(), cache.book.lengths.tolist(), cache.book.free_pages) == state[1:]
     rows, positions = cache.extend([a, b], [2, 1])
     assert rows.tolist() == [a, a, b] and positions.tolist() == [3, 4, 2]
+
+
+def test_rotary_refuses_gradients_that_it_cannot_record():
+    x, at, w = torch.zeros(3, 2, 16, requires_grad=True), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.float64)
+    for call in (ops.rotary, ops.rotary_backward):
+        with pytest.raises(ValueError, match='no_grad'):
+            call(x, at, w, out=torch.zeros(3, 2, 16))
+        with pytest.raises(ValueError, match='frequencies have no gradient'):
+            call(x.detach(), at, w.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(ValueError, match='CUDA'):
+            call(x, at, w.clone().requires_grad_(), out=torch.zeros(3, 2, 16))
