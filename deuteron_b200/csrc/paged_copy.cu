@@ -63,7 +63,7 @@ extern "C" int dtn_copy_pages(void* pool, int64_t planes, int64_t plane_stride_b
   DTN_REQUIRE(planes >= 0 && pages >= 0 && page_bytes >= 0 && pairs >= 0, DTN_ERR_INVALID, "copy pages: negative extent");
   if (planes == 0 || pages == 0 || page_bytes == 0 || pairs == 0) return DTN_OK;
   DTN_REQUIRE(pool && sources && destinations, DTN_ERR_INVALID, "copy pages: null pointer");
-  DTN_REQUIRE(pages < (1LL << 31) && pairs < (1LL << 31) && planes * pairs < (1LL << 31), DTN_ERR_UNSUPPORTED, "copy pages: too many pages for one launch");
+  DTN_REQUIRE(pages < (1LL << 31) && pairs < (1LL << 31) && planes <= ((1LL << 31) - 1) / pairs, DTN_ERR_UNSUPPORTED, "copy pages: too many pages for one launch");
   cudaStream_t s = as_stream(stream);
   CopyParams p = {static_cast<char*>(pool), plane_stride_bytes, page_stride_bytes, page_bytes, planes, pages, pairs, sources, destinations,
                   device_status_word_unless_capturing(s)};

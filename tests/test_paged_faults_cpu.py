@@ -122,3 +122,9 @@ def test_rotary_refuses_gradients_that_it_cannot_record():
             call(x.detach(), at, w.clone().requires_grad_())
         with torch.no_grad(), pytest.raises(ValueError, match='CUDA'):
             call(x, at, w.clone().requires_grad_(), out=torch.zeros(3, 2, 16))
+
+
+def test_copies_of_too_many_planes_are_refused():
+    one = 1 << 20
+    for planes, pairs in ((2 ** 62, 4), (2 ** 33, 2 ** 30), (2 ** 31, 1), (2, 2 ** 30)):
+        assert native.lib().dtn_copy_pages(one, planes, 64, 4, 64, 64, one, one, pairs, None) == native.ERR_UNSUPPORTED, (planes, pairs)
