@@ -633,7 +633,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     h // (q_heads // kv_heads). Heads have a multiple of 16 bytes (at most 256 elements) and start on 16-byte boundaries in the
     pools. Storage float32 / float16 / bfloat16, softmax and sums in FP32 (float16: a probability counts to 2^-23 of itself or 2^-44
     of the largest, whichever is more); `out` is float32 by default, as
-    `gqa_attention` returns it, or a given tensor of float32 or of q's dtype. The values in a page behind a sequence's end do
+    `gqa_attention` returns it, or a given tensor of float32 or of q's dtype, which may be q itself but must not overlap q or the
+    pools otherwise. The values in a page behind a sequence's end do
     not matter, NaN included. A row or length outside the tables, or a page number outside the pool, makes
     `check_device_status` raise PageError; a sequence with such a page gets NaN. Nothing is recorded for gradients.
     """
@@ -661,6 +662,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if out.shape != q.shape or out.dtype not in (torch.float32, q.dtype):
             raise ValueError('out must have the shape of q and dtype float32 or that of q')
         out_token, out_head = _heads(out, 'out', written=True)
+        if out.data_ptr() == q.data_ptr() and q.numel() and (out.dtype != q.dtype or (out_token, out_head) != (q_token, q_head)):
+            raise ValueError('out must be q itself or lie elsewhere')
     _on_current_device(q, k_pages, v_pages, tables, lengths, *[x for x in (rows, out) if x is not None])
     if out is None:
         out = torch.empty_like(q, dtype=torch.float32, memory_format=torch.contiguous_format)

@@ -384,7 +384,7 @@ int dtn_paged_append(const dtn_paged_append_args* args /* host */, void* stream)
 /* Attention of one new token per sequence over a paged cache (pools and tables as above):
  * out[i, h] = sum over t of softmax_t(scale * q[i, h] . k[t]) v[t], t over the last `window` (0: all) of the first lengths[r]
  * tokens of sequence r = rows[i] (rows NULL: r = i). Query head h reads kv head h / (q_heads / kv_heads). A negative row or a
- * length of zero gives zeros. out is FP32, or of `storage` when out_f32 is zero. A row >= sequences or a length beyond the tables is
+ * length of zero gives zeros. out is FP32, or of `storage` when out_f32 is zero; it may be q itself, with its strides and type. A row >= sequences or a length beyond the tables is
  * reported by dtn_device_status (the length is cut), and so is a page number outside the pool, which makes the sequence's
  * output NaN; nothing outside the pools is read. What lies in the pools behind a sequence's end is not used, whatever it holds.
  * Softmax and sums are FP32; with f16 storage a probability counts to 2^-23 of itself or 2^-44 of the largest, whichever is more.

@@ -157,3 +157,18 @@ def test_rotary_records_on_streams_and_in_captures(cuda):
     captured.zero_()
     graph.replay()
     assert torch.equal(captured, expected)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('heads', [(8, 2), (16, 1), (3, 3)])
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_attention_in_place_of_its_queries(cuda, dim, heads, dtype):
+    # 20 long sequences are split between blocks, others are empty or short
+    k_pages, v_pages, tables, lens = M.a_cache([9000, 0, 5, 130] + [700] * 20, heads[1], dim, dtype, 16, 'cuda')
+    projected = torch.randn(24, heads[0] + 2, dim, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    v_pages[int(tables[3, 0]), :, 0, 1] = float('inf')                 # a second pass over one of them
+    for q in (projected[:, 1:-1], projected[:, 1:-1].contiguous()):
+        expected = ops.paged_attention(q, k_pages, v_pages, tables, lens, 0.1, out=torch.empty_like(q))
+        for _ in range(5):
+            place = projected.clone()[:, 1:-1] if not q.is_contiguous() else q.clone()
+            assert ops.paged_attention(place, k_pages, v_pages, tables, lens, 0.1, out=place) is place and torch.equal(place, expected)

@@ -128,3 +128,16 @@ def test_copies_of_too_many_planes_are_refused():
     one = 1 << 20
     for planes, pairs in ((2 ** 62, 4), (2 ** 33, 2 ** 30), (2 ** 31, 1), (2, 2 ** 30)):
         assert native.lib().dtn_copy_pages(one, planes, 64, 4, 64, 64, one, one, pairs, None) == native.ERR_UNSUPPORTED, (planes, pairs)
+
+
+def test_attention_refuses_an_out_that_lies_on_q_otherwise():
+    pool, tables, lens = torch.zeros(4, 2, 8, 16), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for dtype in (torch.float16, torch.float32):
+        memory = torch.zeros(3 * 4 * 16, dtype=torch.float32)
+        q = memory.view(dtype)[:3 * 4 * 16].view(3, 4, 16)
+        outs = [q.reshape(4, 3, 16).transpose(0, 1)] + ([memory.view(3, 4, 16)] if dtype == torch.float16 else [])
+        for out in outs:
+            with pytest.raises(ValueError, match='lie elsewhere'):
+                ops.paged_attention(q, pool.to(dtype), pool.to(dtype), tables, lens, 1.0, out=out)
+        with pytest.raises(ValueError, match='CUDA'):
+            ops.paged_attention(q, pool.to(dtype), pool.to(dtype), tables, lens, 1.0, out=q)
