@@ -204,9 +204,10 @@ class PagedCache:
             raise ValueError('a head has a multiple of 16 bytes and at most 256 elements')
         self.book = PageBook(pages, page_size, max_sequences, pages if max_pages_per_sequence is None else max_pages_per_sequence)
         device = torch.device('cuda' if device is None else device)
-        self.pool = torch.empty((layers, 2, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
-        self.tables = torch.full(self.book.tables.shape, PageBook.NO_PAGE, dtype=torch.int32, device=device)
-        self.lengths = torch.zeros(max_sequences, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):   # tensors made under it could not be changed outside it
+            self.pool = torch.empty((layers, 2, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+            self.tables = torch.full(self.book.tables.shape, PageBook.NO_PAGE, dtype=torch.int32, device=device)
+            self.lengths = torch.zeros(max_sequences, dtype=torch.int32, device=device)
         if self.pool.is_cuda:
             with torch.cuda.device(self.pool.device):
                 native.call('dtn_device_status_prepare', torch.cuda.current_stream().cuda_stream)   # the word that reports go to exists before any capture

@@ -141,3 +141,17 @@ def test_attention_refuses_an_out_that_lies_on_q_otherwise():
                 ops.paged_attention(q, pool.to(dtype), pool.to(dtype), tables, lens, 1.0, out=out)
         with pytest.raises(ValueError, match='CUDA'):
             ops.paged_attention(q, pool.to(dtype), pool.to(dtype), tables, lens, 1.0, out=q)
+
+
+@pytest.mark.parametrize('made', [False, True])
+@pytest.mark.parametrize('used', [False, True])
+def test_a_cache_serves_inside_and_outside_inference_mode(made, used):
+    with torch.inference_mode(made):
+        cache = a_cache()
+        row = cache.open()
+    with torch.inference_mode(used):
+        rows, positions = cache.extend([row], [5])
+        fork = cache.fork(row)
+    cache.truncate(fork, 2)
+    assert positions.tolist() == [0, 1, 2, 3, 4] and cache.lengths.tolist() == [5, 2, 0, 0]
+    assert torch.equal(cache.tables, torch.from_numpy(cache.book.tables))
