@@ -21,8 +21,9 @@ static inline int paged_storage_bytes(int64_t storage) { return storage == DTN_S
 
 #ifdef __CUDACC__
 
+// The first report stands until it is read: a wait that ran out before is not covered by a bad page that may follow from it.
 __device__ __forceinline__ void paged_report(int* status, int code) {
-  if (status != nullptr) atomicExch(status, code | (int)(blockIdx.x & 0xff));
+  if (status != nullptr) atomicCAS(status, 0, code | (int)(blockIdx.x & 0xff));
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }

@@ -172,3 +172,20 @@ def test_attention_in_place_of_its_queries(cuda, dim, heads, dtype):
         for _ in range(5):
             place = projected.clone()[:, 1:-1] if not q.is_contiguous() else q.clone()
             assert ops.paged_attention(place, k_pages, v_pages, tables, lens, 0.1, out=place) is place and torch.equal(place, expected)
+
+
+def test_a_bad_page_does_not_cover_a_wait_that_ran_out(cuda):
+    pool = torch.zeros(2, 1, 4, 64, dtype=torch.float16, device='cuda')
+    two = torch.tensor([2], dtype=torch.int32).cuda()
+    tables, lens = torch.tensor([[2]], dtype=torch.int32).cuda(), torch.tensor([3], dtype=torch.int32).cuda()
+    one = torch.zeros(1, 1, 64, dtype=torch.float16, device='cuda')
+    row = torch.zeros(1, dtype=torch.int32, device='cuda')
+    for call in (lambda: ops.copy_pages(pool, two, two), lambda: ops.paged_append(one, one, pool, pool, tables, row, row),
+                 lambda: ops.paged_attention(one, pool, pool, tables, lens, 1.0)):
+        native.call('dtn_selftest_wait_timeout', 1000, torch.cuda.current_stream().cuda_stream)
+        call()
+        with pytest.raises(native.DeviceWaitError, match='self-test'):
+            ops.check_device_status()
+        call()
+        with pytest.raises(native.PageError):
+            ops.check_device_status()
