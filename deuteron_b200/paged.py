@@ -223,7 +223,7 @@ class PagedCache:
         arrays) on the device; everything travels in one copy."""
         width = self.tables.shape[1]
         lists = [np.array([c[0] for c in copies]), np.array([c[1] for c in copies]), np.array([u[0] * width + u[1] for u in updates]),
-                 np.array([u[2] for u in updates]), np.array(rows), self.book.lengths[list(rows)], *tokens]
+                 np.array([u[2] for u in updates]), np.asarray(rows, dtype=np.int32), self.book.lengths[rows], *tokens]
         sizes = [len(part) for part in lists]
         numbers = torch.from_numpy(np.concatenate([np.asarray(part, dtype=np.int32) for part in lists])).to(self.pool.device, non_blocking=True)   # pageable memory is staged before the call returns
         sources, destinations, places, pages, changed, lengths, *tokens = numbers.split(sizes)
@@ -264,9 +264,12 @@ class PagedCache:
         self._outside_captures()
         rows, counts = list(rows), list(counts)
         copies, updates = self.book.extend(rows, counts)
-        rows, counts = np.array(rows, dtype=np.int64), np.array(counts, dtype=np.int64)
+        rows, lengths = np.array(rows, dtype=np.int32), self.book.lengths[rows]
+        if counts.count(1) == len(counts):                # a decode step
+            return self._apply(copies, updates, rows, (rows, lengths - 1))
+        counts = np.array(counts, dtype=np.int64)
         token_rows = np.repeat(rows, counts)
-        positions = np.arange(len(token_rows)) + np.repeat(self.book.lengths[rows] - np.cumsum(counts), counts)   # the last token's is its row's length - 1
+        positions = np.arange(len(token_rows)) + np.repeat(lengths - np.cumsum(counts), counts)   # the last token's is its row's length - 1
         return self._apply(copies, updates, rows, (token_rows, positions))
 
     def truncate(self, row: int, length: int) -> None:
