@@ -40,10 +40,12 @@
 //
 // Measured (kernel in a graph of 30 calls on three sets of inputs in turn, fraction of the 6540 GB/s of a copy):
 //   96 users, 17..8192 tokens, 32 heads on 8, 128, f16, 1.62 GB: 244 us (1.01); 16 users, 1..4096, 137 MB: 30 us (0.69, of
-//   which 3 us are the launch and the clearing of the counters); one user of 131071, bf16, 537 MB: 88.6 us (0.93; 37 blocks
+//   which 3 us are the launch and the clearing of the counters); one user of 131071, bf16, 537 MB: 88.4 us (0.93; 37 blocks
 //   share each head, joining them costs 3 us, the slowest SM is 8 % behind the mean); 9 users, FP32, 16 heads of 64, 124 MB:
-//   29 us (0.65); 37 tokens of one user: 6 us. Head 64, 32 on 8: 0.88; head 80: 0.82; head 256: 0.82; groups of 16: 0.67, of
-//   32: 0.51; 256 users of 128..256 tokens: 0.70.
+//   28.6 us (0.66); 37 tokens of one user: 6 us. 256 users of 128..256 tokens: 0.70. 64 users of 64..8192 tokens, f16: head 64,
+//   32 on 8, 0.90; head 256, 16 on 4, 0.91; head 128 in groups of 16 on 4 0.85, of 32 on 2 0.54, of 40 and 64 on 2 0.33 and 0.32
+//   (the keys are read twice), of 128 on one 0.17. 32 users, FP32, 8 kv heads: head 64 in groups of 1, 4 and 8 0.95, 0.91 and
+//   0.79; head 128 0.95, 0.88 and 0.69, of 16 0.49.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -930,8 +932,11 @@ static int paged_attention_launch_t(PagedAttentionParams& p, cudaStream_t s) {
   p.heads = p.kv_heads * p.blocks;
   p.whole_sets = p.page_size % C::SUB == 0;
   // Two blocks per SM are enough to read, and where few items are shared by many blocks the fewer parts to join count more:
-  // 8 items 88.6 us against 91.4 with three (131071 tokens each) and 32.7 against 33.7 (32768); 16 items equal; 24 items 70.1
-  // against 68.9, 32 items 44.9 against 43.8.
+  // 8 items of head size 128 in 16 bits 88.6 us against 91.4 with three (131071 tokens each) and 32.7 against 33.7 (32768); 24
+  // items 70.1 against 68.9, 32 items 44.9 against 43.8. Other forms, 256 to 65536 tokens: up to 1024 tokens equal; 8 items of
+  // 16384 tokens, in us against three blocks: f16 128 21.5 / 23.3, 64 15.1 / 16.0, groups of 16 32.2 / 35.9, of 32 49.9 / 56.7,
+  // FP32 64 21.5 / 22.3, 128 35.6 / 37.6; of 65536 within 2 % (f16 64 in groups of 16: 41.1 / 39.1). 16 items go either way: f16
+  // 128 14.1 / 14.7 at 4096 tokens and 89.7 / 87.3 at 65536, f16 64 53.2 / 51.4 and FP32 128 in groups of 8 228 / 212 there.
   const int64_t per_sm = C::BLOCKS_PER_SM > 2 && p.count <= 16 && p.count * p.heads <= 16 ? 2 : C::BLOCKS_PER_SM;
   int64_t grid = (int64_t)sm_count() * per_sm;
   if (grid > PA_MAX_BLOCKS) grid = PA_MAX_BLOCKS;

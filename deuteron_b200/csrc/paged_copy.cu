@@ -1,6 +1,6 @@
 // Copies whole pages of a cache inside its pool: forks (the shared last page of a beam) and compaction (live pages moved to
 // low numbers). Bytes read once and written once; bound by memory: 600 pages of 32 KB in 32 planes (1.26 GB) 191 us, the copy
-// rate (205 us with one vector per thread in flight); 8 pages in 64 planes (34 MB) 5.6 us, 0.91 of it.
+// rate (205 us with one vector per thread in flight); 8 pages in 64 planes (34 MB) 5.9 us, 0.87 of it.
 #include "paged.cuh"
 
 namespace dtn {

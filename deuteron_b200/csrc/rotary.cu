@@ -6,7 +6,9 @@
 // with the sine's sign turned.
 //
 // The angle is p * w_i / 2 pi turns in 64 bits, reduced to a fraction of a turn there (at position 10^6 a 32-bit angle would
-// already be off by 0.03 radians) and only then rounded to 32 bits: sincospif of that fraction is off by about 1e-7. One
+// already be off by 0.03 radians) and only then rounded to 32 bits: sincospif of that fraction is off by about 1e-7. That
+// rounding and a 32-bit sine and cosine are a choice: f16 and bf16 results round to 2^-11 and 2^-8 anyway, and FP32 ones are off by
+// 2.8e-8 in the mean where a 64-bit sine and cosine give 2.4e-8 (4095 x 20 x 96); 2^-21 of a pair's magnitudes bounds it. One
 // sine and cosine per token and pair serves every head of the token, so the 64-bit work is a few instructions per 40 or
 // more vectors moved; the kernels are bound by memory (each value is read and written once).
 #include "paged.cuh"
@@ -92,7 +94,8 @@ template <> struct Access<2> { using type = uint16_t; };
 //
 // Bound by memory. V is the widest that divides the head, its strides and addresses and, in the half layout, the number of
 // pairs: 16 bytes in practice. 16384 tokens x 40 heads x 128 bf16 (336 MB): 54 us, 0.95 of the copy rate; 4095 x 20 x 96 FP32
-// interleaved (63 MB): 12 us, 0.80; append of 16000 tokens, 32 + 8 + 8 heads (393 MB): 61.5 us, 0.98; one token: 2 us. (A
+// interleaved (63 MB): 12 us, 0.80; append of 16000 tokens, 32 + 8 + 8 heads (393 MB): 61.5 us, 0.98, and of 8000 in FP32 64 us,
+// 0.94; one token: 2 us. (A
 // form with the angles in shared memory and a unit per thread and head took 61, 15.7 and 112 us: its index arithmetic.)
 template <typename T, bool TWO, int V>
 __global__ void __launch_bounds__(R_THREADS) rotary_kernel(const RotaryParams p, const int interleaved, const int units, const int tokens_per_block,

@@ -448,7 +448,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str | No
     divides every frequency by the factor; 'ntk' raises the base by factor^(rotary_dim / (rotary_dim - 2)), which leaves the
     first pair alone and divides the last by the factor; 'yarn' (Peng et al., 2023) divides those that turn fewer than `slow`
     times within `original_length`, keeps those that turn more than `fast` times, blends in between by the number of
-    turns, and returns the amplitude 0.1 ln(factor) + 1. `device` defaults to the current CUDA device.
+    turns, and returns the amplitude 0.1 ln(factor) + 1. (Some published models blend linearly in the pair's index between the two
+    bounds, or take another amplitude: their middle pairs differ. Any float64 tensor of frequencies can be passed to `rotary`
+    instead.) `device` defaults to the current CUDA device.
     """
     if type(rotary_dim) is not int or rotary_dim < 0 or rotary_dim % 2:
         raise ValueError(f'rotary_dim must be an even non-negative integer, got {rotary_dim!r}')
@@ -718,5 +720,7 @@ def copy_pages(pages: torch.Tensor, sources: torch.Tensor, destinations: torch.T
 
 
 def check_device_status() -> None:
-    """Synchronises the current stream and raises if a kernel reported a wait that ran out."""
+    """Synchronises the current stream and raises if a kernel reported a wait that ran out (DeviceWaitError) or a page number,
+    position, row or length that a paged cache does not cover (PageError); the first report since the last check. An operator of a
+    paged cache that is captured as the first call on a device reports nothing: call it once, or make a PagedCache, before."""
     native.raise_on_device_status(_stream())
