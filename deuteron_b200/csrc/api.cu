@@ -97,7 +97,12 @@ int dtn_device_status(int* status_out, void* stream) {
 int dtn_device_status_prepare(void* stream) {
   if (dtn::device_status_word_unless_capturing(dtn::as_stream(stream)) != nullptr) return DTN_OK;
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  DTN_CUDA_CHECK(cudaStreamIsCapturing(dtn::as_stream(stream), &capturing));
+  const cudaError_t asked = cudaStreamIsCapturing(dtn::as_stream(stream), &capturing);
+  if (asked == cudaErrorStreamCaptureImplicit) {   // the default stream, beside a capture on a stream that waits for it
+    cudaGetLastError();
+    return DTN_OK;
+  }
+  DTN_CUDA_CHECK(asked);
   DTN_REQUIRE(capturing != cudaStreamCaptureStatusNone, DTN_ERR_CUDA, "dtn_device_status_prepare: no status word on this device");
   return DTN_OK;
 }

@@ -1,5 +1,9 @@
 """Calls of the paged operators that must be reported or must not disturb others."""
+import subprocess
+import sys
+import textwrap
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -189,3 +193,46 @@ def test_a_bad_page_does_not_cover_a_wait_that_ran_out(cuda):
         call()
         with pytest.raises(native.PageError):
             ops.check_device_status()
+
+
+def alone(code):
+    """Runs code in a fresh process, where no operator has been called yet."""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, '-c', 'import sys; sys.path.insert(0, sys.argv[1])\n' + textwrap.dedent(code), str(root)], capture_output=True, text=True, timeout=180)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_the_status_word_is_not_made_inside_a_capture(cuda):
+    alone("""
+        import torch
+        from deuteron_b200 import native, ops
+        x = torch.zeros(8, device='cuda')
+        y = x + 1
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = x + 1
+            native.call('dtn_device_status_prepare', torch.cuda.current_stream().cuda_stream)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert y.sum().item() == 8
+        native.call('dtn_device_status_prepare', 0)
+        assert native.device_status() == 0
+    """)
+
+
+def test_the_status_word_beside_a_capture_that_blocks_the_default_stream(cuda):
+    # the default stream cannot be asked then: the word is not made, the capture goes on
+    alone("""
+        import torch
+        from cuda.bindings import runtime
+        from deuteron_b200 import native
+        torch.zeros(1, device='cuda')
+        error, stream = runtime.cudaStreamCreate()
+        assert int(error) == 0
+        native.call('dtn_capture_begin', int(stream))
+        native.call('dtn_device_status_prepare', 0)
+        error, graph = runtime.cudaStreamEndCapture(stream)
+        assert int(error) == 0, error
+        native.call('dtn_device_status_prepare', 0)
+        assert native.device_status() == 0
+    """)
