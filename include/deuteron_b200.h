@@ -361,7 +361,8 @@ int dtn_rotary(const dtn_rotary_args* args /* host */, void* stream);
  * a negative row stores nothing (padding). k and v are [tokens, kv_heads, dim]; q (q_heads of them, 0 for none) is rotated by
  * the same positions into q_out, which may be q itself. A row >= sequences, a position outside the tables or a page number
  * outside the pool stores nothing and is reported by dtn_device_status (not where the first call on a device is being captured:
- * the status word is allocated outside captures). Two tokens for one place: either may stay. */
+ * the status word is allocated outside captures). No two tokens of a call may have one place: parts of each could stay. Positions are
+ * held to the tables, not to a length. */
 typedef struct {
   const void *k, *v;
   void *k_pages, *v_pages;

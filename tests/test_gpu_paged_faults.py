@@ -236,3 +236,31 @@ def test_the_status_word_beside_a_capture_that_blocks_the_default_stream(cuda):
         native.call('dtn_device_status_prepare', 0)
         assert native.device_status() == 0
     """)
+
+
+@pytest.mark.parametrize('layout', ['half', 'interleaved'])
+@pytest.mark.parametrize('pairs', [32, 13])
+def test_strides_beyond_32_bits(cuda, pairs, layout):
+    # tokens, then heads, 2^31 elements and more apart
+    stride = 2 ** 31 + 2 ** 10
+    buffer = torch.empty(2 * stride + 6 * 64, dtype=torch.float16, device='cuda')
+    w, _ = ops.rotary_frequencies(2 * pairs)
+    positions = torch.tensor([5, 100, 7000]).cuda()
+    x = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(6)).half().cuda()
+    expected = ops.rotary(x, positions, w, layout=layout)
+    for strides in ((stride, 64, 1), (64, stride, 1)):
+        view = buffer.as_strided((3, 2, 64), strides)
+        view.copy_(x)
+        assert torch.equal(ops.rotary(view, positions, w, layout=layout), expected)
+        assert ops.rotary(view, positions, w, layout=layout, out=view) is view and torch.equal(view, expected)
+    tables, rows = torch.tensor([[1, 0]], dtype=torch.int32).cuda(), torch.zeros(3, dtype=torch.int32, device='cuda')
+    k_pages, v_pages = torch.zeros(2, 2, 2, 4, 64, dtype=torch.float16, device='cuda')
+    positions = torch.arange(3, device='cuda')
+    view.copy_(x)
+    result = ops.paged_append(view, view, k_pages, v_pages, tables, rows, positions, frequencies=w, layout=layout, q=view)
+    assert torch.equal(result, ops.rotary(x, positions, w, layout=layout))
+    assert torch.equal(k_pages[1, :, :3].transpose(0, 1), result) and torch.equal(v_pages[1, :, :3].transpose(0, 1), x)
+    lens, step = torch.tensor([3], dtype=torch.int32).cuda(), view[:1]
+    step.copy_(result[2:])
+    plain = ops.paged_attention(result[2:], k_pages, v_pages, tables, lens, 0.125, out=torch.empty_like(result[2:]))
+    assert torch.equal(ops.paged_attention(step, k_pages, v_pages, tables, lens, 0.125, out=step), plain)
