@@ -23,11 +23,11 @@
 //   product starts from zero and is added to the FP32 numerator apart: the tensor core's own accumulator truncates. Three
 //   bf16 terms leave 2^-24 of a probability. f16 has too few exponents for that: 2^-24 is its smallest step. So its
 //   probabilities are 2^BIAS times larger (the factor is in the sums as well and cancels), which puts the largest at 2^15, and
-//   the second of two terms is 2^REST times what the first leaves, with a product of its own that is scaled back when it is
-//   added. That leaves 2^-23 of a probability, or 2^-44 of 1 where that is more: 2^-44 is 2^-(25 + BIAS + REST), half a step
-//   of the second term; 1 is a token whose score is the maximum that the block keeps. (Two terms of one scale left 2^-25 of 1: 48
-//   tokens, one of them with a zero value and all but 1e-6 of the mass, were off by 1e-3, now by 5e-7. Neither form is
-//   slower than the other anywhere: the 96 users 247.3 and 247.3 us, groups of 16 98.9 and 98.9, head size 80 69.8 and 70.1.)
+//   the second of two terms is REST = 2^12 times what the first leaves, with a product of its own that is scaled back when it
+//   is added. That leaves 2^-23 of a probability, or 2^-44 of 1 where that is more: half a step of the second term, 2^-25, over
+//   2^BIAS and REST; 1 is a token whose score is the maximum that the warp keeps. (Two terms of one scale left 2^-25 of 1: 48
+//   tokens, one of them with a zero value and all but 4e-5 of the mass, were off by 1e-3, now by 5e-7. Neither form is
+//   slower than the other: the 96 users 246.9 and 246.9 us, groups of 16 99.6 and 100.0, head size 80 70.0 and 70.4.)
 //   Products, FP32 storage. Plain fused multiply-adds: four lanes share a token's score, a lane owns dim / 32 columns of V.
 //   More than 8 query heads per kv head: HB = 2 or 4 warps share a team's stage, each with its 8 heads; beyond 32 the
 //   heads are split into blocks that read the keys again. From 16 heads on the products and the instructions around them, not the bytes, set
